@@ -123,6 +123,10 @@ SIGNATURES = {
                           _vp]),
     "ait_attn_bwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _ull, _vp, _i,
                           _vp, _i, _vp, _i, _vp]),
+    "ait_packed_attn_fwd_workspace_bytes": (_sz, [_vp]),
+    "ait_packed_attn_fwd": (_i, [_vp] + [_vp, _ll, _ll] * 4 + [_vp, _vp, _sz, _vp]),
+    "ait_packed_attn_bwd_workspace_bytes": (_sz, [_vp]),
+    "ait_packed_attn_bwd": (_i, [_vp] + [_vp, _ll, _ll] * 5 + [_vp] + [_vp, _ll, _ll] * 3 + [_vp, _vp, _sz, _vp]),
 }
 
 GEMM_RELU, GEMM_ACCUMULATE, GEMM_ATOMIC, GEMM_BIAS_ROW, GEMM_MASK_POS, GEMM_COLSUM = 1, 2, 4, 8, 16, 32
@@ -213,6 +217,16 @@ class TransformerGrads(ctypes.Structure):
         [("enc_slf", MhaGrads), ("dec_slf", MhaGrads), ("dec_enc", MhaGrads),
          ("enc_ffn", FfnGrads), ("dec_ffn", FfnGrads)]
 
+
+class PackedAttn(ctypes.Structure):
+    """ait_packed_attn."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("cu_q", "cu_k", "k_len", "bias_table", "bucket_of")] + \
+        [(n, ctypes.c_int) for n in ("n_seq", "total_q", "total_k", "max_q", "max_k", "heads", "kv_heads", "d", "dtype", "causal",
+                                     "n_buckets", "max_distance", "zero_rest")] + [("scale", ctypes.c_float)]
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1}      # AIT_DTYPE_*
+MAX_BUCKETS, MAX_BIAS_DISTANCE = 512, 2048          # AIT_MAX_*
 
 PROBE_GEMM, PROBE_ROI_FWD, PROBE_ROI_BWD = 1, 2, 3
 

@@ -1,0 +1,342 @@
+// ait_amd/csrc/packed_attn.hip -- ait_packed_attn_fwd: attention over packed sequences, forward (layout of the products:
+// packed_attn_impl.h).
+//
+//   s_ij = scale q_i . k_j + bias[bucket(j - i - (len_k - len_q))],   o_i = sum_j softmax_j(s_ij) v_j
+//
+// One pass over the keys with the running maximum and sum (kept in units of log2, f32).  A wave has 32 query rows as the columns
+// of its score blocks, a workgroup NW waves that share every K / V tile; tiles are double-buffered, the next one's 16-byte loads
+// go straight into shared memory while this one is multiplied, one barrier a tile.  The rows of a workgroup are (position,
+// head) pairs of one key head: `pack` heads to a position, so that a single new token still fills the block's columns with the
+// heads that share its keys.
+#include "packed_attn_impl.h"
+
+namespace {
+using namespace ait_packed;
+
+struct FwdArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  long long qs, qh, ks, kh, vs, vh, os, oh;      // row and head strides in elements
+  Seqs s;
+  Bias bias;
+  int H, Hk, d, causal, pack, splits, numbers;
+  float scale;
+  float* part_o;      // [splits][total_q * H][d] unnormalised, and
+  float* part_ml;     // [splits][total_q * H][2] maximum, sum: only where splits > 1
+};
+
+template <typename T, int D, int NW, bool BIAS, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(const FwdArgs a) {
+  constexpr int NT = NW * 64, BM = NW * 32, NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int units = a.H / a.pack, unit = blockIdx.x % units, group = a.H / a.Hk;
+  // key heads run fastest (workgroups 8 apart share an L2: they read the same key head where there are 8, 4, 2 or 1 of them),
+  // a sequence's last rows first (with a causal mask they have the most to do)
+  const int kvh = unit % a.Hk, head0 = kvh * group + (unit / a.Hk) * a.pack;
+  int seq, block, qstart, qlen, kstart, klen;
+  if (!find_block(a.s.cu_q, a.s.n_seq, a.s.rest, a.s.total_q, a.pack, BM, a.numbers - 1 - (int)(blockIdx.x / units), seq, block, qstart, qlen))
+    return;
+  if (seq == a.s.n_seq) {          // rows of no sequence
+    if constexpr (!SPLIT) {
+      const int r = block * BM + wave * 32 + (lane & 31), n = r / a.pack;
+      if (n < qlen)
+        for (int e = 8 * h; e < a.d; e += 16) {
+          T* p = reinterpret_cast<T*>(a.o) + (long long)(qstart + n) * a.os + (long long)(head0 + r - n * a.pack) * a.oh + e;
+          store4(p, 0.f, 0.f, 0.f, 0.f);
+          store4(p + 4, 0.f, 0.f, 0.f, 0.f);
+        }
+      if (n < qlen && h == 0 && a.lse) a.lse[(long long)(head0 + r - n * a.pack) * a.s.total_q + qstart + n] = kNegInf;
+    }
+    return;
+  }
+  keys_of(a.s, seq, kstart, klen);
+  const int rows = qlen * a.pack, off = klen - qlen;
+  const int row0 = block * BM + wave * 32, row = row0 + (lane & 31);
+  const int rowc = row < rows ? row : rows - 1, pos = rowc / a.pack, head = head0 + rowc - pos * a.pack;
+  const int kmax = a.causal ? min(klen, pos + off + 1) : klen;                           // this lane's query sees keys below it
+  const int wfirst = min(row0, rows - 1) / a.pack, wlast = min(row0 + 31, rows - 1) / a.pack;
+  const int wsure = a.causal ? min(klen, wfirst + off + 1) : klen, wend = row0 < rows ? (a.causal ? min(klen, wlast + off + 1) : klen) : 0;
+  const int gend = a.causal ? min(klen, (min(block * BM + BM, rows) - 1) / a.pack + off + 1) : klen;
+  int t0 = 0, t1 = gend > 0 ? (gend + KB - 1) / KB : 0;
+  if constexpr (SPLIT) {
+    const int per = (t1 + a.splits - 1) / a.splits;
+    t0 = blockIdx.y * per;
+    t1 = min(t1, t0 + per);
+  }
+
+  Frag<T> qf[NCH];
+  {
+    const T* qr = reinterpret_cast<const T*>(a.q) + (long long)(qstart + pos) * a.qs + (long long)head * a.qh;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < rows);
+  }
+  const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
+  Loader<T, D, NT> lk, lv;
+  lk.init(tid, kstr, dby);
+  lv.init(tid, vstr, dby);
+  const T* kb = reinterpret_cast<const T*>(a.k) + (long long)kstart * a.ks + (long long)kvh * a.kh;
+  const T* vb = reinterpret_cast<const T*>(a.v) + (long long)kstart * a.vs + (long long)kvh * a.vh;
+  const unsigned lds0 = lds_addr(lds);
+  auto fetch = [&](int t, int stage) {
+    const long long r = (long long)t * KB;
+    lk.load(kb + r * a.ks, klen - r, kstr, dby, lds0 + stage * 2 * kTile, wave);
+    lv.load(vb + r * a.vs, klen - r, vstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
+  };
+  const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile);
+  float far_lo = 0.f, far_hi = 0.f;
+  if (t0 < t1) fetch(t0, 0);
+  if constexpr (BIAS) {
+    fill_bias<NT>(a.bias, a.H, head0, a.pack, const_cast<float*>(bl), tid);
+    __syncthreads();
+    bl += (head - head0) * bias_row(a.bias.max_distance);
+    far_lo = bl[0];
+    far_hi = bl[2 * (a.bias.max_distance + kPad)];
+  }
+
+  const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[b][r] = 0.f;
+  float m = kNegInf, l = 0.f;
+
+  for (int t = t0; t < t1; t++) {
+    const int stage = (t - t0) & 1, k0 = t * KB;
+    loads_done_barrier();
+    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+    if (k0 >= wend) continue;
+    const unsigned char* kt = lds + stage * 2 * kTile;
+    const unsigned char* vt = kt + kTile;
+    f32x16 s[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[x][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);
+    }
+    if constexpr (BIAS) {
+      const int md = a.bias.max_distance;
+      if (k0 + KB - 1 - (wfirst + off) <= -md || k0 - (wlast + off) >= md) {
+        const float f = k0 - (wlast + off) >= md ? far_hi : far_lo;
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[x][r] = __builtin_fmaf(s[x][r], sc, f);
+      } else {
+        const float* p = bl + (k0 + 4 * h - (pos + off) + md + kPad);
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[x][r] = __builtin_fmaf(s[x][r], sc, p[32 * x + 8 * (r >> 2) + (r & 3)]);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[x][r] *= sc;
+    }
+    if (k0 + KB > wsure) {
+      const int lim = kmax - k0 - 4 * h;
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[x][r] = 32 * x + 8 * (r >> 2) + (r & 3) < lim ? s[x][r] : kNegInf;
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+    top = column_max(top);
+    const float mn = fmaxf(m, top), mu = mn == kNegInf ? 0.f : mn;
+    const float alpha = fast_exp2(m - mu);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[x][r] = fast_exp2(s[x][r] - mu);
+        sum += s[x][r];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[b][r] *= alpha;
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int cc = 0; cc < 2; cc++) {
+        const Frag<T> pf = acc_frag<T>(s[x], cc);
+#pragma unroll
+        for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
+      }
+  }
+
+  if (row >= rows) return;
+  l = column_sum(l);
+  const long long at = (long long)(qstart + pos);
+  if constexpr (SPLIT) {
+    const long long id = (long long)blockIdx.y * a.s.total_q * a.H + at * a.H + head;
+    if (h == 0) {
+      a.part_ml[2 * id] = m;
+      a.part_ml[2 * id + 1] = l;
+    }
+    float* p = a.part_o + id * a.d;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int dd = 32 * b + 8 * i + 4 * h;
+        if (dd < a.d) store4(p + dd, acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]);
+      }
+  } else {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);        // (a row that sees nothing: zeros; NaN stays NaN)
+    if (a.lse && h == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    T* p = reinterpret_cast<T*>(a.o) + at * a.os + (long long)head * a.oh;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int dd = 32 * b + 8 * i + 4 * h;
+        if (dd < a.d) store4(p + dd, acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv);
+      }
+  }
+}
+
+// the splits of a row joined, in their order: one wave per (query row, head)
+template <typename T>
+__global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long long n = (long long)a.s.total_q * a.H, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= n) return;
+  const int at = (int)(id / a.H);
+  const bool in = at >= clamped(a.s.cu_q, 0, a.s.total_q) && at < clamped(a.s.cu_q, a.s.n_seq, a.s.total_q);
+  if (!in && !a.s.rest) return;                          // no sequence's row: left as it is, or set to zero
+  const int head = (int)(id - (long long)at * a.H), dd = lane * 4, splits = in ? a.splits : 0;
+  float m = kNegInf;
+  for (int s = 0; s < splits; s++) m = fmaxf(m, a.part_ml[2 * (s * n + id)]);
+  const float mu = m == kNegInf ? 0.f : m;
+  float l = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+  for (int s = 0; s < splits; s++) {
+    const float w = fast_exp2(a.part_ml[2 * (s * n + id)] - mu), ls = a.part_ml[2 * (s * n + id) + 1];
+    l += w * ls;
+    if (dd < a.d) {
+      const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (s * n + id) * a.d + dd);
+      o0 += w * p[0]; o1 += w * p[1]; o2 += w * p[2]; o3 += w * p[3];
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (a.lse && lane == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (dd < a.d) store4(reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+}
+
+template <typename T, int D, int NW, bool BIAS, bool SPLIT>
+int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
+  const int bytes = 4 * Tile<T, D>::kBytes + bias_bytes;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          bytes) != hipSuccess)
+    return AIT_ELAUNCH;
+  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), dim3((unsigned)(a.numbers * (a.H / a.pack)), (unsigned)a.splits), dim3(NW * 64),
+                     bytes, st, a);
+  AIT_CHECK_LAUNCH();
+  if constexpr (SPLIT) {
+    hipLaunchKernelGGL((packed_join_kernel<T>), dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  return AIT_OK;
+}
+template <typename T, int D, int NW>
+int launch_nw(const FwdArgs& a, int bias_bytes, hipStream_t st) {
+  if (a.bias.table) return a.splits > 1 ? launch<T, D, NW, true, true>(a, bias_bytes, st) : launch<T, D, NW, true, false>(a, bias_bytes, st);
+  return a.splits > 1 ? launch<T, D, NW, false, true>(a, 0, st) : launch<T, D, NW, false, false>(a, 0, st);
+}
+template <typename T>
+int launch_t(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
+  if (a.d <= 64) return nw == 1 ? launch_nw<T, 64, 1>(a, bias_bytes, st) : launch_nw<T, 64, 4>(a, bias_bytes, st);
+  return nw == 1 ? launch_nw<T, 128, 1>(a, bias_bytes, st) : launch_nw<T, 128, 4>(a, bias_bytes, st);
+}
+
+// what the sizes decide: heads packed to a position, waves of a workgroup, parts of the key axis
+struct Shape { int pack, nw, splits; };
+Shape shape_of(const ait_packed_attn& p) {
+  Shape r;
+  const int group = p.heads / p.kv_heads;
+  const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
+  // a few new tokens: the heads of a key head fill the 32 columns of one wave
+  const bool few = max_q * group <= 32;
+  r.pack = few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
+  r.nw = max_q * r.pack <= 32 ? 1 : 4;
+  const long long wgs = block_numbers(p.total_q, r.pack, r.nw * 32, p.n_seq, 1) * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
+  long long s = r.nw == 1 ? (1024 + wgs - 1) / wgs : 1;
+  if (s > tiles / 2) s = tiles / 2;
+  if (s > 64) s = 64;
+  r.splits = s < 1 ? 1 : (int)s;
+  return r;
+}
+size_t workspace(const ait_packed_attn& p, const Shape& s) {
+  return s.splits > 1 ? (size_t)s.splits * p.total_q * p.heads * (p.d + 2) * sizeof(float) : 0;
+}
+}  // namespace
+
+namespace ait_packed {
+int check(const ait_packed_attn* p) {
+  if (!p || p->n_seq < 0 || p->total_q < 0 || p->total_k < 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads || p->d <= 0)
+    return AIT_EINVAL;
+  if (p->dtype != AIT_DTYPE_F32 && p->dtype != AIT_DTYPE_BF16) return AIT_EINVAL;
+  if (p->max_q < 0 || p->max_k < 0 || !(p->scale == p->scale)) return AIT_EINVAL;
+  if (p->d > 128 || p->d % 8) return AIT_EUNSUPPORTED;
+  if (p->bias_table) {
+    if (!p->bucket_of || p->n_buckets <= 0 || p->max_distance < 0) return AIT_EINVAL;
+    if (p->n_buckets > AIT_MAX_BUCKETS || p->max_distance > AIT_MAX_BIAS_DISTANCE) return AIT_EUNSUPPORTED;
+  }
+  if ((p->n_seq > 0 && p->total_q > 0) && (!p->cu_q || !p->cu_k)) return AIT_EINVAL;
+  // 32-bit counters: block numbers times heads, and rows times heads
+  if ((long long)p->total_q * p->heads + (long long)(p->n_seq + 1LL) * p->heads >= (1LL << 31)) return AIT_EUNSUPPORTED;
+  if ((long long)p->total_k * p->heads + (long long)(p->n_seq + 1LL) * p->heads >= (1LL << 40)) return AIT_EUNSUPPORTED;
+  return AIT_OK;
+}
+int check_strides(const ait_packed_attn* p, const void* base, long long row, long long head, long long rows) {
+  const int es = p->dtype == AIT_DTYPE_F32 ? 4 : 2;
+  if (rows > 0 && !base) return AIT_EINVAL;
+  if ((unsigned long long)base % 16 || (row * es) % 16 || (head * es) % 16 || row < 0 || head < 0) return AIT_EUNSUPPORTED;
+  if (row * es * KB >= (1LL << 31)) return AIT_EUNSUPPORTED;      // a tile's 32-bit offsets
+  return AIT_OK;
+}
+}  // namespace ait_packed
+
+AIT_API size_t ait_packed_attn_fwd_workspace_bytes(const ait_packed_attn* p) {
+  if (ait_packed::check(p) != AIT_OK) return 0;
+  return workspace(*p, shape_of(*p));
+}
+
+AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                long long k_head, const void* v, long long v_row, long long v_head, void* o, long long o_row,
+                                long long o_head, float* lse, void* workspace_ptr, size_t workspace_bytes, void* stream) {
+  AIT_TRY_RC(ait_packed::check(p));
+  if (p->n_seq == 0 || p->total_q == 0) return AIT_OK;
+  AIT_TRY_RC(ait_packed::check_strides(p, q, q_row, q_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, o, o_row, o_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, k, k_row, k_head, p->total_k));
+  AIT_TRY_RC(ait_packed::check_strides(p, v, v_row, v_head, p->total_k));
+  const Shape sh = shape_of(*p);
+  const size_t need = workspace(*p, sh);
+  if (need && (!workspace_ptr || workspace_bytes < need)) return AIT_EWORKSPACE;
+  FwdArgs a{q, k, v, o, lse, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
+            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
+            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
+            p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
+            (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), p->scale, nullptr, nullptr};
+  if (need) {
+    a.part_o = static_cast<float*>(workspace_ptr);
+    a.part_ml = a.part_o + (size_t)sh.splits * p->total_q * p->heads * p->d;
+  }
+  const int bias_bytes = p->bias_table ? sh.pack * bias_row(p->max_distance) * 4 : 0;
+  return p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, sh.nw, bias_bytes, ait_stream(stream)) : launch_t<__bf16>(a, sh.nw, bias_bytes, ait_stream(stream));
+}

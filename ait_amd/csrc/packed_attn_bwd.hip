@@ -1,0 +1,485 @@
+// ait_amd/csrc/packed_attn_bwd.hip -- ait_packed_attn_bwd (layout of the products: packed_attn_impl.h).
+//
+//   P_ij = exp(s_ij - lse_i),  dP_ij = dO_i . v_j,  dS_ij = P_ij (dP_ij - delta_i),  delta_i = dO_i . O_i
+//   dQ_i = scale sum_j dS_ij k_j,   dK_j = scale sum_i dS_ij q_i,   dV_j = sum_i P_ij dO_i,   d table[bucket] = sum dS_ij
+//
+// Two passes that each own what they write, so no sum goes through atomics on memory and results repeat bit for bit: the first
+// has a block of query rows per workgroup and runs over the keys (three products; it also forms delta and the bias's
+// gradient), the second a block of keys and runs over the query rows of every head that shares them (four products).  The two
+// score products are computed in both: 14 instead of 10 multiplications per pair and value, against f32 sums of dQ through
+// memory.
+#include "packed_attn_impl.h"
+
+namespace {
+using namespace ait_packed;
+
+constexpr int NW = 4, NT = NW * 64, BM = NW * 32;
+constexpr int kHist = 96;       // relative positions that a 64 x 32 block spans
+
+struct BwdArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* d_o;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  long long qs, qh, ks, kh, vs, vh, os, oh, dos, doh, dqs, dqh, dks, dkh, dvs, dvh;
+  Seqs s;
+  Bias bias;
+  int H, Hk, d, causal, qnumbers, knumbers;
+  float scale;
+  float* lse2;        // [H][total_q] log2 of the rows' sums (+infinity where a row sees nothing: its probabilities are zero)
+  float* delta;       // [H][total_q]
+  float* part_table;  // [qnumbers][H][n_buckets]; null: the table's gradient is not wanted
+  float* d_table;
+};
+
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const BwdArgs a) {
+  constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int unit = blockIdx.x % a.H, group = a.H / a.Hk, kvh = unit % a.Hk, head = kvh * group + unit / a.Hk;
+  const int number = a.qnumbers - 1 - (int)(blockIdx.x / a.H), nb = a.bias.n_buckets, md = a.bias.max_distance;
+  float* part = BIAS && a.part_table ? a.part_table + ((size_t)number * a.H + head) * nb : nullptr;
+  int seq, block, qstart, qlen, kstart, klen;
+  const bool has = find_block(a.s.cu_q, a.s.n_seq, a.s.rest, a.s.total_q, 1, BM, number, seq, block, qstart, qlen);
+  if (!has || seq == a.s.n_seq) {
+    if constexpr (BIAS)
+      if (part)
+        for (int b = tid; b < nb; b += NT) part[b] = 0.f;
+    if (!has) return;
+    const int r = block * BM + wave * 32 + (lane & 31);
+    if (r < qlen)
+      for (int e = 8 * h; e < a.d; e += 16) {
+        T* p = reinterpret_cast<T*>(a.dq) + (long long)(qstart + r) * a.dqs + (long long)head * a.dqh + e;
+        store4(p, 0.f, 0.f, 0.f, 0.f);
+        store4(p + 4, 0.f, 0.f, 0.f, 0.f);
+      }
+    return;
+  }
+  keys_of(a.s, seq, kstart, klen);
+  const int off = klen - qlen, row0 = block * BM + wave * 32, row = row0 + (lane & 31), pos = min(row, qlen - 1);
+  const int kmax = a.causal ? min(klen, pos + off + 1) : klen;
+  const int wfirst = min(row0, qlen - 1), wlast = min(row0 + 31, qlen - 1);
+  const int wsure = a.causal ? min(klen, wfirst + off + 1) : klen, wend = row0 < qlen ? (a.causal ? min(klen, wlast + off + 1) : klen) : 0;
+  const int gend = a.causal ? min(klen, min(block * BM + BM, qlen) + off) : klen;
+  const int t1 = gend > 0 ? (gend + KB - 1) / KB : 0;
+
+  const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
+  Loader<T, D, NT> lk, lv;
+  lk.init(tid, kstr, dby);
+  lv.init(tid, vstr, dby);
+  const T* kb = reinterpret_cast<const T*>(a.k) + (long long)kstart * a.ks + (long long)kvh * a.kh;
+  const T* vb = reinterpret_cast<const T*>(a.v) + (long long)kstart * a.vs + (long long)kvh * a.vh;
+  const unsigned lds0 = lds_addr(lds);
+  auto fetch = [&](int t, int stage) {
+    const long long r = (long long)t * KB;
+    lk.load(kb + r * a.ks, klen - r, kstr, dby, lds0 + stage * 2 * kTile, wave);
+    lv.load(vb + r * a.vs, klen - r, vstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
+  };
+  if (t1 > 0) fetch(0, 0);
+
+  Frag<T> qf[NCH], gf[NCH];
+  float delta = 0.f, l2;
+  {
+    const long long at = qstart + pos;
+    const T* qr = reinterpret_cast<const T*>(a.q) + at * a.qs + (long long)head * a.qh;
+    const T* gr = reinterpret_cast<const T*>(a.d_o) + at * a.dos + (long long)head * a.doh;
+    const T* orow = reinterpret_cast<const T*>(a.o) + at * a.os + (long long)head * a.oh;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) {
+      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < qlen);
+      gf[c] = global_frag<T>(gr, 16 * c + 8 * h, a.d, row < qlen);
+      const Frag<T> of = global_frag<T>(orow, 16 * c + 8 * h, a.d, row < qlen);
+#pragma unroll
+      for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)of[e], delta);
+    }
+    delta = column_sum(delta);
+    const float l = a.lse[(long long)head * a.s.total_q + at];
+    l2 = l == kNegInf ? -kNegInf : l * kLog2e;
+    if (row < qlen && h == 0) {
+      a.lse2[(long long)head * a.s.total_q + at] = l2;
+      a.delta[(long long)head * a.s.total_q + at] = delta;
+    }
+    if (row >= qlen || l == kNegInf) { l2 = -kNegInf; delta = 0.f; }
+  }
+  float* bl = reinterpret_cast<float*>(lds + 4 * kTile);                 // the head's bias, then per wave: a block's sums by
+  float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kHist + nb);    // relative position, and the sums by bucket
+  float* acc_b = hist + kHist;
+  float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
+  if constexpr (BIAS) {
+    fill_bias<NT>(a.bias, a.H, head, 1, bl, tid);
+    if (part) {
+      for (int x = lane; x < kHist + nb; x += 64) hist[x] = 0.f;
+    }
+    __syncthreads();
+    far_lo = bl[0];
+    far_hi = bl[2 * (md + kPad)];
+  }
+
+  const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[b][r] = 0.f;
+
+  for (int t = 0; t < t1; t++) {
+    const int stage = t & 1, k0 = t * KB;
+    loads_done_barrier();
+    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+    if (k0 >= wend) continue;
+    const unsigned char* kt = lds + stage * 2 * kTile;
+    const unsigned char* vt = kt + kTile;
+    bool near = false, right = false;
+    if constexpr (BIAS) {
+      right = k0 - (wlast + off) >= md;
+      near = !right && k0 + KB - 1 - (wfirst + off) > -md;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) s = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s);
+#pragma unroll
+      for (int c = 0; c < NCH; c++) dp = mma(row_frag<T, D>(vt, rb, x, c), gf[c], dp);
+      if (BIAS && near) {
+        const float* p = bl + (k0 + 32 * x + 4 * h - (pos + off) + md + kPad);
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], sc, p[8 * (r >> 2) + (r & 3)] - l2);
+      } else {
+        const float f = (BIAS ? (right ? far_hi : far_lo) : 0.f) - l2;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], sc, f);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = fast_exp2(s[r]) * (dp[r] - delta);
+      if (k0 + KB > wsure) {
+        const int lim = kmax - k0 - 32 * x - 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 8 * (r >> 2) + (r & 3) < lim ? s[r] : 0.f;
+      }
+      if constexpr (BIAS) {
+        if (part) {
+          if (near) {
+            // key - query over the block, the block's last column (31) at its first key being 0
+            float* p = hist + 32 * x + 4 * h + 31 - (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; r++) __hip_atomic_fetch_add(p + 8 * (r >> 2) + (r & 3), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          } else {
+            float u = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) u += s[r];
+            sum_lo += right ? 0.f : u;
+            sum_hi += right ? u : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int cc = 0; cc < 2; cc++) {
+        const Frag<T> df = acc_frag<T>(s, cc);
+#pragma unroll
+        for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(kt, cb, x, cc, b), df, acc[b]);
+      }
+    }
+    if constexpr (BIAS) {
+      if (part && near) {      // this wave's own memory, in order: no barrier
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const int i = lane + 64 * x;
+          if (i < kHist) {
+            const float u = hist[i];
+            hist[i] = 0.f;
+            __hip_atomic_fetch_add(acc_b + bucket(a.bias, k0 - (row0 + 31 + off) + i), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    }
+  }
+
+  if (row < qlen) {
+    T* p = reinterpret_cast<T*>(a.dq) + (long long)(qstart + pos) * a.dqs + (long long)head * a.dqh;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int dd = 32 * b + 8 * i + 4 * h;
+        if (dd < a.d)
+          store4(p + dd, acc[b][4 * i] * a.scale, acc[b][4 * i + 1] * a.scale, acc[b][4 * i + 2] * a.scale, acc[b][4 * i + 3] * a.scale);
+      }
+  }
+  if constexpr (BIAS) {
+    if (part) {
+      sum_lo = wave_sum(sum_lo);
+      sum_hi = wave_sum(sum_hi);
+      if (lane == 0) {
+        acc_b[bucket(a.bias, -md)] += sum_lo;
+        acc_b[bucket(a.bias, md)] += sum_hi;
+      }
+      __syncthreads();
+      const float* w0 = bl + bias_row(md) + kHist;
+      for (int b = tid; b < nb; b += NT) {
+        float u = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) u += w0[w * (kHist + nb) + b];
+        part[b] = u;
+      }
+    }
+  }
+}
+
+// d table[b][head]: the workgroups' parts in a fixed order
+__global__ __launch_bounds__(256) void packed_table_kernel(const BwdArgs a) {
+  __shared__ float sums[256];
+  const int head = blockIdx.x, b = blockIdx.y * 16 + (threadIdx.x & 15), nb = a.bias.n_buckets;
+  float u = 0.f;
+  if (b < nb)
+    for (int n = threadIdx.x >> 4; n < a.qnumbers; n += 16) u += a.part_table[((size_t)n * a.H + head) * nb + b];
+  sums[threadIdx.x] = u;
+  __syncthreads();
+  if (threadIdx.x < 16 && b < nb) {
+    u = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) u += sums[threadIdx.x + 16 * i];
+    a.d_table[(size_t)b * a.H + head] = u;
+  }
+}
+
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(const BwdArgs a) {
+  constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int kvh = blockIdx.x % a.Hk, group = a.H / a.Hk, number = (int)(blockIdx.x / a.Hk), md = a.bias.max_distance;
+  int seq, block, kstart, kroom, klen;
+  // key blocks are numbered by the rows the sequences OCCUPY: keys behind k_len get zeros
+  if (!find_block(a.s.cu_k, a.s.n_seq, a.s.rest, a.s.total_k, 1, BM, number, seq, block, kstart, kroom)) return;
+  const int key0 = block * BM + wave * 32, key = key0 + (lane & 31);
+  int qstart = 0, qlen = 0;
+  klen = 0;
+  if (seq < a.s.n_seq) {
+    int ks;
+    keys_of(a.s, seq, ks, klen);
+    qstart = clamped(a.s.cu_q, seq, a.s.total_q);
+    qlen = max(0, clamped(a.s.cu_q, seq + 1, a.s.total_q) - qstart);
+  }
+  const int off = klen - qlen;
+  // query rows that see a key j: positions >= j - off with a causal mask
+  const int gfirst = a.causal ? max(0, block * BM - off) : 0, wfirst = a.causal ? max(0, key0 - off) : 0;
+  const int wsure = a.causal ? max(0, min(key0 + 31, klen - 1) - off) : 0;          // from here on every key of the wave is seen
+  const int t0 = gfirst / KB, tq = block * BM < klen ? max(0, (qlen + KB - 1) / KB - t0) : 0, total = tq * group;
+
+  const unsigned qstr = (unsigned)(a.qs * sizeof(T)), gstr = (unsigned)(a.dos * sizeof(T)), dby = a.d * sizeof(T);
+  Loader<T, D, NT> lq, lg;
+  lq.init(tid, qstr, dby);
+  lg.init(tid, gstr, dby);
+  const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse2 | delta of KB rows
+  auto fetch = [&](int it, int stage) {
+    const int g = it / tq, t = t0 + it - g * tq, head = kvh * group + g;
+    const long long r = (long long)t * KB;
+    lq.load(reinterpret_cast<const T*>(a.q) + (qstart + r) * a.qs + (long long)head * a.qh, qlen - r, qstr, dby, lds0 + stage * 2 * kTile, wave);
+    lg.load(reinterpret_cast<const T*>(a.d_o) + (qstart + r) * a.dos + (long long)head * a.doh, qlen - r, gstr, dby,
+            lds0 + stage * 2 * kTile + kTile, wave);
+    if (wave < 2) {
+      const float* src = (wave ? a.delta : a.lse2) + (long long)head * a.s.total_q + qstart + r;
+      const int n = (int)min((long long)KB, qlen - r);
+      const i32x4 rsrc = tile_rsrc(src, n * 4);
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                   : : "v"(lane * 4), "s"(rsrc), "s"((unsigned)__builtin_amdgcn_readfirstlane((int)(rows0 + stage * 512 + wave * 256))) : "m0", "memory");
+    }
+  };
+  const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile + 1024);
+  if (total > 0) fetch(0, 0);
+
+  Frag<T> kf[NCH], vf[NCH];
+  {
+    const bool there = key < klen;
+    const long long at = kstart + (there ? key : 0);
+    const T* kr = reinterpret_cast<const T*>(a.k) + at * a.ks + (long long)kvh * a.kh;
+    const T* vr = reinterpret_cast<const T*>(a.v) + at * a.vs + (long long)kvh * a.vh;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) {
+      kf[c] = global_frag<T>(kr, 16 * c + 8 * h, a.d, there);
+      vf[c] = global_frag<T>(vr, 16 * c + 8 * h, a.d, there);
+    }
+  }
+  const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16 ak[NB], av[NB];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) ak[b][r] = av[b][r] = 0.f;
+  float far_lo = 0.f, far_hi = 0.f;
+
+  for (int it = 0; it < total; it++) {
+    const int stage = it & 1, g = it / tq, t = t0 + it - g * tq, r0 = t * KB;
+    if constexpr (BIAS) {
+      if (it == g * tq) {      // another head: its bias
+        __syncthreads();
+        fill_bias<NT>(a.bias, a.H, kvh * group + g, 1, const_cast<float*>(bl), tid);
+        __syncthreads();
+        far_lo = bl[0];
+        far_hi = bl[2 * (md + kPad)];
+      }
+    }
+    loads_done_barrier();
+    if (it + 1 < total) fetch(it + 1, stage ^ 1);
+    if (r0 + KB <= wfirst || key0 >= klen) continue;
+    const unsigned char* qt = lds + stage * 2 * kTile;
+    const unsigned char* gt = qt + kTile;
+    const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * 512);
+    const int last = min(r0 + KB, qlen) - 1;
+    bool near = false, right = false;
+    if constexpr (BIAS) {
+      right = key0 - (last + off) >= md;
+      near = !right && key0 + 31 - (r0 + off) > -md;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) s = mma(row_frag<T, D>(qt, rb, x, c), kf[c], s);
+#pragma unroll
+      for (int c = 0; c < NCH; c++) dp = mma(row_frag<T, D>(gt, rb, x, c), vf[c], dp);
+      const float far = BIAS ? (right ? far_hi : far_lo) : 0.f;
+      const float* p = bl + (key - (r0 + 32 * x + 4 * h + off) + md + kPad);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 l2 = *reinterpret_cast<const f32x4*>(rows + 32 * x + 8 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float f = (BIAS && near) ? p[-8 * i - j] : far;
+          s[4 * i + j] = fast_exp2(__builtin_fmaf(s[4 * i + j], sc, f - l2[j]));
+        }
+      }
+      // a row's first positions do not see the wave's last keys; rows behind the sequence and keys behind k_len are zeros in Q,
+      // dO, K and V, but their "probabilities" are not
+      const bool edge = r0 < wsure || r0 + KB > qlen || key0 + 32 > klen;
+      if (edge) {
+        const int from = a.causal ? key - off : 0;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int y = r0 + 32 * x + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (!(y >= from && y < qlen && key < klen)) { s[r] = 0.f; dp[r] = 0.f; }
+        }
+      }
+#pragma unroll
+      for (int cc = 0; cc < 2; cc++) {
+        const Frag<T> pf = acc_frag<T>(s, cc);
+#pragma unroll
+        for (int b = 0; b < NB; b++) av[b] = mma(col_frag<T, D>(gt, cb, x, cc, b), pf, av[b]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(rows + 64 + 32 * x + 8 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[4 * i + j] *= dp[4 * i + j] - dl[j];
+      }
+#pragma unroll
+      for (int cc = 0; cc < 2; cc++) {
+        const Frag<T> df = acc_frag<T>(s, cc);
+#pragma unroll
+        for (int b = 0; b < NB; b++) ak[b] = mma(col_frag<T, D>(qt, cb, x, cc, b), df, ak[b]);
+      }
+    }
+  }
+
+  if (key >= kroom) return;
+  T* pk = reinterpret_cast<T*>(a.dk) + (long long)(kstart + key) * a.dks + (long long)kvh * a.dkh;
+  T* pv = reinterpret_cast<T*>(a.dv) + (long long)(kstart + key) * a.dvs + (long long)kvh * a.dvh;
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int dd = 32 * b + 8 * i + 4 * h;
+      if (dd < a.d) {
+        store4(pk + dd, ak[b][4 * i] * a.scale, ak[b][4 * i + 1] * a.scale, ak[b][4 * i + 2] * a.scale, ak[b][4 * i + 3] * a.scale);
+        store4(pv + dd, av[b][4 * i], av[b][4 * i + 1], av[b][4 * i + 2], av[b][4 * i + 3]);
+      }
+    }
+}
+
+template <typename K>
+int set_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? AIT_OK : AIT_ELAUNCH;
+}
+template <typename T, int D, bool BIAS>
+int launch(const BwdArgs& a, hipStream_t st) {
+  const int bias = BIAS ? bias_row(a.bias.max_distance) * 4 : 0;
+  const int qb = 4 * Tile<T, D>::kBytes + bias + (BIAS ? NW * (kHist + a.bias.n_buckets) * 4 : 0), kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
+  AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS>, qb));
+  AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS>, kb));
+  if (a.s.total_q > 0) {
+    hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS>), dim3((unsigned)(a.qnumbers * a.H)), dim3(NT), qb, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  if (a.s.total_k > 0) {
+    hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS>), dim3((unsigned)(a.knumbers * a.Hk)), dim3(NT), kb, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  return AIT_OK;
+}
+template <typename T>
+int launch_t(const BwdArgs& a, hipStream_t st) {
+  if (a.bias.table) return a.d <= 64 ? launch<T, 64, true>(a, st) : launch<T, 128, true>(a, st);
+  return a.d <= 64 ? launch<T, 64, false>(a, st) : launch<T, 128, false>(a, st);
+}
+long long q_numbers(const ait_packed_attn& p) { return block_numbers(p.total_q, 1, BM, p.n_seq, p.zero_rest ? 1 : 0); }
+}  // namespace
+
+AIT_API size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p) {
+  if (ait_packed::check(p) != AIT_OK) return 0;
+  size_t n = 2 * (size_t)p->heads * p->total_q;
+  if (p->bias_table) n += (size_t)q_numbers(*p) * p->heads * p->n_buckets;
+  return n * sizeof(float);
+}
+
+AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
+                                long long o_head, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
+                                long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
+                                long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream) {
+  AIT_TRY_RC(ait_packed::check(p));
+  if (p->n_seq == 0 || (p->total_q == 0 && p->total_k == 0)) return AIT_OK;
+  if (!p->cu_q || !p->cu_k) return AIT_EINVAL;
+  AIT_TRY_RC(ait_packed::check_strides(p, q, q_row, q_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, o, o_row, o_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, d_o, do_row, do_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, dq, dq_row, dq_head, p->total_q));
+  AIT_TRY_RC(ait_packed::check_strides(p, k, k_row, k_head, p->total_k));
+  AIT_TRY_RC(ait_packed::check_strides(p, v, v_row, v_head, p->total_k));
+  AIT_TRY_RC(ait_packed::check_strides(p, dk, dk_row, dk_head, p->total_k));
+  AIT_TRY_RC(ait_packed::check_strides(p, dv, dv_row, dv_head, p->total_k));
+  if (p->total_q > 0 && !lse) return AIT_EINVAL;
+  const size_t need = ait_packed_attn_bwd_workspace_bytes(p);
+  if (!workspace || workspace_bytes < need) return AIT_EWORKSPACE;
+  BwdArgs a{q, k, v, o, d_o, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
+            dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
+            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
+            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
+            p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p),
+            (int)block_numbers(p->total_k, 1, BM, p->n_seq, p->zero_rest ? 1 : 0), p->scale, nullptr, nullptr, nullptr, d_table};
+  a.lse2 = static_cast<float*>(workspace);
+  a.delta = a.lse2 + (size_t)p->heads * p->total_q;
+  if (p->bias_table && d_table) a.part_table = a.delta + (size_t)p->heads * p->total_q;
+  const hipStream_t st = ait_stream(stream);
+  AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, st) : launch_t<__bf16>(a, st));
+  if (p->bias_table && d_table) {
+    if (p->total_q == 0) a.qnumbers = 0;
+    hipLaunchKernelGGL(packed_table_kernel, dim3((unsigned)p->heads, (unsigned)((p->n_buckets + 15) / 16)), dim3(256), 0, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  return AIT_OK;
+}

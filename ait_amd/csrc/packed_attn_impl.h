@@ -1,0 +1,299 @@
+// ait_amd/csrc/packed_attn_impl.h -- shared by packed_attn.hip (forward) and packed_attn_bwd.hip.
+//
+// Attention over sequences that lie one behind another in memory.  Every product runs on 32 x 32 matrix blocks in the
+// TRANSPOSED form: the scores as S^T = K Q^T, so that an accumulator column -- one lane and its partner 32 lanes away -- is
+// one query.  The softmax's running maximum, its sum and the rescaling are then values of a lane, the probabilities leave the
+// accumulators in the operand order of the second product (O^T = V^T P^T), and nothing passes through shared memory between
+// the two.  V^T comes out of the row-major tile by gfx950's transposing LDS read.
+//
+// One operand block ("Frag") is eight values a lane: of row / column lane & 31, reduction indices 8 (lane >> 5) + 0..7 of a
+// chunk of 16.  bf16: one v_mfma_f32_32x32x16_bf16 per chunk; f32: eight v_mfma_f32_32x32x2_f32, instruction e taking element e
+// of both halves -- the same chunk, so the kernels are one source for both types (f32 products are exact f32 products).
+#pragma once
+#include "common.h"
+
+namespace ait_packed {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+constexpr int KB = 64;              // keys (or, in the gradient of keys and values, queries) of a tile in shared memory
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kNegInf = -__builtin_inff();
+
+template <typename T> struct FragOf;
+template <> struct FragOf<__bf16> { using type = bf16x8; };
+template <> struct FragOf<float> { using type = f32x8; };
+template <typename T> using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ f32x16 mma(const bf16x8& a, const bf16x8& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// eight accumulator values (registers 8 cc .. 8 cc + 7) as an operand: reduction index 16 cc + 8 (e / 4) + 4 (lane >> 5) + e % 4
+// of the 32 the block has.  bf16: rounded to nearest even here -- the one rounding of the probabilities (and of dS in the
+// backward), to the type of the tensor they are multiplied with, as the matrix unit asks; sums stay in f32.
+template <typename T>
+__device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int cc) {
+  Frag<T> f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = (T)c[8 * cc + e];
+  return f;
+}
+
+// ---- tiles in shared memory: KB rows of D values, 16-byte chunk c of row r at position c ^ swz(r) -------------------------
+// Row operands (16 bytes of 32 consecutive rows) and transposed reads (32 bytes of four consecutive rows) both spread over
+// all 64 banks.  Chunk positions differ from chunks in the low bits only, so every offset below is one base XOR a constant.
+template <typename T, int D>
+struct Tile {
+  static constexpr int kRow = D * (int)sizeof(T);
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kBytes = KB * kRow;
+  __device__ static __forceinline__ int swz(int r) {
+    return kChunks >= 16 ? (4 * (r & 3) | ((r >> 2) & 3)) : (2 * (r & 3) | ((r >> 2) & 1));
+  }
+};
+
+// operand block of tile rows 32 rt .. + 31, values 16 c .. + 15 of each.  `base` = row_base<T, D>(lane)
+template <typename T, int D>
+__device__ __forceinline__ int row_base(int lane) {
+  const int r = lane & 31, h = lane >> 5;
+  return r * Tile<T, D>::kRow + (((sizeof(T) == 4 ? 2 * h : h) ^ Tile<T, D>::swz(r)) * 16);
+}
+template <typename T, int D>
+__device__ __forceinline__ Frag<T> row_frag(const unsigned char* tile, int base, int rt, int c) {
+  const unsigned char* p = tile + rt * 32 * Tile<T, D>::kRow;
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const bf16x8*>(p + (base ^ (c * 32)));
+  } else {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p + (base ^ (c * 64)));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(p + (base ^ (c * 64) ^ 16));
+    f32x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) { f[e] = lo[e]; f[4 + e] = hi[e]; }
+    return f;
+  }
+}
+
+// operand block of the tile TRANSPOSED: row = value 32 db + (lane & 31), reduction = tile rows 32 rt + 16 cc + the order of
+// acc_frag.  `base` = col_base<T, D>(lane)
+template <typename T, int D>
+__device__ __forceinline__ int col_base(int lane) {
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {      // the address a lane gives to the transposing read: four rows, 16 values, per 16 lanes
+    const int i = lane & 15, r = 4 * h + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    return r * Tile<T, D>::kRow + (chunk ^ Tile<T, D>::swz(r)) * 16 + (i & 1) * 8;
+  } else {
+    const int d = lane & 31;
+    return 4 * h * Tile<T, D>::kRow + ((d >> 2) ^ Tile<T, D>::swz(4 * h)) * 16 + (d & 3) * 4;
+  }
+}
+template <typename T, int D>
+__device__ __forceinline__ Frag<T> col_frag(const unsigned char* tile, int base, int rt, int cc, int db) {
+  constexpr int R = Tile<T, D>::kRow;
+  const unsigned char* p = tile + (rt * 32 + cc * 16) * R;
+  if constexpr (sizeof(T) == 2) {
+    constexpr int kUp = Tile<T, D>::kChunks >= 16 ? 32 : 0;      // what eight rows further down change in the swizzle
+    const int b = base ^ (db * 64);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + b));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (b ^ kUp) + 8 * R));
+    s16x8 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+    return __builtin_bit_cast(bf16x8, v);
+  } else {
+    const int b = base ^ (db * 128);
+    f32x8 f;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      f[e] = *reinterpret_cast<const float*>(p + (b ^ ((4 * (e & 3) | 2 * (e >> 2)) * 16)) + (8 * (e >> 2) + (e & 3)) * R);
+    return f;
+  }
+}
+
+// ---- global -> shared memory -----------------------------------------------------------------------------------------------
+// 16 bytes a lane straight into shared memory.  The buffer descriptor ends behind the sequence's last row (tile by tile: a
+// 64-bit base and at most KB rows of 32-bit offsets, so long caches need no wider offsets), and what lies outside arrives as
+// zeros: rows of the next sequence, the cache's unwritten tail and the padding of d to D never reach a product.
+__device__ __forceinline__ i32x4 tile_rsrc(const void* base, unsigned bytes) {
+  const unsigned long long p = (unsigned long long)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)p);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(p >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00027000;
+  return r;
+}
+__device__ __forceinline__ void load_lds16(unsigned voff, const i32x4& rsrc, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "s"(dst) : "m0", "memory");
+}
+// all of this wave's memory operations are done, and every wave of the workgroup says the same
+__device__ __forceinline__ void loads_done_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, int D, int NT>
+struct Loader {
+  static constexpr int kN = Tile<T, D>::kBytes / (NT * 16);          // instructions of a wave per tile
+  unsigned voff[kN];
+  // stride: bytes from row to row; d_bytes: bytes of a row that exist (a multiple of 16)
+  __device__ __forceinline__ void init(int tid, unsigned stride, unsigned d_bytes) {
+#pragma unroll
+    for (int j = 0; j < kN; j++) {
+      const int p = (tid >> 6) * kN * 64 + j * 64 + (tid & 63);
+      const int r = p / Tile<T, D>::kChunks, c = (p % Tile<T, D>::kChunks) ^ Tile<T, D>::swz(r);
+      voff[j] = (unsigned)(c * 16) < d_bytes ? (unsigned)r * stride + c * 16 : 0x80000000u;
+    }
+  }
+  // rows: how many of the tile's rows exist (any number; 0 or less: all zeros)
+  __device__ __forceinline__ void load(const void* base, long long rows, unsigned stride, unsigned d_bytes, unsigned lds, int wave) const {
+    const unsigned n = rows <= 0 ? 0u : (unsigned)(rows < KB ? rows : KB);
+    const i32x4 rsrc = tile_rsrc(base, n ? (n - 1) * stride + d_bytes : 0u);
+#pragma unroll
+    for (int j = 0; j < kN; j++) load_lds16(voff[j], rsrc, (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (wave * kN + j) * 1024)));
+  }
+};
+
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(const lds_u8*)p; }
+
+// eight values of a row in memory as an operand (values >= d, and rows that are not there: zero)
+template <typename T>
+__device__ __forceinline__ Frag<T> global_frag(const T* row, int at, int d, bool there) {
+  Frag<T> f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = (T)0.f;
+  if (there && at < d) {
+    if constexpr (sizeof(T) == 2) {
+      f = *reinterpret_cast<const bf16x8*>(row + at);
+    } else {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(row + at), hi = *reinterpret_cast<const f32x4*>(row + at + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) { f[e] = lo[e]; f[4 + e] = hi[e]; }
+    }
+  }
+  return f;
+}
+
+// four consecutive values of a row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 2) {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    bf16x4 v;
+    v[0] = (__bf16)a; v[1] = (__bf16)b; v[2] = (__bf16)c; v[3] = (__bf16)d;
+    *reinterpret_cast<bf16x4*>(p) = v;
+  } else {
+    f32x4 v;
+    v[0] = a; v[1] = b; v[2] = c; v[3] = d;
+    *reinterpret_cast<f32x4*>(p) = v;
+  }
+}
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the two lanes of an accumulator column (32 apart): both get both values, in the same order
+__device__ __forceinline__ void column_pair(float v, float& lo, float& hi) {
+  lo = hi = v;      // the upper half of one register swaps places with the lower half of the other (as attn_impl.h swap16)
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(lo), "+v"(hi));
+}
+__device__ __forceinline__ float column_max(float v) {
+  float a, b;
+  column_pair(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float column_sum(float v) {
+  float a, b;
+  column_pair(v, a, b);
+  return a + b;
+}
+
+// ---- which rows a workgroup has ---------------------------------------------------------------------------------------------
+// Row blocks of BM are numbered so that no host knows the lengths: block j of sequence b has number start(b) * mul / BM + b + j.
+// A sequence of n rows needs at most n / BM + 1 of the n / BM + 1 numbers up to its successor's first, so numbers never clash;
+// the few unused ones are workgroups that end at once.  Lengths and starts come from device memory and are clamped to the
+// tensors they index, so that a bad table gives wrong rows, never a wrong address.
+__device__ __forceinline__ int clamped(const int* cu, int i, int total) {
+  const int v = cu[i];
+  return v < 0 ? 0 : v > total ? total : v;
+}
+// With `rest` the rows behind the last sequence count as one more, number n_seq: the blocks that set them to zero.
+__device__ __forceinline__ bool find_block(const int* cu, int n_seq, int rest, int total, int mul, int bm, int number, int& seq, int& block,
+                                           int& start, int& len) {
+  int lo = 0, hi = n_seq - 1 + rest;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int)((long long)clamped(cu, mid, total) * mul / bm) + mid <= number) lo = mid;
+    else hi = mid - 1;
+  }
+  seq = lo;
+  start = clamped(cu, lo, total);
+  len = (lo < n_seq ? clamped(cu, lo + 1, total) : total) - start;
+  block = number - (int)((long long)start * mul / bm) - lo;
+  return block >= 0 && (long long)block * bm < (long long)len * mul;
+}
+static inline long long block_numbers(long long total, int mul, int bm, int n_seq, int rest) {
+  return total * mul / bm + n_seq + rest;
+}
+
+struct Seqs {
+  const int* cu_q;
+  const int* cu_k;
+  const int* k_len;        // may be null: the keys of a sequence end where the next one's begin
+  int n_seq, total_q, total_k, rest;
+};
+__device__ __forceinline__ void keys_of(const Seqs& s, int seq, int& start, int& len) {
+  start = clamped(s.cu_k, seq, s.total_k);
+  len = clamped(s.cu_k, seq + 1, s.total_k) - start;
+  if (len < 0) len = 0;
+  if (s.k_len) {
+    const int l = s.k_len[seq];
+    len = l < 0 ? 0 : l < len ? l : len;
+  }
+}
+
+// ---- the bias: one value per relative position and head, constant beyond max_distance on either side --------------------------
+// A workgroup keeps the values of its heads in shared memory, kPad of the outermost ones on either side: a 64 x 32 block that
+// touches the inner range reads them at one address per lane plus constants; a block that does not adds one constant.
+struct Bias {
+  const float* table;      // [n_buckets, H]; null: no bias
+  const int* bucket_of;    // [2 max_distance + 1], by key - query + max_distance
+  int n_buckets, max_distance;
+};
+constexpr int kPad = 96;
+__host__ __device__ static inline int bias_row(int max_distance) { return 2 * (max_distance + kPad) + 1; }
+__device__ __forceinline__ int bucket(const Bias& b, int rel) {
+  const int m = b.max_distance, i = (rel < -m ? -m : rel > m ? m : rel) + m, v = b.bucket_of[i];
+  return v < 0 ? 0 : v >= b.n_buckets ? b.n_buckets - 1 : v;
+}
+// in units of the exponent to base 2.  The lowest finite values stay finite: a row that sees nothing else still has its softmax
+__device__ __forceinline__ float bias_log2(float t) {
+  const float v = t * kLog2e;
+  return (v == kNegInf && t != kNegInf) ? -3.402823466e38f : v;
+}
+
+template <int NT>
+__device__ __forceinline__ void fill_bias(const Bias& b, int H, int head0, int heads, float* lds, int tid) {
+  const int w = bias_row(b.max_distance);
+  for (int g = 0; g < heads; g++)
+    for (int x = tid; x < w; x += NT)
+      lds[g * w + x] = bias_log2(b.table[(size_t)bucket(b, x - b.max_distance - kPad) * H + head0 + g]);
+}
+
+int check(const ait_packed_attn* p);
+int check_strides(const ait_packed_attn* p, const void* base, long long row, long long head, long long rows);
+
+}  // namespace ait_packed

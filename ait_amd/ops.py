@@ -783,3 +783,114 @@ def conv_bwd_weight_bf16s(dy16, x16, geom, kh, kw, split_k=8, partials=False):
                                                   _lib.launch_ctx(dy16.device), _lib.cur_stream(dy16.device))
     _lib.check(rc, "ait_conv_bwd_weight_bf16s")
     return dw
+
+
+# ------------------------------------------------------------------------------------------
+# packed sequences (ait_packed_attn_*; autograd in ait_amd/packed.py)
+# ------------------------------------------------------------------------------------------
+def _need(ok, what):
+    if not ok:
+        raise _lib.AitHipError("packed_attn: " + what)
+
+
+def _index(name, t, n, device):
+    _need(torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == n, "`%s` must be an int32 tensor of %d values" % (name, n))
+    _need(t.device == device, "`%s` is on %s, the tensors on %s" % (name, t.device, device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _fit(t):
+    """t [rows, heads, d] with unit element stride, row / head pitches and a base of whole 16-byte vectors -- itself, or a copy"""
+    v = 16 // t.element_size()
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] < 2 or (t.stride(i) % v == 0 and t.stride(i) >= 0) for i in (0, 1)) \
+        and t.stride(0) * t.element_size() < 2 ** 25
+    return t if ok or t.numel() == 0 else t.contiguous()
+
+
+def _row_head(t):
+    """(pointer, row pitch, head pitch): pitches of dimensions of size one are free, the library wants whole vectors"""
+    v = 16 // t.element_size()
+    return ctypes.c_void_p(t.data_ptr()), t.stride(0) - t.stride(0) % v, t.stride(1) - t.stride(1) % v
+
+
+def packed_attn_desc(q, k, v, cu_q, cu_k, k_len=None, max_q=None, max_k=None, causal=False, scale=None, table=None, bucket_of=None):
+    """checks the arguments and returns (ait_packed_attn, the tensors it points at)"""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _need(torch.is_tensor(t) and t.dim() == 3, "`%s` must be [rows, heads, d]" % n)
+        _need(t.dtype in _lib.DTYPES, "float32 or bfloat16 expected, got %s for `%s`" % (t.dtype, n))
+        _need(t.dtype == q.dtype and t.device == q.device, "q, k and v share one type and device")
+    (tq, H, d), (tk, Hk, dk) = q.shape, k.shape
+    _need(tuple(v.shape) == (tk, Hk, dk) and dk == d, "k and v must be [rows, kv_heads, %d] alike (got %s, %s)" % (d, tuple(k.shape), tuple(v.shape)))
+    _need(H > 0 and Hk > 0 and H % Hk == 0, "%d heads cannot share %d key heads" % (H, Hk))
+    _need(0 < d <= 128 and d % 8 == 0, "head width %d: a multiple of 8 up to 128 expected" % d)
+    _need(max(tq, tk) < 2 ** 31, "row counts must fit 31 bits")
+    _need(torch.is_tensor(cu_q) and cu_q.dim() == 1 and cu_q.numel() > 0, "`cu_q` must be an int32 tensor of n_seq + 1 values")
+    n = cu_q.numel() - 1
+    dev = q.device
+    cu_q, cu_k = _index("cu_q", cu_q, n + 1, dev), _index("cu_k", cu_k, n + 1, dev)
+    k_len = None if k_len is None else _index("k_len", k_len, n, dev)
+    p = _lib.PackedAttn()
+    if table is not None:
+        _need(torch.is_tensor(table) and table.dim() == 2 and table.shape[1] == H and table.shape[0] > 0 and table.dtype == torch.float32
+              and table.device == dev, "the bias table must be a float32 [n_buckets, %d] tensor on %s" % (H, dev))
+        _need(torch.is_tensor(bucket_of) and bucket_of.dim() == 1 and bucket_of.numel() % 2 == 1, "`bucket_of` must have 2 * max_distance + 1 values")
+        bucket_of = _index("bucket_of", bucket_of, bucket_of.numel(), dev)
+        _need(table.shape[0] <= _lib.MAX_BUCKETS and bucket_of.numel() // 2 <= _lib.MAX_BIAS_DISTANCE,
+              "at most %d buckets and a distance of %d" % (_lib.MAX_BUCKETS, _lib.MAX_BIAS_DISTANCE))
+        table = table.contiguous()
+        p.n_buckets, p.max_distance = table.shape[0], bucket_of.numel() // 2
+        p.bias_table, p.bucket_of = table.data_ptr(), bucket_of.data_ptr()
+    if not q.is_cuda:
+        raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % q.device)
+    p.cu_q, p.cu_k, p.k_len = cu_q.data_ptr(), cu_k.data_ptr(), None if k_len is None else k_len.data_ptr()
+    p.n_seq, p.total_q, p.total_k, p.heads, p.kv_heads, p.d = n, tq, tk, H, Hk, d
+    p.max_q, p.max_k = min(int(max_q or 0), tq), min(int(max_k or 0), tk)
+    p.dtype, p.causal, p.scale = _lib.DTYPES[q.dtype], int(bool(causal)), float(d ** -0.5 if scale is None else scale)
+    return p, (cu_q, cu_k, k_len, table, bucket_of)
+
+
+def packed_attn_fwd(p, q, k, v, out=None, want_lse=False):
+    """ait_packed_attn_fwd: o [total_q, heads, d] (rows of no sequence: zero, or left as they are in a given `out`), lse
+    [heads, total_q] or None.  p: packed_attn_desc's."""
+    L = _lib.lib()
+    dev = q.device
+    q, k, v = _fit(q), _fit(k), _fit(v)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        p.zero_rest = 1
+        if p.n_seq == 0:
+            out.zero_()
+    else:
+        _need(out.is_cuda and out.device == dev and out.dtype == q.dtype and out.shape == q.shape and _fit(out) is out
+              and all(out.shape[i] < 2 or out.stride(i) > 0 for i in (0, 1)),
+              "`out` must be a %s tensor of q's shape with 16-byte rows" % q.dtype)
+        p.zero_rest = 0
+    lse = torch.empty((p.heads, p.total_q), dtype=torch.float32, device=dev) if want_lse else None
+    with torch.cuda.device(dev):
+        n = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(p))
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        rc = L.ait_packed_attn_fwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(out), _p(lse),
+                                   None if ws is None else ctypes.c_void_p(ws.data_ptr()), n, _lib.cur_stream(dev))
+    _lib.check(rc, "ait_packed_attn_fwd")
+    return out, lse
+
+
+def packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=False):
+    """ait_packed_attn_bwd: (dq, dk, dv, d_table f32 [n_buckets, heads] or None)"""
+    L = _lib.lib()
+    dev = q.device
+    q, k, v, o, d_o = _fit(q), _fit(k), _fit(v), _fit(o), _fit(d_o)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    p.zero_rest = 1
+    if p.n_seq == 0:
+        dq.zero_(), dk.zero_(), dv.zero_()
+    dt = torch.zeros((p.n_buckets, p.heads), dtype=torch.float32, device=dev) if want_table and (p.n_seq == 0 or p.total_q == 0) else \
+        torch.empty((p.n_buckets, p.heads), dtype=torch.float32, device=dev) if want_table else None
+    with torch.cuda.device(dev):
+        n = L.ait_packed_attn_bwd_workspace_bytes(ctypes.byref(p))
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        rc = L.ait_packed_attn_bwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(o), *_row_head(d_o), _p(lse),
+                                   *_row_head(dq), *_row_head(dk), *_row_head(dv), _p(dt), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
+                                   _lib.cur_stream(dev))
+    _lib.check(rc, "ait_packed_attn_bwd")
+    return dq, dk, dv, dt

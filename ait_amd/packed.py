@@ -1,0 +1,96 @@
+"""Transformer operators on packed token sequences, with gradients: sequences of any lengths lie one behind another in
+[rows, ...] tensors, `cu_seqlens` [n_seq + 1] int32 holds where each begins.
+
+    packed_attention(q, k, v, cu_q, cu_k)                 any lengths, grouped heads, causal or not, caches for new tokens
+    relative_buckets / RelativePositionBias               a learned bias of its scores by buckets of the relative position
+
+The general-length counterparts of the 64-token blocks in ait_amd/system.py (ScaledDotProductAttention,
+lib/model/system/Modules.py:16-29; the sinusoid table of PositionalEncoding, lib/model/system/Models.py:26-50).  float32 or
+bfloat16 tensors on a GPU; there is no CPU path.  The kernels run on the current stream of the tensors' device, take their
+scratch from torch's allocator per call and may be captured into a graph.
+"""
+import torch
+import torch.nn as nn
+
+from . import _lib, ops
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of):
+        table32 = None if table is None else table.float()
+        p, keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table32, bucket_of)
+        grad = any(ctx.needs_input_grad[:4])
+        o, lse = ops.packed_attn_fwd(p, q, k, v, want_lse=grad)
+        if grad:
+            ctx.save_for_backward(q, k, v, o, lse, *[t for t in keep if t is not None])
+            ctx.there = [t is not None for t in keep]
+            ctx.cfg = (max_q, max_k, causal, scale, None if table is None else table.dtype)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o):
+        q, k, v, o, lse, *keep = ctx.saved_tensors
+        cu_q, cu_k, k_len, table, bucket_of = [keep.pop(0) if t else None for t in ctx.there]
+        max_q, max_k, causal, scale, dt = ctx.cfg
+        p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)
+        dq, dk, dv, d_table = ops.packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=table is not None and ctx.needs_input_grad[3])
+        n = ctx.needs_input_grad
+        return (dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, None if d_table is None else d_table.to(dt)) + (None,) * 8
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=None, causal=False, scale=None, bias=None):
+    """softmax(scale q k^T + bias) v of every sequence and head -> [total_q, heads, d].
+
+    q [total_q, heads, d], k / v [total_k, kv_heads, d] (float32 or bfloat16; head h reads key head h // (heads // kv_heads); any
+    strides, views of a fused projection are read in place where their rows are whole 16-byte vectors and copied where not; d a
+    multiple of 8 up to 128).  cu_q, cu_k: int32 starts [n_seq + 1], the first 0, not descending; cu_k None: the keys are packed
+    like the queries.  k_len int32 [n_seq]: the sequence's keys are the first k_len of its rows -- a cache whose rows behind them
+    may hold anything.  causal: the last query is level with the last key and a query sees no later key.  scale: d ** -0.5.
+    bias: (table [n_buckets, heads], bucket_of), or a RelativePositionBias.  max_q / max_k: the longest lengths where the host
+    knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis).
+
+    A query that sees no key gives zeros; so do rows behind the last sequence, and neither takes part in a gradient.  Gradients
+    of q, k, v and the table; a captured backward belongs to a forward captured in the same graph."""
+    table = bucket_of = None
+    if bias is not None:
+        table, bucket_of = (bias.weight, bias.bucket_of) if isinstance(bias, RelativePositionBias) else bias
+        if not torch.is_tensor(table) or table.dtype not in _lib.DTYPES:
+            raise _lib.AitHipError("packed_attn: the bias table must be a float32 or bfloat16 tensor")
+    return _PackedAttention.apply(q, k, v, table, cu_q, cu_q if cu_k is None else cu_k, k_len, max_q, max_k, bool(causal), scale, bucket_of)
+
+
+def relative_buckets(n_buckets, max_distance, two_sided, device=None):
+    """int32 [2 * max_distance + 1]: the bucket of every relative position key - query from -max_distance to max_distance (those
+    further away share the outermost ones').  The bucketing of Raffel et al., "Exploring the Limits of Transfer Learning with a
+    Unified Text-to-Text Transformer" (2020), section 2.1: of the n buckets of a side the first n // 2 hold one distance each,
+    the others steps of equal ratio up to max_distance.  two_sided: half the buckets for keys behind the query, half for those
+    ahead; else all keys ahead share bucket 0.  Borders are found in whole numbers: step t begins at the least distance a with
+    (a / e) ** N >= (max_distance / e) ** t, e the exact buckets and N the others."""
+    side = n_buckets // 2 if two_sided else n_buckets
+    e = side // 2
+    if n_buckets <= 0 or (two_sided and n_buckets % 2) or e < 1 or max_distance <= e:
+        raise ValueError("relative_buckets: %d buckets%s do not reach from exact steps to a distance of %d"
+                         % (n_buckets, " on two sides" if two_sided else "", max_distance))
+    if n_buckets > _lib.MAX_BUCKETS or max_distance > _lib.MAX_BIAS_DISTANCE:
+        raise ValueError("relative_buckets: at most %d buckets and a distance of %d" % (_lib.MAX_BUCKETS, _lib.MAX_BIAS_DISTANCE))
+    N, of = side - e, []
+    t = 0
+    for a in range(max_distance + 1):
+        while t < N - 1 and a >= e and a ** N * e ** (t + 1) >= max_distance ** (t + 1) * e ** N:
+            t += 1
+        of.append(a if a < e else e + t)
+    of[max_distance] = side - 1
+    ahead = [side + of[a] for a in range(1, max_distance + 1)] if two_sided else [0] * max_distance
+    return torch.tensor(of[::-1] + ahead, dtype=torch.int32, device=device)
+
+
+class RelativePositionBias(nn.Module):
+    """A learned bias per head and bucket of the relative position, for packed_attention(bias=...); as the sinusoid table of
+    PositionalEncoding it is shared by all sequences.  weight [n_buckets, n_head]."""
+
+    def __init__(self, n_head, n_buckets=32, max_distance=128, two_sided=True):
+        super().__init__()
+        self.weight = nn.Parameter(torch.zeros(n_buckets, n_head))
+        self.register_buffer("bucket_of", relative_buckets(n_buckets, max_distance, two_sided), persistent=False)

@@ -865,6 +865,65 @@ int ait_sk_sqsum_fwd(const float* a, const float* b, long long n, float* y, void
 int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long n, float* da,
                      float* db, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Attention over packed sequences of any lengths, with grouped heads and a learned relative position bias.
+ * The general-length counterpart of ait_attn_fwd / _bwd (T = 64, d = 64): no score leaves the chip.  Stands beside
+ * ScaledDotProductAttention.forward (lib/model/system/Modules.py:16-29); the reference has no packed form of it.
+ *
+ *   s_ij = scale q_i . k_j + table[bucket_of[clamp(j - i - (len_k - len_q)) + max_distance]][head]
+ *   o_i  = sum_j softmax_j(s_ij) v_j        over the keys j that query i sees: all of its sequence, or with `causal`
+ *                                           those with j - i <= len_k - len_q (the last query sees every key)
+ *
+ * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and lse = -infinity, and
+ * takes part in no gradient.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
+ * multiplied, whatever it holds; a key INSIDE the sequence that a causal mask hides from a query must be finite (its value is
+ * multiplied by a probability of zero).
+ *
+ *   q [total_q, heads, d], k / v [total_k, kv_heads, d], o as q: element (row, head, e) at row * _row + head * _head + e, both
+ *     pitches and the base multiples of 16 bytes, else AIT_EUNSUPPORTED.  Head h reads key head h / (heads / kv_heads).
+ *   cu_q [n_seq + 1], cu_k [n_seq + 1] int32 on the device: sequence b has query rows cu_q[b] .. cu_q[b + 1] - 1, ascending from 0;
+ *     k_len [n_seq] int32 or NULL: it has k_len[b] keys (at most cu_k[b + 1] - cu_k[b]) from cu_k[b] on -- a cache.  Values
+ *     outside the tensors are clamped to them.  Rows of q behind the last sequence are not read; those of o (dq, dk, dv) are
+ *     left as they are, or set to zero with zero_rest.
+ *   max_q, max_k: the longest lengths as far as the host knows them (0: unknown).  They choose how work is cut up, and nothing
+ *     but the order of sums depends on them.
+ *   dtype AIT_DTYPE_F32 (exact f32 products) or AIT_DTYPE_BF16 (f32 scores, statistics and sums; probabilities and dS are
+ *     rounded to bf16 where they enter a product) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
+ *   bias_table f32 [n_buckets, heads] or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
+ *     table): the bucket of relative position key - query, where the last query is level with the last key; further away the
+ *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
+ *   lse f32 [heads, total_q] or NULL: log of the sum of exp of a row's scores, which the backward reads.
+ *
+ * Backward: dq / dk / dv (pitches as given), and with a bias d_table f32 [n_buckets, heads] (overwritten; NULL: not wanted).
+ * No atomics on memory: results are the same from run to run, and do not depend on what else runs.
+ * Workspaces: the caller's, used by one call at a time.
+ * ------------------------------------------------------------------------------------- */
+#define AIT_DTYPE_F32 0
+#define AIT_DTYPE_BF16 1
+#define AIT_MAX_BUCKETS 512
+#define AIT_MAX_BIAS_DISTANCE 2048
+typedef struct {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* k_len;
+  const float* bias_table;
+  const int32_t* bucket_of;
+  int n_seq, total_q, total_k, max_q, max_k;
+  int heads, kv_heads, d, dtype, causal;
+  int n_buckets, max_distance, zero_rest;
+  float scale;
+} ait_packed_attn;
+size_t ait_packed_attn_fwd_workspace_bytes(const ait_packed_attn* p);
+int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                        long long k_head, const void* v, long long v_row, long long v_head, void* o, long long o_row,
+                        long long o_head, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p);
+int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                        long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
+                        long long o_head, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
+                        long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
+                        long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
