@@ -125,6 +125,9 @@ SIGNATURES = {
                           _vp, _i, _vp, _i, _vp]),
     "ait_packed_attn_fwd_workspace_bytes": (_sz, [_vp]),
     "ait_packed_attn_fwd": (_i, [_vp] + [_vp, _ll, _ll] * 4 + [_vp, _vp, _sz, _vp]),
+    "ait_gated_norm_fwd": (_i, [_vp, _vp, _ll, _vp, _ll, _vp, _vp]),
+    "ait_gated_norm_bwd_workspace_bytes": (_sz, [_vp]),
+    "ait_gated_norm_bwd": (_i, [_vp, _vp] + [_vp, _ll] * 5 + [_vp] * 6 + [_sz, _vp]),
     "ait_packed_attn_bwd_workspace_bytes": (_sz, [_vp]),
     "ait_packed_attn_bwd": (_i, [_vp] + [_vp, _ll, _ll] * 5 + [_vp] + [_vp, _ll, _ll] * 3 + [_vp, _vp, _sz, _vp]),
 }
@@ -225,8 +228,16 @@ class PackedAttn(ctypes.Structure):
                                      "n_buckets", "max_distance", "zero_rest")] + [("scale", ctypes.c_float)]
 
 
+class GatedNorm(ctypes.Structure):
+    """ait_gated_norm."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "f", "gate", "cu_seqlens", "w_post", "b_post", "w_pre", "b_pre", "scale")] + \
+        [(n, ctypes.c_longlong) for n in ("x_row", "f_row", "gate_row")] + \
+        [(n, ctypes.c_int) for n in ("rows", "width", "n_seq", "dtype_x", "dtype_f", "layer", "zero_rest")] + [("eps", ctypes.c_float)]
+
+
 DTYPES = {torch.float32: 0, torch.bfloat16: 1}      # AIT_DTYPE_*
 MAX_BUCKETS, MAX_BIAS_DISTANCE = 512, 2048          # AIT_MAX_*
+MAX_NORM_WIDTH = 8192
 
 PROBE_GEMM, PROBE_ROI_FWD, PROBE_ROI_BWD = 1, 2, 3
 

@@ -1,0 +1,528 @@
+// ait_amd/csrc/gated_norm.hip -- ait_gated_norm_fwd / _bwd: the norm behind a block, its gate and residual scale, the residual
+// and the norm in front of the next block, one pass over the rows.
+//
+//   m = norm(f) w_post (+ b_post),   y = x + scale * gate * m,   h = norm(y) w_pre (+ b_pre)
+//   norm(t) = (t - mean) / sqrt(mean((t - mean)^2) + eps), or without the means
+//
+// Bound by memory: x, f and the gate are read once, y and h written once; a row lives in the registers of its G waves between
+// the two norms (all sums f32, the variance from the centred values).  The backward reads x, f, gate, dy, dh and forms the row
+// again from them and the four saved statistics, in f32 -- y as it was before it was rounded -- and keeps the column sums (the
+// parameters' gradients) in registers over the rows of a workgroup; the workgroups' parts are added in order by a second
+// kernel, so results repeat bit for bit.
+#include "common.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct NormArgs {
+  const void* x;
+  const void* f;
+  const void* gate;
+  const float* w_post;
+  const float* b_post;
+  const float* w_pre;
+  const float* b_pre;
+  const float* scale;
+  const int* cu;
+  long long x_row, f_row, g_row, y_row, h_row;
+  int rows, width, layer, gate_kind, n_seq;      // gate_kind: 0 none, 1 a row's own, 2 its sequence's
+  float eps;
+  void* y;
+  void* h;
+  float* stats;        // [rows][4]: mean of f, 1 / deviation of f, mean of y, 1 / deviation of y
+  // backward
+  const void* dy;
+  const void* dh;
+  long long dy_row, dh_row, dx_row, df_row, dg_row;
+  void* dx;
+  void* df;
+  void* dgate;
+  float* parts;        // [units][n_parts][width] of the parameters, then [units + n_seq][width] of the sequences' gates
+  int units, per, n_parts;      // a unit: a group of waves and its `per` consecutive rows
+  int zero_rest;
+};
+// which parts there are: w_post, w_pre, then scale, b_post, b_pre where given
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int at, int width, bool vec, float* v) {
+  if (vec) {
+    if (at < width) {
+      if constexpr (sizeof(T) == 2) {
+        const bf16x8 t = *reinterpret_cast<const bf16x8*>(row + at);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (float)t[e];
+      } else {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(row + at), b = *reinterpret_cast<const f32x4*>(row + at + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = at + e < width ? (float)row[at + e] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int at, int width, bool vec, const float* v) {
+  if (vec) {
+    if (at >= width) return;
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 t;
+#pragma unroll
+      for (int e = 0; e < 8; e++) t[e] = (__bf16)v[e];
+      *reinterpret_cast<bf16x8*>(row + at) = t;
+    } else {
+      f32x4 a, b;
+#pragma unroll
+      for (int e = 0; e < 4; e++) { a[e] = v[e]; b[e] = v[4 + e]; }
+      *reinterpret_cast<f32x4*>(row + at) = a;
+      *reinterpret_cast<f32x4*>(row + at + 4) = b;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (at + e < width) row[at + e] = (T)v[e];
+  }
+}
+
+// sums over the G waves of a row, two at a time; every lane gets them.  `slot` alternates so that one barrier a sum is enough
+template <int G>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* lds, int& slot, int group_wave, int wave) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (G > 1) {
+    float* p = lds + (slot & 1) * 32;
+    slot++;
+    if ((threadIdx.x & 63) == 0) { p[2 * wave] = a; p[2 * wave + 1] = b; }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < G; w++) { a += p[2 * (group_wave + w)]; b += p[2 * (group_wave + w) + 1]; }
+  }
+}
+
+__device__ __forceinline__ int clamp_row(const int* cu, int i, int rows) {
+  const int v = cu[i];
+  return v < 0 ? 0 : v > rows ? rows : v;
+}
+// the sequence of a row, n_seq behind the last one
+__device__ __forceinline__ int seq_of(const int* cu, int n_seq, int rows, int row) {
+  if (row >= clamp_row(cu, n_seq, rows)) return n_seq;
+  int lo = 0, hi = n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (clamp_row(cu, mid, rows) <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// G waves a row, V blocks of eight values a lane: a row has up to 64 G * 8 V values.  NT threads: NT / 64 / G rows at a time
+template <int G> struct Block { static constexpr int kWaves = G < 4 ? 4 : G, kThreads = kWaves * 64, kRows = kWaves / G; };
+
+template <typename X, typename F, int G, int V>
+__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(const NormArgs a, const bool vec) {
+  __shared__ float lds[64];
+  const int wave = threadIdx.x >> 6, group = wave / G, gl = threadIdx.x - group * G * 64;
+  const int row = blockIdx.x * Block<G>::kRows + group, W = a.width;
+  int slot = 0;
+  const bool there = row < a.rows;
+  const int rc = there ? row : a.rows - 1;
+  const float inv_w = 1.f / W;
+  const int seq = a.gate_kind == 2 ? seq_of(a.cu, a.n_seq, a.rows, rc) : 0;
+  const bool dead = a.gate_kind == 2 && seq == a.n_seq;          // behind the last sequence: left as it is, or set to zero
+  const bool write = there && (!dead || a.zero_rest);
+  float f[V][8], x[V][8];
+#pragma unroll
+  for (int v = 0; v < V; v++) load8(reinterpret_cast<const F*>(a.f) + rc * a.f_row, (gl + v * G * 64) * 8, W, vec, f[v]);
+#pragma unroll
+  for (int v = 0; v < V; v++) load8(reinterpret_cast<const X*>(a.x) + rc * a.x_row, (gl + v * G * 64) * 8, W, vec, x[v]);
+  float mean = 0.f, s1 = 0.f, s2 = 0.f;
+  if (a.layer) {
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) s1 += f[v][e];
+    row_sum2<G>(s1, s2, lds, slot, group * G, wave);
+    mean = s1 * inv_w;
+  }
+  s1 = s2 = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      f[v][e] -= (gl + v * G * 64) * 8 + e < W ? mean : 0.f;
+      s1 = __builtin_fmaf(f[v][e], f[v][e], s1);
+    }
+  row_sum2<G>(s1, s2, lds, slot, group * G, wave);
+  const float r = 1.f / __builtin_sqrtf(s1 * inv_w + a.eps), fmean = mean;
+  s1 = s2 = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int at = (gl + v * G * 64) * 8;
+    float p[8];
+    load8(a.w_post, at, W, vec, p);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[v][e] = f[v][e] * r * p[e];
+    if (a.b_post) {
+      load8(a.b_post, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[v][e] += p[e];
+    }
+    if (a.gate_kind) {
+      load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[v][e] *= p[e];
+    }
+    if (a.scale) {
+      load8(a.scale, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[v][e] *= p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      x[v][e] += f[v][e];
+      s1 += x[v][e];
+    }
+    if (dead) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[v][e] = 0.f;
+    }
+    if (write) store8(reinterpret_cast<X*>(a.y) + rc * a.y_row, at, W, vec, x[v]);
+  }
+  mean = 0.f;
+  if (a.layer) {
+    row_sum2<G>(s1, s2, lds, slot, group * G, wave);
+    mean = s1 * inv_w;
+  }
+  s1 = s2 = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      x[v][e] -= (gl + v * G * 64) * 8 + e < W ? mean : 0.f;
+      s1 = __builtin_fmaf(x[v][e], x[v][e], s1);
+    }
+  row_sum2<G>(s1, s2, lds, slot, group * G, wave);
+  const float ry = 1.f / __builtin_sqrtf(s1 * inv_w + a.eps);
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int at = (gl + v * G * 64) * 8;
+    float p[8];
+    load8(a.w_pre, at, W, vec, p);
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[v][e] = x[v][e] * ry * p[e];
+    if (a.b_pre) {
+      load8(a.b_pre, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[v][e] += p[e];
+    }
+    if (dead) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[v][e] = 0.f;
+    }
+    if (write) store8(reinterpret_cast<F*>(a.h) + rc * a.h_row, at, W, vec, x[v]);
+  }
+  if (a.stats && there && gl == 0) {
+    f32x4 s;
+    s[0] = fmean; s[1] = r; s[2] = mean; s[3] = ry;
+    *reinterpret_cast<f32x4*>(a.stats + 4ll * row) = s;
+  }
+}
+
+// one workgroup: `per` rows, one behind another per group of waves (a workgroup's groups take them in turn)
+template <typename X, typename F, int G, int V>
+__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(const NormArgs a, const bool vec) {
+  constexpr int R = Block<G>::kRows;
+  __shared__ float lds[64];
+  const int wave = threadIdx.x >> 6, group = wave / G, gl = threadIdx.x - group * G * 64, W = a.width;
+  const float inv_w = 1.f / W;
+  int slot = 0;
+  // column sums: [part][value]; a group's rows are `per` / R consecutive ones
+  float cp[V][8], cq[V][8], cs[V][8], bp[V][8], bq[V][8], cg[V][8];
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) cp[v][e] = cq[v][e] = cs[v][e] = bp[v][e] = bq[v][e] = cg[v][e] = 0.f;
+  const int unit = blockIdx.x * R + group, first = unit * a.per, last = min(first + a.per, a.rows);
+  float* gate_parts = a.parts + (size_t)a.units * a.n_parts * W;
+  int seq = 0;
+  if (a.gate_kind == 2 && first < a.rows) seq = seq_of(a.cu, a.n_seq, a.rows, first);
+  for (int i = 0; i < a.per; i++) {          // (every group makes every turn: the sums meet at barriers)
+    const int row = first + i;
+    const bool there = row < last;
+    const int rc = there ? row : a.rows - 1;
+    if (a.gate_kind == 2 && there && seq < a.n_seq && row >= clamp_row(a.cu, seq + 1, a.rows)) {
+      // the sequence's share of this workgroup is complete: units and sequences only ever go up together, so unit + sequence
+      // numbers the pairs that meet without a clash
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        store8(gate_parts + (size_t)(unit + seq) * W, (gl + v * G * 64) * 8, W, vec, cg[v]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) cg[v][e] = 0.f;
+      }
+      seq = seq_of(a.cu, a.n_seq, a.rows, row);
+    }
+    const bool dead = !there || (a.gate_kind == 2 && seq == a.n_seq);
+    const bool write = there && (!dead || a.zero_rest);
+    const int L = dead ? 0 : W;             // a dead row is a row of zeros, whatever memory holds
+    f32x4 st = *reinterpret_cast<const f32x4*>(a.stats + 4ll * rc);
+    if (dead) st[0] = st[1] = st[2] = st[3] = 0.f;
+    float f[V][8], y[V][8], g[V][8], d[V][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int at = (gl + v * G * 64) * 8;
+      float p[8], q[8];
+      load8(reinterpret_cast<const F*>(a.f) + rc * a.f_row, at, L, vec, f[v]);
+      load8(reinterpret_cast<const X*>(a.x) + rc * a.x_row, at, L, vec, y[v]);
+      load8(reinterpret_cast<const F*>(a.dh) + rc * a.dh_row, at, L, vec, d[v]);
+      load8(a.w_post, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        f[v][e] = at + e < W ? (f[v][e] - st[0]) * st[1] : 0.f;       // norm(f)
+        g[v][e] = f[v][e] * p[e];                                    // m
+      }
+      if (a.b_post) {
+        load8(a.b_post, at, W, vec, p);
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[v][e] += p[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = 1.f;
+      if (a.gate_kind) load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) q[e] = 1.f;
+      if (a.scale) load8(a.scale, at, W, vec, q);
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[v][e] = at + e < W ? (y[v][e] + g[v][e] * p[e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
+      load8(a.w_pre, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        cq[v][e] = __builtin_fmaf(d[v][e], y[v][e], cq[v][e]);
+        bq[v][e] += d[v][e];
+        d[v][e] *= p[e];
+        s1 = __builtin_fmaf(d[v][e], y[v][e], s1);
+        s2 += d[v][e];
+      }
+    }
+    row_sum2<G>(s1, s2, lds, slot, group * G, wave);
+    s1 *= inv_w;
+    s2 = a.layer ? s2 * inv_w : 0.f;
+    float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int at = (gl + v * G * 64) * 8;
+      float p[8], q[8], u[8];
+      load8(reinterpret_cast<const X*>(a.dy) + rc * a.dy_row, at, L, vec, u);
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] = u[e] + st[3] * (d[v][e] - s2 - y[v][e] * s1);        // d y
+      if (write) store8(reinterpret_cast<X*>(a.dx) + rc * a.dx_row, at, W, vec, u);
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = q[e] = 1.f;
+      if (a.gate_kind) load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, vec, p);
+      if (a.scale) load8(a.scale, at, W, vec, q);
+      float k[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float um = u[e] * g[v][e];
+        cs[v][e] = __builtin_fmaf(um, p[e], cs[v][e]);
+        k[e] = um * q[e];                                            // d gate
+        cg[v][e] += k[e];
+        u[e] *= p[e] * q[e];                                         // d m
+        bp[v][e] += u[e];
+        cp[v][e] = __builtin_fmaf(u[e], f[v][e], cp[v][e]);
+      }
+      if (a.gate_kind == 1 && there) store8(reinterpret_cast<F*>(a.dgate) + rc * a.dg_row, at, W, vec, k);
+      load8(a.w_post, at, W, vec, p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        d[v][e] = u[e] * p[e];
+        t1 = __builtin_fmaf(d[v][e], f[v][e], t1);
+        t2 += d[v][e];
+      }
+    }
+    row_sum2<G>(t1, t2, lds, slot, group * G, wave);
+    t1 *= inv_w;
+    t2 = a.layer ? t2 * inv_w : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) d[v][e] = st[1] * (d[v][e] - t2 - f[v][e] * t1);
+      if (write) store8(reinterpret_cast<F*>(a.df) + rc * a.df_row, (gl + v * G * 64) * 8, W, vec, d[v]);
+    }
+  }
+  if (unit >= a.units) return;
+  float* parts = a.parts + (size_t)unit * a.n_parts * W;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int at = (gl + v * G * 64) * 8;
+    float* p = parts;
+    store8(p, at, W, vec, cp[v]);
+    store8(p += W, at, W, vec, cq[v]);
+    if (a.scale) store8(p += W, at, W, vec, cs[v]);
+    if (a.b_post) store8(p += W, at, W, vec, bp[v]);
+    if (a.b_pre) store8(p += W, at, W, vec, bq[v]);
+    if (a.gate_kind == 2 && first < a.rows && seq < a.n_seq) store8(gate_parts + (size_t)(unit + seq) * W, at, W, vec, cg[v]);
+  }
+}
+
+// the units' parts of the parameters' gradients added in order: 16 values and 64 rows of units to a workgroup
+struct SumArgs {
+  const float* parts;
+  float* out[5];
+  int units, n_parts, width;
+};
+__global__ __launch_bounds__(1024) void gated_norm_sum_kernel(const SumArgs a) {
+  __shared__ float sums[1024];
+  const int t = threadIdx.x, n = a.n_parts * a.width, c = blockIdx.x * 16 + (t & 15);
+  float u = 0.f;
+  if (c < n)
+    for (int i = t >> 4; i < a.units; i += 64) u += a.parts[(size_t)i * n + c];
+  sums[t] = u;
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if ((t >> 4) < o) sums[t] += sums[t + 16 * o];
+    __syncthreads();
+  }
+  if (t < 16 && c < n) {
+    const int part = c / a.width;
+    a.out[part][c - part * a.width] = sums[t];
+  }
+}
+// a sequence's gate: the parts of the units that have rows of it
+template <typename F>
+__global__ __launch_bounds__(256) void gated_norm_gate_kernel(const NormArgs a) {
+  const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+  if (c >= a.width) return;
+  const int start = clamp_row(a.cu, b, a.rows), end = clamp_row(a.cu, b + 1, a.rows);
+  const float* parts = a.parts + (size_t)a.units * a.n_parts * a.width;
+  float u = 0.f;
+  if (end > start)
+    for (int i = start / a.per; i <= (end - 1) / a.per; i++) u += parts[(size_t)(i + b) * a.width + c];
+  reinterpret_cast<F*>(a.dgate)[(long long)b * a.dg_row + c] = (F)u;
+}
+
+constexpr int kMaxWidth = 8192;
+bool aligned(const void* p, long long row, int es) { return !p || ((unsigned long long)p % 16 == 0 && (row * es) % 16 == 0); }
+
+template <typename X, typename F, bool BWD, int G, int V>
+int launch_gv(const NormArgs& a, bool vec, hipStream_t st) {
+  const int rows = BWD ? a.units : a.rows;
+  const dim3 grid((unsigned)((rows + Block<G>::kRows - 1) / Block<G>::kRows)), block(Block<G>::kThreads);
+  if constexpr (BWD) hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V>), grid, block, 0, st, a, vec);
+  else hipLaunchKernelGGL((gated_norm_fwd_kernel<X, F, G, V>), grid, block, 0, st, a, vec);
+  AIT_CHECK_LAUNCH();
+  return AIT_OK;
+}
+template <typename X, typename F, bool BWD>
+int launch_xf(const NormArgs& a, bool vec, hipStream_t st) {
+  if (a.width <= 512) return launch_gv<X, F, BWD, 1, 1>(a, vec, st);
+  if (a.width <= 1024) return launch_gv<X, F, BWD, 2, 1>(a, vec, st);
+  if (a.width <= 2048) return launch_gv<X, F, BWD, 4, 1>(a, vec, st);
+  if (a.width <= 4096) return launch_gv<X, F, BWD, 8, 1>(a, vec, st);
+  return launch_gv<X, F, BWD, 8, 2>(a, vec, st);
+}
+template <bool BWD>
+int launch(const ait_gated_norm& p, const NormArgs& a, bool vec, hipStream_t st) {
+  if (p.dtype_x == AIT_DTYPE_BF16) return launch_xf<__bf16, __bf16, BWD>(a, vec, st);
+  if (p.dtype_f == AIT_DTYPE_BF16) return launch_xf<float, __bf16, BWD>(a, vec, st);
+  return launch_xf<float, float, BWD>(a, vec, st);
+}
+
+int check(const ait_gated_norm* p) {
+  if (!p || p->rows < 0 || p->width <= 0 || p->n_seq < 0 || !(p->eps >= 0.f)) return AIT_EINVAL;
+  if ((p->dtype_x != AIT_DTYPE_F32 && p->dtype_x != AIT_DTYPE_BF16) || (p->dtype_f != AIT_DTYPE_F32 && p->dtype_f != AIT_DTYPE_BF16)) return AIT_EINVAL;
+  if (p->width > kMaxWidth || (p->dtype_x == AIT_DTYPE_BF16 && p->dtype_f == AIT_DTYPE_F32)) return AIT_EUNSUPPORTED;
+  if ((long long)p->rows + 4096 >= (1ll << 31)) return AIT_EUNSUPPORTED;
+  if (!p->w_post || !p->w_pre) return AIT_EINVAL;
+  if (p->rows > 0 && (!p->x || !p->f)) return AIT_EINVAL;
+  if (p->x_row < 0 || p->f_row < 0 || p->gate_row < 0) return AIT_EINVAL;
+  if (p->cu_seqlens && !p->gate) return AIT_EINVAL;
+  return AIT_OK;
+}
+NormArgs args_of(const ait_gated_norm& p) {
+  NormArgs a{};
+  a.x = p.x; a.f = p.f; a.gate = p.gate;
+  a.w_post = p.w_post; a.b_post = p.b_post; a.w_pre = p.w_pre; a.b_pre = p.b_pre; a.scale = p.scale;
+  a.cu = p.cu_seqlens;
+  a.x_row = p.x_row; a.f_row = p.f_row; a.g_row = p.gate_row;
+  a.rows = p.rows; a.width = p.width; a.layer = p.layer; a.gate_kind = p.gate ? (p.cu_seqlens ? 2 : 1) : 0; a.n_seq = p.n_seq;
+  a.eps = p.eps; a.zero_rest = p.zero_rest;
+  return a;
+}
+bool inputs_aligned(const ait_gated_norm& p) {
+  const int xs = p.dtype_x == AIT_DTYPE_F32 ? 4 : 2, fs = p.dtype_f == AIT_DTYPE_F32 ? 4 : 2;
+  return p.width % 8 == 0 && aligned(p.x, p.x_row, xs) && aligned(p.f, p.f_row, fs) && aligned(p.gate, p.gate_row, fs) &&
+         aligned(p.w_post, 0, 4) && aligned(p.b_post, 0, 4) && aligned(p.w_pre, 0, 4) && aligned(p.b_pre, 0, 4) && aligned(p.scale, 0, 4);
+}
+// units of the backward: about two workgroups' groups a CU, each with a run of rows
+void units_of(const ait_gated_norm& p, int& units, int& per) {
+  const int groups = p.width <= 512 ? 2048 : p.width <= 1024 ? 1024 : p.width <= 2048 ? 512 : 256;
+  per = p.rows > 0 ? (p.rows + groups - 1) / groups : 1;
+  units = (p.rows + per - 1) / per;
+}
+int parts_of(const ait_gated_norm& p) { return 2 + (p.scale ? 1 : 0) + (p.b_post ? 1 : 0) + (p.b_pre ? 1 : 0); }
+}  // namespace
+
+AIT_API int ait_gated_norm_fwd(const ait_gated_norm* p, void* y, long long y_row, void* h, long long h_row, float* stats, void* stream) {
+  AIT_TRY_RC(check(p));
+  if (p->rows == 0) return AIT_OK;
+  if (!y || !h || y_row < p->width || h_row < p->width || (unsigned long long)stats % 16) return AIT_EINVAL;
+  NormArgs a = args_of(*p);
+  a.y = y; a.h = h; a.y_row = y_row; a.h_row = h_row; a.stats = stats;
+  const bool vec = inputs_aligned(*p) && aligned(y, y_row, p->dtype_x == AIT_DTYPE_F32 ? 4 : 2) && aligned(h, h_row, p->dtype_f == AIT_DTYPE_F32 ? 4 : 2);
+  return launch<false>(*p, a, vec, ait_stream(stream));
+}
+
+AIT_API size_t ait_gated_norm_bwd_workspace_bytes(const ait_gated_norm* p) {
+  if (check(p) != AIT_OK) return 0;
+  int units, per;
+  units_of(*p, units, per);
+  return ((size_t)units * parts_of(*p) + (p->cu_seqlens ? (size_t)units + p->n_seq : 0)) * p->width * sizeof(float);
+}
+
+AIT_API int ait_gated_norm_bwd(const ait_gated_norm* p, const float* stats, const void* dy, long long dy_row, const void* dh, long long dh_row,
+                               void* dx, long long dx_row, void* df, long long df_row, void* d_gate, long long dg_row, float* d_w_post,
+                               float* d_w_pre, float* d_scale, float* d_b_post, float* d_b_pre, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  AIT_TRY_RC(check(p));
+  if (!d_w_post || !d_w_pre || (p->scale && !d_scale) || (p->b_post && !d_b_post) || (p->b_pre && !d_b_pre)) return AIT_EINVAL;
+  if (p->gate && (p->rows > 0 || p->cu_seqlens) && (!d_gate || dg_row < p->width)) return AIT_EINVAL;
+  if (p->rows > 0 && (!stats || (unsigned long long)stats % 16 || !dy || !dh || !dx || !df || dx_row < p->width || df_row < p->width || dy_row < 0 || dh_row < 0))
+    return AIT_EINVAL;
+  const size_t need = ait_gated_norm_bwd_workspace_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return AIT_EWORKSPACE;
+  if ((unsigned long long)workspace % 16) return AIT_EINVAL;
+  NormArgs a = args_of(*p);
+  a.stats = const_cast<float*>(stats);
+  a.dy = dy; a.dh = dh; a.dx = dx; a.df = df; a.dgate = d_gate;
+  a.dy_row = dy_row; a.dh_row = dh_row; a.dx_row = dx_row; a.df_row = df_row; a.dg_row = dg_row;
+  units_of(*p, a.units, a.per);
+  a.n_parts = parts_of(*p);
+  a.parts = static_cast<float*>(workspace);
+  const hipStream_t st = ait_stream(stream);
+  const int xs = p->dtype_x == AIT_DTYPE_F32 ? 4 : 2, fs = p->dtype_f == AIT_DTYPE_F32 ? 4 : 2;
+  const bool vec = inputs_aligned(*p) && aligned(dy, dy_row, xs) && aligned(dh, dh_row, fs) && aligned(dx, dx_row, xs) && aligned(df, df_row, fs) &&
+                   aligned(d_gate, dg_row, fs);
+  if (p->rows > 0) AIT_TRY_RC(launch<true>(*p, a, vec, st));
+  SumArgs s{a.parts, {d_w_post, d_w_pre, nullptr, nullptr, nullptr}, a.units, a.n_parts, p->width};
+  int n = 2;
+  if (p->scale) s.out[n++] = d_scale;
+  if (p->b_post) s.out[n++] = d_b_post;
+  if (p->b_pre) s.out[n++] = d_b_pre;
+  hipLaunchKernelGGL(gated_norm_sum_kernel, dim3((unsigned)((a.n_parts * p->width + 15) / 16)), dim3(1024), 0, st, s);
+  AIT_CHECK_LAUNCH();
+  if (a.gate_kind == 2 && p->n_seq > 0) {
+    const dim3 grid((unsigned)((p->width + 255) / 256), (unsigned)p->n_seq);
+    if (p->dtype_f == AIT_DTYPE_F32) hipLaunchKernelGGL(gated_norm_gate_kernel<float>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(gated_norm_gate_kernel<__bf16>, grid, dim3(256), 0, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  return AIT_OK;
+}

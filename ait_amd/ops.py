@@ -894,3 +894,88 @@ def packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=False):
                                    _lib.cur_stream(dev))
     _lib.check(rc, "ait_packed_attn_bwd")
     return dq, dk, dv, dt
+
+
+def _rows2d(t):
+    """t [rows, width] with unit element stride, or a copy that has it"""
+    return t if t.stride(1) == 1 and t.stride(0) >= 0 or t.numel() == 0 else t.contiguous()
+
+
+def gated_norm_desc(x, f, w_post, w_pre, b_post=None, b_pre=None, gate=None, scale=None, layer=False, eps=1e-6, cu_seqlens=None):
+    """checks the arguments and returns (ait_gated_norm, the tensors it points at).  x, f [rows, width]"""
+    def need(ok, what):
+        if not ok:
+            raise _lib.AitHipError("gated_norm: " + what)
+    for n, t in (("x", x), ("f", f)):
+        need(torch.is_tensor(t) and t.dim() == 2 and t.dtype in _lib.DTYPES, "`%s` must be a float32 or bfloat16 [rows, width] tensor" % n)
+    need(x.shape == f.shape and x.device == f.device, "x and f must have one shape and device (got %s, %s)" % (tuple(x.shape), tuple(f.shape)))
+    need(not (x.dtype == torch.bfloat16 and f.dtype == torch.float32), "a bfloat16 stream takes a bfloat16 branch")
+    rows, W = x.shape
+    dev = x.device
+    need(0 < W <= _lib.MAX_NORM_WIDTH, "width %d: 1 to %d expected" % (W, _lib.MAX_NORM_WIDTH))
+    need(rows < 2 ** 31 - 4096, "row counts must fit 31 bits")
+    par = []
+    for n, t in (("post_weight", w_post), ("post_bias", b_post), ("pre_weight", w_pre), ("pre_bias", b_pre), ("scale", scale)):
+        need(t is not None or n in ("post_bias", "pre_bias", "scale"), "`%s` is missing" % n)
+        need(t is None or (torch.is_tensor(t) and t.dtype == torch.float32 and tuple(t.shape) == (W,) and t.device == dev),
+             "`%s` must be a float32 [%d] tensor on %s" % (n, W, dev))
+        par.append(None if t is None else t.contiguous())
+    n_seq = 0
+    need(cu_seqlens is None or gate is not None, "`cu_seqlens` says whose gate a row takes: there is no gate")
+    if gate is not None:
+        if cu_seqlens is not None:
+            need(torch.is_tensor(cu_seqlens) and cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() > 0
+                 and cu_seqlens.device == dev, "`cu_seqlens` must be an int32 tensor on %s" % dev)
+            n_seq, cu_seqlens = cu_seqlens.numel() - 1, cu_seqlens.contiguous()
+        need(torch.is_tensor(gate) and gate.dtype == f.dtype and gate.device == dev
+             and tuple(gate.shape) == ((rows if cu_seqlens is None else n_seq), W),
+             "the gate must be a %s [%d, %d] tensor on %s" % (f.dtype, rows if cu_seqlens is None else n_seq, W, dev))
+        gate = _rows2d(gate)
+    if not x.is_cuda:
+        raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % dev)
+    x, f = _rows2d(x), _rows2d(f)
+    p = _lib.GatedNorm()
+    ptr = lambda t: None if t is None else t.data_ptr()
+    p.x, p.f, p.gate, p.cu_seqlens, p.x_row, p.f_row = ptr(x), ptr(f), ptr(gate), ptr(cu_seqlens), x.stride(0), f.stride(0)
+    p.gate_row = 0 if gate is None else gate.stride(0)
+    p.w_post, p.b_post, p.w_pre, p.b_pre, p.scale = (ptr(t) for t in par)
+    p.rows, p.width, p.n_seq, p.dtype_x, p.dtype_f, p.layer, p.zero_rest, p.eps = rows, W, n_seq, _lib.DTYPES[x.dtype], _lib.DTYPES[f.dtype], \
+        int(bool(layer)), 1, float(eps)
+    if gate is not None and gate.numel() == 0 and p.gate is None:
+        p.gate = p.w_post            # (an empty gate is still a gate; nothing reads it)
+    return p, (x, f, gate, cu_seqlens, *par)
+
+
+def gated_norm_fwd(p, x, f, want_stats=False):
+    """ait_gated_norm_fwd: y as x, h as f, stats [rows, 4] or None"""
+    dev = x.device
+    y, h = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(f.shape, dtype=f.dtype, device=dev)
+    stats = torch.empty((p.rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+    with torch.cuda.device(dev):
+        rc = _lib.lib().ait_gated_norm_fwd(ctypes.byref(p), ctypes.c_void_p(y.data_ptr()), p.width, ctypes.c_void_p(h.data_ptr()), p.width,
+                                           _p(stats), _lib.cur_stream(dev))
+    _lib.check(rc, "ait_gated_norm_fwd")
+    return y, h, stats
+
+
+def gated_norm_bwd(p, x, f, gate, stats, dy, dh):
+    """ait_gated_norm_bwd: dx, df, d gate, and the f32 gradients of post_weight, post_bias, pre_weight, pre_bias, scale (None where
+    there is none)"""
+    L = _lib.lib()
+    dev = x.device
+    dy, dh = _rows2d(dy), _rows2d(dh)
+    e = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+    dx, df, dg = e(x), e(f), e(gate)
+    n = 2 + sum(t is not None for t in (p.scale, p.b_post, p.b_pre))
+    flat = torch.empty((n, p.width), dtype=torch.float32, device=dev)
+    it = iter(flat)
+    dwp, dwq = next(it), next(it)
+    ds, dbp, dbq = (next(it) if t is not None else None for t in (p.scale, p.b_post, p.b_pre))
+    vp = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+    with torch.cuda.device(dev):
+        nb = L.ait_gated_norm_bwd_workspace_bytes(ctypes.byref(p))
+        ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
+        rc = L.ait_gated_norm_bwd(ctypes.byref(p), vp(stats), vp(dy), dy.stride(0), vp(dh), dh.stride(0), vp(dx), p.width, vp(df), p.width,
+                                  vp(dg), p.width, vp(dwp), vp(dwq), vp(ds), vp(dbp), vp(dbq), vp(ws), ws.numel(), _lib.cur_stream(dev))
+    _lib.check(rc, "ait_gated_norm_bwd")
+    return dx, df, dg, dwp, dbp, dwq, dbq, ds

@@ -3,9 +3,11 @@
 
     packed_attention(q, k, v, cu_q, cu_k)                 any lengths, grouped heads, causal or not, caches for new tokens
     relative_buckets / RelativePositionBias               a learned bias of its scores by buckets of the relative position
+    gated_norm(x, f, post_weight=..., pre_weight=...)     the norms behind and before a block, its gate and residual scale
 
 The general-length counterparts of the 64-token blocks in ait_amd/system.py (ScaledDotProductAttention,
-lib/model/system/Modules.py:16-29; the sinusoid table of PositionalEncoding, lib/model/system/Models.py:26-50).  float32 or
+lib/model/system/Modules.py:16-29; the sinusoid table of PositionalEncoding, lib/model/system/Models.py:26-50; the residual and
+LayerNorm behind a sub-layer, lib/model/system/SubLayers.py:98-100).  float32 or
 bfloat16 tensors on a GPU; there is no CPU path.  The kernels run on the current stream of the tensors' device, take their
 scratch from torch's allocator per call and may be captured into a graph.
 """
@@ -94,3 +96,57 @@ class RelativePositionBias(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.zeros(n_buckets, n_head))
         self.register_buffer("bucket_of", relative_buckets(n_buckets, max_distance, two_sided), persistent=False)
+
+
+class _GatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, gate, w_post, b_post, w_pre, b_pre, scale, cu_seqlens, layer, eps):
+        f32 = lambda t: None if t is None else t.float()
+        p, keep = ops.gated_norm_desc(x, f, f32(w_post), f32(w_pre), f32(b_post), f32(b_pre), gate, f32(scale), layer, eps, cu_seqlens)
+        grad = any(ctx.needs_input_grad[:8])
+        y, h, stats = ops.gated_norm_fwd(p, x, f, want_stats=grad)
+        if grad:
+            ctx.save_for_backward(stats, *[t for t in keep if t is not None])
+            ctx.there = [t is not None for t in keep]
+            ctx.cfg = (layer, eps, [None if t is None else t.dtype for t in (w_post, b_post, w_pre, b_pre, scale)])
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        stats, *keep = ctx.saved_tensors
+        x, f, gate, cu_seqlens, w_post, b_post, w_pre, b_pre, scale = [keep.pop(0) if t else None for t in ctx.there]
+        layer, eps, types = ctx.cfg
+        p, _keep = ops.gated_norm_desc(x, f, w_post, w_pre, b_post, b_pre, gate, scale, layer, eps, cu_seqlens)
+        dx, df, dg, *par = ops.gated_norm_bwd(p, x, f, gate, stats, dy, dh)
+        grads = [dx, df, dg] + [None if t is None else t.to(dt) for t, dt in zip(par, types)]
+        return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None, None, None)
+
+
+def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, gate=None, scale=None, kind="rms", eps=1e-6, cu_seqlens=None):
+    """The norm behind a block and the one before the next, with what is between them, in one pass over the rows -> (y, h):
+
+        m = norm(f) * post_weight (+ post_bias);   y = x + scale * gate * m;   h = norm(y) * pre_weight (+ pre_bias)
+
+    x [..., width] the residual stream, f the block's output: both float32, both bfloat16, or a float32 stream with a bfloat16
+    branch; y is of x's type, h of f's.  kind: "rms" (by the root of the mean square) or "layer" (about the mean).  gate: None,
+    one of f's shape and type, or with cu_seqlens (int32 [n_seq + 1], the first 0, not descending) one row per sequence of the
+    packed rows of a two-dimensional x; rows behind the last sequence then give zeros.  scale: None or [width], the learned
+    factor of the branch.  Parameters are float32 or bfloat16 [width]; sums, statistics and the row between the two norms are
+    f32.  width up to 8192."""
+    if kind not in ("rms", "layer"):
+        raise ValueError("gated_norm: kind must be 'rms' or 'layer'")
+    if not (torch.is_tensor(x) and torch.is_tensor(f) and x.dim() >= 1 and x.shape == f.shape):
+        raise _lib.AitHipError("gated_norm: x and f must be tensors of one shape")
+    if cu_seqlens is not None and x.dim() != 2:
+        raise _lib.AitHipError("gated_norm: with cu_seqlens x must be [rows, width]")
+    for n, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("post_bias", post_bias), ("pre_bias", pre_bias), ("scale", scale)):
+        if t is not None and not (torch.is_tensor(t) and t.dtype in _lib.DTYPES):
+            raise _lib.AitHipError("gated_norm: `%s` must be a float32 or bfloat16 tensor" % n)
+    shape = x.shape
+    if x.dim() != 2:
+        if gate is not None and gate.shape != shape:
+            raise _lib.AitHipError("gated_norm: a gate without cu_seqlens has x's shape")
+        x, f, gate = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, f, gate))
+    y, h = _GatedNorm.apply(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale, cu_seqlens, kind == "layer", eps)
+    return y.view(shape), h.view(shape)

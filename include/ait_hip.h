@@ -924,6 +924,41 @@ int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row
                         long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
                         long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * The norm behind a block, its gate and residual scale, the residual, and the norm in front of the next block, fused: the rows
+ * of any width beside ait_ln_fwd's LayerNorm(dropout(a) + residual) of 512 values (lib/model/system/SubLayers.py:98-100,184-186).
+ *     m = norm(f) w_post (+ b_post) ;  y = x + scale * gate * m ;  h = norm(y) w_pre (+ b_pre)
+ *     layer != 0: norm(t) = (t - mean t) / sqrt(var t + eps), var about the mean; layer == 0: t / sqrt(mean t^2 + eps)
+ *   x [rows, width] of dtype_x (pitch x_row elements), f of dtype_f; (AIT_DTYPE_F32, F32), (F32, BF16) and (BF16, BF16).
+ *     y as x, h as f.  width up to 8192; rows of whole 16-byte vectors (width, pitches, bases) take wide loads, others single ones.
+ *   gate NULL, [rows, width] of dtype_f, or with cu_seqlens int32 [n_seq + 1] (ascending from 0) [n_seq, width]: row r's is that
+ *     of its sequence; rows behind the last sequence are not read, and what belongs to them is left as it is (zero_rest: zeroed).
+ *   scale, b_post, b_pre: NULL or f32 [width]; w_post, w_pre f32 [width].
+ *   stats f32 [rows, 4] (16-byte base): what the backward reads; NULL in inference.
+ * h is formed from y before its rounding to dtype_x, and so is the backward.  Backward: gradients of everything given (of y and
+ * h: dy, dh), f32 for the parameters (overwritten).  No atomics: results are the same from run to run.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* x;
+  const void* f;
+  const void* gate;
+  const int32_t* cu_seqlens;
+  const float* w_post;
+  const float* b_post;
+  const float* w_pre;
+  const float* b_pre;
+  const float* scale;
+  long long x_row, f_row, gate_row;
+  int rows, width, n_seq, dtype_x, dtype_f, layer, zero_rest;
+  float eps;
+} ait_gated_norm;
+int ait_gated_norm_fwd(const ait_gated_norm* p, void* y, long long y_row, void* h, long long h_row, float* stats, void* stream);
+size_t ait_gated_norm_bwd_workspace_bytes(const ait_gated_norm* p);
+int ait_gated_norm_bwd(const ait_gated_norm* p, const float* stats, const void* dy, long long dy_row, const void* dh, long long dh_row,
+                       void* dx, long long dx_row, void* df, long long df_row, void* d_gate, long long dg_row, float* d_w_post,
+                       float* d_w_pre, float* d_scale, float* d_b_post, float* d_b_pre, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

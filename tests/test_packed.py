@@ -267,3 +267,157 @@ def test_c_entries_refuse_bad_arguments():
     p = dict(n_seq=2, total_q=2, total_k=20000, max_q=1, max_k=10000)
     need = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(_lib.PackedAttn(**{**base, **p})))
     assert need > 0 and fwd(**p) == EWORKSPACE
+
+
+# ------------------------------------------------------------------------------------------
+# gated norm: reference and bounds
+# ------------------------------------------------------------------------------------------
+def norm_ref(x, f, post, pre, post_b, pre_b, gate, scale, layer, eps, cu, dy, dh):
+    """[(value, bound)] of y, h, dx, df, post, post_b, pre, pre_b, gate, scale gradients in 64 bits (None where there is none);
+    rows of no sequence are not part of it.  Sums of a row are trees of at most 40 terms' depth (32 values a lane, 6 steps in a
+    wave, 8 waves), columns' are as deep as there are rows."""
+    ux, uf, e1 = torch.finfo(x.dtype).eps / 2, torch.finfo(f.dtype).eps / 2, 2.0 ** -24
+    c = lambda t: None if t is None else t.detach().cpu().to(F8)
+    x, f, post, pre, post_b, pre_b, gate, scale, dy, dh = (c(t) for t in (x, f, post, pre, post_b, pre_b, gate, scale, dy, dh))
+    n = x.shape[0] if cu is None else int(cu[-1])
+    x, f, dy, dh = x[:n], f[:n], dy[:n], dh[:n]
+    mean = lambda t: t.mean(1, keepdim=True)
+    seq = None if cu is None else torch.repeat_interleave(torch.arange(len(cu) - 1), torch.tensor([int(b - a) for a, b in zip(cu[:-1], cu[1:])]))
+    G = torch.ones_like(x) if gate is None else gate if cu is None else gate[seq]
+    S = torch.ones(x.shape[1], dtype=F8) if scale is None else scale
+    D = 48 * e1
+
+    def hat(t, et):
+        tc = t - mean(t) if layer else t
+        r = (mean(tc * tc) + eps) ** -0.5
+        ec = et + (mean(et) + D * mean(t.abs()) if layer else 0) + e1 * t.abs()
+        th = tc * r
+        rr = mean(th.abs() * r * ec) * 1.01 + D                      # relative error of r
+        return th, r, r * ec + th.abs() * rr * 1.01 + e1 * th.abs(), rr
+
+    def back(d, th, eth, r, rr, ed):
+        s1, s2 = mean(d * th), (mean(d) if layer else torch.zeros_like(mean(d)))
+        es1 = mean(d.abs() * eth + ed * th.abs()) * 1.01 + D * mean((d * th).abs())
+        es2 = (mean(ed) + D * mean(d.abs())) if layer else 0
+        out = r * (d - s2 - th * s1)
+        return out, r * (ed + 4 * e1 * (d.abs() + s2.abs() + (th * s1).abs()) + es2 + th.abs() * es1 + eth * s1.abs()) * 1.01 + out.abs() * rr * 1.01
+
+    zero = torch.zeros_like(x)
+    fh, fr, efh, frr = hat(f, zero)
+    b = 0 if post_b is None else post_b
+    m = fh * post + b
+    em = efh * post.abs() + 4 * e1 * ((fh * post).abs() + (0 if post_b is None else post_b.abs()))
+    sg = S * G
+    y = x + sg * m
+    ey = sg.abs() * em + 6 * e1 * (x.abs() + (sg * m).abs())
+    yh, yr, eyh, yrr = hat(y, ey)
+    h = yh * pre + (0 if pre_b is None else pre_b)
+    eh = eyh * pre.abs() + 4 * e1 * ((yh * pre).abs() + (0 if pre_b is None else pre_b.abs()))
+    rnd = lambda t, e, u: (t, e + u * (t.abs() + e))
+    d = dh * pre
+    bk, ebk = back(d, yh, eyh, yr, yrr, e1 * d.abs())
+    t = dy + bk
+    et = ebk + 2 * e1 * (dy.abs() + bk.abs())
+    dm, edm = t * sg, sg.abs() * et + 4 * e1 * (t * sg).abs()
+    df, edf = back(dm * post, fh, efh, fr, frr, edm * post.abs() + e1 * (dm * post).abs())
+    N = (n + 80) * e1
+    col = lambda v, e: (v.sum(0), (e + N * v.abs()).sum(0))
+    out = dict(y=rnd(y, ey, ux), h=rnd(h, eh, uf), x=rnd(t, et, ux), f=rnd(df, edf, uf),
+               post=col(dm * fh, edm * fh.abs() + dm.abs() * efh), pre=col(dh * yh, dh.abs() * eyh))
+    if post_b is not None:
+        out["post_b"] = col(dm, edm)
+    if pre_b is not None:
+        out["pre_b"] = col(dh, 0 * dh)
+    k = t * G * m
+    if scale is not None:
+        out["scale"] = col(k, (et * m.abs() + t.abs() * em) * G.abs() + 4 * e1 * k.abs())
+    if gate is not None:
+        k = t * S * m
+        ek = (et * m.abs() + t.abs() * em) * S.abs() + 4 * e1 * k.abs()
+        if cu is not None:
+            z = torch.zeros(gate.shape, dtype=F8)
+            k, ek = z.index_add(0, seq, k), z.index_add(0, seq, ek + N * k.abs())
+        out["gate"] = rnd(k, ek, uf)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [("float32", "float32"), ("float32", "bfloat16"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("rows,width,kind,gate,scale,odd", [
+    (1, 8, "rms", "row", True, False), (37, 512, "layer", "none", True, False), (300, 512, "rms", "sequence", True, False), (5, 17, "layer", "row", False, False),
+    (64, 513, "layer", "sequence", True, False), (130, 1024, "rms", "row", True, True), (9, 2048, "layer", "sequence", False, False),
+    (21, 4096, "rms", "sequence", True, True), (17, 8192, "layer", "row", True, False), (600, 100, "layer", "sequence", True, False), (3, 5120, "rms", "none", False, False),
+    (2100, 40, "layer", "sequence", True, True), (5, 1, "rms", "row", True, False)])
+def test_gated_norm(types, rows, width, kind, gate, scale, odd):
+    xt, ft = (getattr(torch, t) for t in types)
+    g = torch.Generator().manual_seed(rows + width)
+    r = lambda *s: torch.randn(*s, generator=g)
+    def rowed(t, dt):          # odd: rows of a wider matrix
+        if not odd:
+            return t.to(dt).cuda()
+        w = torch.full((t.shape[0], t.shape[1] + 24), float("nan"), dtype=dt, device="cuda")
+        w[:, 8:8 + t.shape[1]] = t.to(dt)
+        return w[:, 8:8 + t.shape[1]]
+    x, f = rowed(r(rows, width) * 2, xt), rowed(r(rows, width) + 0.5, ft)
+    cu, n = None, rows
+    if gate == "sequence":
+        cut = [0, rows // 3, rows // 3, rows // 3 + 1 if rows > 3 else rows // 3, rows // 2, rows - rows // 10]
+        cu, n = torch.tensor(cut, dtype=torch.int32).cuda(), cut[-1]
+        x[n:], f[n:] = float("nan"), float("inf")
+    gt = None if gate == "none" else rowed(torch.sigmoid(r(rows if gate == "row" else 5, width)), ft)
+    par = {k: (1 if k in ("post", "pre") else 0.2) + 0.3 * r(width).cuda() for k in ("post", "pre", "scale", "post_b", "pre_b")}
+    if not scale:
+        par["scale"] = None
+    if kind == "rms":
+        par["post_b"] = par["pre_b"] = None
+    leaves = {k: t.detach().requires_grad_(True) for k, t in dict(x=x, f=f, gate=gt, **par).items() if t is not None}
+    L = leaves.get
+    dy, dh = rowed(r(rows, width), xt), rowed(r(rows, width), ft)
+    y, h = packed.gated_norm(L("x"), L("f"), post_weight=L("post"), pre_weight=L("pre"), post_bias=L("post_b"), pre_bias=L("pre_b"), gate=L("gate"),
+                             scale=L("scale"), kind=kind, eps=1e-5, cu_seqlens=cu)
+    names = list(leaves)
+    got = dict(zip(names, torch.autograd.grad([y, h], [leaves[k] for k in names], [dy, dh])), y=y, h=h)
+    want = norm_ref(x, f, par["post"], par["pre"], par["post_b"], par["pre_b"], gt, par["scale"], kind == "layer", 1e-5,
+                    None if cu is None else cu.tolist(), dy, dh)
+    assert set(want) == set(got)
+    for k, w in want.items():
+        t = got[k]
+        if k in ("x", "f", "y", "h"):
+            assert bool((t[n:] == 0).all()), k + ": rows behind the last sequence"
+            t = t[:n]
+        within(t, w, k)
+
+
+def test_gated_norm_refuses_what_it_does_not_take():
+    t = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt)
+    good = dict(x=t(6, 32), f=t(6, 32), post_weight=t(32), pre_weight=t(32))
+
+    def call(**kw):
+        a = {**good, **kw}
+        return packed.gated_norm(a.pop("x"), a.pop("f"), **a)
+    with pytest.raises(_lib.AitHipError, match="no CPU fallback"):
+        call()
+    cu = starts([2, 4])
+    for change in (dict(x=t(6, 31)), dict(x=t(6, 32, dt=torch.float16), f=t(6, 32, dt=torch.float16)), dict(x=t(6, 32, dt=torch.bfloat16)),
+                   dict(post_weight=t(31)), dict(pre_weight=None), dict(scale=t(6, 32)), dict(gate=t(5, 32)), dict(gate=t(6, 32, dt=torch.bfloat16)),
+                   dict(cu_seqlens=cu), dict(gate=t(6, 32), cu_seqlens=cu), dict(gate=t(2, 32), cu_seqlens=cu.long()), dict(post_bias=t(32).half()),
+                   dict(x=t(6, 8200), f=t(6, 8200), post_weight=t(8200), pre_weight=t(8200)), dict(x=t(2, 3, 32), f=t(2, 3, 32), gate=t(2, 32), cu_seqlens=cu),
+                   dict(x=t(2, 3, 32), f=t(2, 3, 32), gate=t(6, 32))):
+        with pytest.raises(_lib.AitHipError):
+            call(**change)
+            pytest.fail("taken: %s" % list(change))
+    with pytest.raises(ValueError):
+        call(kind="batch")
+    L = _lib.lib()
+    base = dict(x=4096, f=4096, w_post=4096, w_pre=4096, x_row=32, f_row=32, rows=6, width=32, dtype_x=0, dtype_f=0, eps=1e-6)
+    fwd = lambda y=4096, yr=32, **kw: L.ait_gated_norm_fwd(ctypes.byref(_lib.GatedNorm(**{**base, **kw})), y, yr, 4096, 32, None, None)
+    bwd = lambda ws=4096, n=1 << 30, dg=None, **kw: L.ait_gated_norm_bwd(
+        ctypes.byref(_lib.GatedNorm(**{**base, **kw})), 4096, *(4096, 32) * 4, dg, 32, 4096, 4096, None, None, None, ws, n, None)
+    for f in (fwd, bwd):
+        for kw in (dict(rows=-1), dict(width=0), dict(dtype_x=2), dict(dtype_f=-1), dict(w_post=None), dict(w_pre=None), dict(x=None), dict(f=None),
+                   dict(eps=-1.0), dict(cu_seqlens=4096), dict(x_row=-1), dict(n_seq=-1)):
+            assert f(**kw) == -1, kw
+        for kw in (dict(width=8193), dict(dtype_x=1, dtype_f=0)):
+            assert f(**kw) == -4, kw
+    assert fwd(y=None) == -1 and fwd(yr=31) == -1
+    assert bwd(ws=None) == -2 and bwd(n=64) == -2 and bwd(scale=4096) == -1 and bwd(gate=4096, gate_row=32) == -1
