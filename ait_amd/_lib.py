@@ -124,12 +124,12 @@ SIGNATURES = {
     "ait_attn_bwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _ull, _vp, _i,
                           _vp, _i, _vp, _i, _vp]),
     "ait_packed_attn_fwd_workspace_bytes": (_sz, [_vp]),
-    "ait_packed_attn_fwd": (_i, [_vp] + [_vp, _ll, _ll] * 4 + [_vp, _vp, _sz, _vp]),
+    "ait_packed_attn_fwd": (_i, [_vp] + [_vp, _ll, _ll] * 4 + [_vp, _vp, _vp, _sz, _vp]),
     "ait_gated_norm_fwd": (_i, [_vp, _vp, _ll, _vp, _ll, _vp, _vp]),
     "ait_gated_norm_bwd_workspace_bytes": (_sz, [_vp]),
     "ait_gated_norm_bwd": (_i, [_vp, _vp] + [_vp, _ll] * 5 + [_vp] * 6 + [_sz, _vp]),
     "ait_packed_attn_bwd_workspace_bytes": (_sz, [_vp]),
-    "ait_packed_attn_bwd": (_i, [_vp] + [_vp, _ll, _ll] * 5 + [_vp] + [_vp, _ll, _ll] * 3 + [_vp, _vp, _sz, _vp]),
+    "ait_packed_attn_bwd": (_i, [_vp] + [_vp, _ll, _ll] * 4 + [_vp] + [_vp, _ll, _ll] + [_vp] + [_vp, _ll, _ll] * 3 + [_vp, _vp, _sz, _vp]),
 }
 
 GEMM_RELU, GEMM_ACCUMULATE, GEMM_ATOMIC, GEMM_BIAS_ROW, GEMM_MASK_POS, GEMM_COLSUM = 1, 2, 4, 8, 16, 32
@@ -391,6 +391,28 @@ def dev_ptr(t: torch.Tensor, dtype=torch.float32, dense_any_format=False):
                                       and t.is_contiguous(memory_format=torch.channels_last)):
         raise AitHipError("tensor must be contiguous")
     return ctypes.c_void_p(t.data_ptr())
+
+
+class on_device:
+    """`with torch.cuda.device(dev)` that costs nothing where `dev` is current already"""
+
+    def __init__(self, dev):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def raw_stream(device):
+    """cur_stream's handle as a number, without building a stream object"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def cur_stream(device=None):

@@ -18,7 +18,8 @@ struct FwdArgs {
   const void* k;
   const void* v;
   void* o;
-  float* lse;
+  float* lse;          // [H][total_q] log2 of a row's sum (+infinity where a row sees nothing: its probabilities are zero)
+  void* rest;          // bf16: what rounding took from o, contiguous
   long long qs, qh, ks, kh, vs, vh, os, oh;      // row and head strides in elements
   Seqs s;
   Bias bias;
@@ -27,6 +28,16 @@ struct FwdArgs {
   float* part_o;      // [splits][total_q * H][d] unnormalised, and
   float* part_ml;     // [splits][total_q * H][2] maximum, sum: only where splits > 1
 };
+
+// four values of o; for a backward also what their rounding takes away.  The backward's delta = dO . O is subtracted from
+// scores' gradients of like size, so O's rounding to bf16 would be the largest error of dQ and dK
+template <typename T>
+__device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, int head, int dd, float v0, float v1, float v2, float v3) {
+  store4(p, v0, v1, v2, v3);
+  if constexpr (sizeof(T) == 2)
+    if (a.rest)
+      store4(reinterpret_cast<T*>(a.rest) + (at * a.H + head) * a.d + dd, v0 - (float)(T)v0, v1 - (float)(T)v1, v2 - (float)(T)v2, v3 - (float)(T)v3);
+}
 
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(const FwdArgs a) {
@@ -49,7 +60,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
           store4(p, 0.f, 0.f, 0.f, 0.f);
           store4(p + 4, 0.f, 0.f, 0.f, 0.f);
         }
-      if (n < qlen && h == 0 && a.lse) a.lse[(long long)(head0 + r - n * a.pack) * a.s.total_q + qstart + n] = kNegInf;
+      if (n < qlen && h == 0 && a.lse) a.lse[(long long)(head0 + r - n * a.pack) * a.s.total_q + qstart + n] = -kNegInf;
     }
     return;
   }
@@ -198,14 +209,14 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
       }
   } else {
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);        // (a row that sees nothing: zeros; NaN stays NaN)
-    if (a.lse && h == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    if (a.lse && h == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? -kNegInf : m + __builtin_amdgcn_logf(l);
     T* p = reinterpret_cast<T*>(a.o) + at * a.os + (long long)head * a.oh;
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int dd = 32 * b + 8 * i + 4 * h;
-        if (dd < a.d) store4(p + dd, acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv);
+        if (dd < a.d) store_o<T>(a, p + dd, at, head, dd, acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv);
       }
   }
 }
@@ -233,8 +244,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (a.lse && lane == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
-  if (dd < a.d) store4(reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+  if (a.lse && lane == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? -kNegInf : m + __builtin_amdgcn_logf(l);
+  if (dd < a.d) store_o<T>(a, reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, at, head, dd, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
 }
 
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
@@ -318,17 +329,18 @@ AIT_API size_t ait_packed_attn_fwd_workspace_bytes(const ait_packed_attn* p) {
 
 AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                 long long k_head, const void* v, long long v_row, long long v_head, void* o, long long o_row,
-                                long long o_head, float* lse, void* workspace_ptr, size_t workspace_bytes, void* stream) {
+                                long long o_head, float* lse, void* o_rest, void* workspace_ptr, size_t workspace_bytes, void* stream) {
   AIT_TRY_RC(ait_packed::check(p));
   if (p->n_seq == 0 || p->total_q == 0) return AIT_OK;
   AIT_TRY_RC(ait_packed::check_strides(p, q, q_row, q_head, p->total_q));
   AIT_TRY_RC(ait_packed::check_strides(p, o, o_row, o_head, p->total_q));
   AIT_TRY_RC(ait_packed::check_strides(p, k, k_row, k_head, p->total_k));
   AIT_TRY_RC(ait_packed::check_strides(p, v, v_row, v_head, p->total_k));
+  if ((unsigned long long)o_rest % 16) return AIT_EUNSUPPORTED;
   const Shape sh = shape_of(*p);
   const size_t need = workspace(*p, sh);
   if (need && (!workspace_ptr || workspace_bytes < need)) return AIT_EWORKSPACE;
-  FwdArgs a{q, k, v, o, lse, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
+  FwdArgs a{q, k, v, o, lse, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,

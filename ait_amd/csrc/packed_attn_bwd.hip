@@ -22,7 +22,8 @@ struct BwdArgs {
   const void* v;
   const void* o;
   const void* d_o;
-  const float* lse;
+  const void* rest;   // bf16: what rounding took from o, contiguous; or null
+  const float* lse;   // [H][total_q] log2 of the rows' sums
   void* dq;
   void* dk;
   void* dv;
@@ -31,7 +32,6 @@ struct BwdArgs {
   Bias bias;
   int H, Hk, d, causal, qnumbers, knumbers;
   float scale;
-  float* lse2;        // [H][total_q] log2 of the rows' sums (+infinity where a row sees nothing: its probabilities are zero)
   float* delta;       // [H][total_q]
   float* part_table;  // [qnumbers][H][n_buckets]; null: the table's gradient is not wanted
   float* d_table;
@@ -97,15 +97,18 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
       const Frag<T> of = global_frag<T>(orow, 16 * c + 8 * h, a.d, row < qlen);
 #pragma unroll
       for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)of[e], delta);
+      if constexpr (sizeof(T) == 2) {
+        if (a.rest) {
+          const Frag<T> rf = global_frag<T>(reinterpret_cast<const T*>(a.rest) + (at * a.H + head) * a.d, 16 * c + 8 * h, a.d, row < qlen);
+#pragma unroll
+          for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)rf[e], delta);
+        }
+      }
     }
     delta = column_sum(delta);
-    const float l = a.lse[(long long)head * a.s.total_q + at];
-    l2 = l == kNegInf ? -kNegInf : l * kLog2e;
-    if (row < qlen && h == 0) {
-      a.lse2[(long long)head * a.s.total_q + at] = l2;
-      a.delta[(long long)head * a.s.total_q + at] = delta;
-    }
-    if (row >= qlen || l == kNegInf) { l2 = -kNegInf; delta = 0.f; }
+    l2 = a.lse[(long long)head * a.s.total_q + at];
+    if (row < qlen && h == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
+    if (row >= qlen) l2 = -kNegInf;
   }
   float* bl = reinterpret_cast<float*>(lds + 4 * kTile);                 // the head's bias, then per wave: a block's sums by
   float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kHist + nb);    // relative position, and the sums by bucket
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
   Loader<T, D, NT> lq, lg;
   lq.init(tid, qstr, dby);
   lg.init(tid, gstr, dby);
-  const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse2 | delta of KB rows
+  const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse | delta of KB rows
   auto fetch = [&](int it, int stage) {
     const int g = it / tq, t = t0 + it - g * tq, head = kvh * group + g;
     const long long r = (long long)t * KB;
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
     lg.load(reinterpret_cast<const T*>(a.d_o) + (qstart + r) * a.dos + (long long)head * a.doh, qlen - r, gstr, dby,
             lds0 + stage * 2 * kTile + kTile, wave);
     if (wave < 2) {
-      const float* src = (wave ? a.delta : a.lse2) + (long long)head * a.s.total_q + qstart + r;
+      const float* src = (wave ? a.delta : a.lse) + (long long)head * a.s.total_q + qstart + r;
       const int n = (int)min((long long)KB, qlen - r);
       const i32x4 rsrc = tile_rsrc(src, n * 4);
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
@@ -441,14 +444,14 @@ long long q_numbers(const ait_packed_attn& p) { return block_numbers(p.total_q, 
 
 AIT_API size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p) {
   if (ait_packed::check(p) != AIT_OK) return 0;
-  size_t n = 2 * (size_t)p->heads * p->total_q;
+  size_t n = (size_t)p->heads * p->total_q;
   if (p->bias_table) n += (size_t)q_numbers(*p) * p->heads * p->n_buckets;
   return n * sizeof(float);
 }
 
 AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                 long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
-                                long long o_head, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
+                                long long o_head, const void* o_rest, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
                                 long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
                                 long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream) {
   AIT_TRY_RC(ait_packed::check(p));
@@ -463,16 +466,15 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
   AIT_TRY_RC(ait_packed::check_strides(p, dk, dk_row, dk_head, p->total_k));
   AIT_TRY_RC(ait_packed::check_strides(p, dv, dv_row, dv_head, p->total_k));
   if (p->total_q > 0 && !lse) return AIT_EINVAL;
+  if ((unsigned long long)o_rest % 16) return AIT_EUNSUPPORTED;
   const size_t need = ait_packed_attn_bwd_workspace_bytes(p);
   if (!workspace || workspace_bytes < need) return AIT_EWORKSPACE;
-  BwdArgs a{q, k, v, o, d_o, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
+  BwdArgs a{q, k, v, o, d_o, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
             dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
             p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p),
-            (int)block_numbers(p->total_k, 1, BM, p->n_seq, p->zero_rest ? 1 : 0), p->scale, nullptr, nullptr, nullptr, d_table};
-  a.lse2 = static_cast<float*>(workspace);
-  a.delta = a.lse2 + (size_t)p->heads * p->total_q;
+            (int)block_numbers(p->total_k, 1, BM, p->n_seq, p->zero_rest ? 1 : 0), p->scale, static_cast<float*>(workspace), nullptr, d_table};
   if (p->bias_table && d_table) a.part_table = a.delta + (size_t)p->heads * p->total_q;
   const hipStream_t st = ait_stream(stream);
   AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, st) : launch_t<__bf16>(a, st));

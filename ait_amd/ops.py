@@ -786,72 +786,98 @@ def conv_bwd_weight_bf16s(dy16, x16, geom, kh, kw, split_k=8, partials=False):
 
 
 # ------------------------------------------------------------------------------------------
-# packed sequences (ait_packed_attn_*; autograd in ait_amd/packed.py)
+# packed sequences (ait_packed_attn_*, ait_gated_norm_*; autograd in ait_amd/packed.py)
 # ------------------------------------------------------------------------------------------
-def _need(ok, what):
-    if not ok:
-        raise _lib.AitHipError("packed_attn: " + what)
+def _refuse(op, what, *a):
+    raise _lib.AitHipError(op + ": " + (what % a if a else what))
 
 
-def _index(name, t, n, device):
-    _need(torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == n, "`%s` must be an int32 tensor of %d values" % (name, n))
-    _need(t.device == device, "`%s` is on %s, the tensors on %s" % (name, t.device, device))
+def _index(op, name, t, n, device):
+    if not (torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == n):
+        _refuse(op, "`%s` must be an int32 tensor of %d values", name, n)
+    if t.device != device:
+        _refuse(op, "`%s` is on %s, the tensors on %s", name, t.device, device)
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _fit(t):
     """t [rows, heads, d] with unit element stride, row / head pitches and a base of whole 16-byte vectors -- itself, or a copy"""
-    v = 16 // t.element_size()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] < 2 or (t.stride(i) % v == 0 and t.stride(i) >= 0) for i in (0, 1)) \
-        and t.stride(0) * t.element_size() < 2 ** 25
+    es = t.element_size()
+    v = 16 // es
+    (rows, heads, _), (sr, sh, se) = t.shape, t.stride()
+    ok = se == 1 and t.data_ptr() % 16 == 0 and (rows < 2 or (sr % v == 0 and sr * es < 2 ** 25)) and (heads < 2 or sh % v == 0)
     return t if ok or t.numel() == 0 else t.contiguous()
 
 
 def _row_head(t):
-    """(pointer, row pitch, head pitch): pitches of dimensions of size one are free, the library wants whole vectors"""
-    v = 16 // t.element_size()
-    return ctypes.c_void_p(t.data_ptr()), t.stride(0) - t.stride(0) % v, t.stride(1) - t.stride(1) % v
+    """pointer, row pitch, head pitch; those of a dimension of size one are free"""
+    (rows, heads, _), (sr, sh, _) = t.shape, t.stride()
+    return t.data_ptr(), sr if rows > 1 else 0, sh if heads > 1 else 0
 
 
 def packed_attn_desc(q, k, v, cu_q, cu_k, k_len=None, max_q=None, max_k=None, causal=False, scale=None, table=None, bucket_of=None):
     """checks the arguments and returns (ait_packed_attn, the tensors it points at)"""
+    op = "packed_attn"
     for n, t in (("q", q), ("k", k), ("v", v)):
-        _need(torch.is_tensor(t) and t.dim() == 3, "`%s` must be [rows, heads, d]" % n)
-        _need(t.dtype in _lib.DTYPES, "float32 or bfloat16 expected, got %s for `%s`" % (t.dtype, n))
-        _need(t.dtype == q.dtype and t.device == q.device, "q, k and v share one type and device")
-    (tq, H, d), (tk, Hk, dk) = q.shape, k.shape
-    _need(tuple(v.shape) == (tk, Hk, dk) and dk == d, "k and v must be [rows, kv_heads, %d] alike (got %s, %s)" % (d, tuple(k.shape), tuple(v.shape)))
-    _need(H > 0 and Hk > 0 and H % Hk == 0, "%d heads cannot share %d key heads" % (H, Hk))
-    _need(0 < d <= 128 and d % 8 == 0, "head width %d: a multiple of 8 up to 128 expected" % d)
-    _need(max(tq, tk) < 2 ** 31, "row counts must fit 31 bits")
-    _need(torch.is_tensor(cu_q) and cu_q.dim() == 1 and cu_q.numel() > 0, "`cu_q` must be an int32 tensor of n_seq + 1 values")
-    n = cu_q.numel() - 1
+        if not (torch.is_tensor(t) and t.dim() == 3):
+            _refuse(op, "`%s` must be [rows, heads, d]", n)
+        if t.dtype not in _lib.DTYPES:
+            _refuse(op, "float32 or bfloat16 expected, got %s for `%s`", t.dtype, n)
     dev = q.device
-    cu_q, cu_k = _index("cu_q", cu_q, n + 1, dev), _index("cu_k", cu_k, n + 1, dev)
-    k_len = None if k_len is None else _index("k_len", k_len, n, dev)
+    if not (k.dtype == q.dtype == v.dtype and k.device == dev == v.device):
+        _refuse(op, "q, k and v share one type and device")
+    (tq, H, d), (tk, Hk, dk) = q.shape, k.shape
+    if v.shape != k.shape or dk != d:
+        _refuse(op, "k and v must be [rows, kv_heads, %d] alike (got %s, %s)", d, tuple(k.shape), tuple(v.shape))
+    if H <= 0 or Hk <= 0 or H % Hk:
+        _refuse(op, "%d heads cannot share %d key heads", H, Hk)
+    if d <= 0 or d > 128 or d % 8:
+        _refuse(op, "head width %d: a multiple of 8 up to 128 expected", d)
+    if max(tq, tk) >= 2 ** 31:
+        _refuse(op, "row counts must fit 31 bits")
+    if not (torch.is_tensor(cu_q) and cu_q.dim() == 1 and cu_q.numel() > 0):
+        _refuse(op, "`cu_q` must be an int32 tensor of n_seq + 1 values")
+    n = cu_q.numel() - 1
+    cu_q, cu_k = _index(op, "cu_q", cu_q, n + 1, dev), _index(op, "cu_k", cu_k, n + 1, dev)
     p = _lib.PackedAttn()
+    if k_len is not None:
+        k_len = _index(op, "k_len", k_len, n, dev)
     if table is not None:
-        _need(torch.is_tensor(table) and table.dim() == 2 and table.shape[1] == H and table.shape[0] > 0 and table.dtype == torch.float32
-              and table.device == dev, "the bias table must be a float32 [n_buckets, %d] tensor on %s" % (H, dev))
-        _need(torch.is_tensor(bucket_of) and bucket_of.dim() == 1 and bucket_of.numel() % 2 == 1, "`bucket_of` must have 2 * max_distance + 1 values")
-        bucket_of = _index("bucket_of", bucket_of, bucket_of.numel(), dev)
-        _need(table.shape[0] <= _lib.MAX_BUCKETS and bucket_of.numel() // 2 <= _lib.MAX_BIAS_DISTANCE,
-              "at most %d buckets and a distance of %d" % (_lib.MAX_BUCKETS, _lib.MAX_BIAS_DISTANCE))
+        if not (torch.is_tensor(table) and table.dim() == 2 and table.shape[1] == H and table.shape[0] > 0 and table.dtype == torch.float32
+                and table.device == dev):
+            _refuse(op, "the bias table must be a float32 [n_buckets, %d] tensor on %s", H, dev)
+        if not (torch.is_tensor(bucket_of) and bucket_of.dim() == 1 and bucket_of.numel() % 2 == 1):
+            _refuse(op, "`bucket_of` must have 2 * max_distance + 1 values")
+        bucket_of = _index(op, "bucket_of", bucket_of, bucket_of.numel(), dev)
+        if table.shape[0] > _lib.MAX_BUCKETS or bucket_of.numel() // 2 > _lib.MAX_BIAS_DISTANCE:
+            _refuse(op, "at most %d buckets and a distance of %d", _lib.MAX_BUCKETS, _lib.MAX_BIAS_DISTANCE)
         table = table.contiguous()
         p.n_buckets, p.max_distance = table.shape[0], bucket_of.numel() // 2
-        p.bias_table, p.bucket_of = table.data_ptr(), bucket_of.data_ptr()
     if not q.is_cuda:
-        raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % q.device)
-    p.cu_q, p.cu_k, p.k_len = cu_q.data_ptr(), cu_k.data_ptr(), None if k_len is None else k_len.data_ptr()
+        raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % dev)
     p.n_seq, p.total_q, p.total_k, p.heads, p.kv_heads, p.d = n, tq, tk, H, Hk, d
-    p.max_q, p.max_k = min(int(max_q or 0), tq), min(int(max_k or 0), tk)
-    p.dtype, p.causal, p.scale = _lib.DTYPES[q.dtype], int(bool(causal)), float(d ** -0.5 if scale is None else scale)
-    return p, (cu_q, cu_k, k_len, table, bucket_of)
+    if max_q:
+        p.max_q = min(int(max_q), tq)
+    if max_k:
+        p.max_k = min(int(max_k), tk)
+    p.dtype, p.causal, p.scale = _lib.DTYPES[q.dtype], 1 if causal else 0, d ** -0.5 if scale is None else float(scale)
+    keep = (cu_q, cu_k, k_len, table, bucket_of)
+    packed_attn_point(p, *keep)
+    return p, keep
 
 
-def packed_attn_fwd(p, q, k, v, out=None, want_lse=False):
-    """ait_packed_attn_fwd: o [total_q, heads, d] (rows of no sequence: zero, or left as they are in a given `out`), lse
-    [heads, total_q] or None.  p: packed_attn_desc's."""
+def packed_attn_point(p, cu_q, cu_k, k_len, table, bucket_of):
+    """the descriptor's device tables"""
+    p.cu_q, p.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    if k_len is not None:
+        p.k_len = k_len.data_ptr()
+    if table is not None:
+        p.bias_table, p.bucket_of = table.data_ptr(), bucket_of.data_ptr()
+
+
+def packed_attn_fwd(p, q, k, v, out=None, for_backward=False):
+    """ait_packed_attn_fwd: o [total_q, heads, d] (rows of no sequence: zero, or left as they are in a given `out`) and, for the
+    backward, lse [heads, total_q] and what rounding took from o (bf16; else None).  p: packed_attn_desc's."""
     L = _lib.lib()
     dev = q.device
     q, k, v = _fit(q), _fit(k), _fit(v)
@@ -861,21 +887,26 @@ def packed_attn_fwd(p, q, k, v, out=None, want_lse=False):
         if p.n_seq == 0:
             out.zero_()
     else:
-        _need(out.is_cuda and out.device == dev and out.dtype == q.dtype and out.shape == q.shape and _fit(out) is out
-              and all(out.shape[i] < 2 or out.stride(i) > 0 for i in (0, 1)),
-              "`out` must be a %s tensor of q's shape with 16-byte rows" % q.dtype)
+        if not (out.is_cuda and out.device == dev and out.dtype == q.dtype and out.shape == q.shape and _fit(out) is out
+                and all(out.shape[i] < 2 or out.stride(i) > 0 for i in (0, 1))):
+            _refuse("packed_attn", "`out` must be a %s tensor of q's shape with 16-byte rows", q.dtype)
         p.zero_rest = 0
-    lse = torch.empty((p.heads, p.total_q), dtype=torch.float32, device=dev) if want_lse else None
-    with torch.cuda.device(dev):
+    lse = rest = None
+    if for_backward:
+        lse = torch.empty((p.heads, p.total_q), dtype=torch.float32, device=dev)
+        if q.dtype == torch.bfloat16:
+            rest = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    with _lib.on_device(dev):
         n = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = L.ait_packed_attn_fwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(out), _p(lse),
-                                   None if ws is None else ctypes.c_void_p(ws.data_ptr()), n, _lib.cur_stream(dev))
+        rc = L.ait_packed_attn_fwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(out),
+                                   None if lse is None else lse.data_ptr(), None if rest is None else rest.data_ptr(),
+                                   None if ws is None else ws.data_ptr(), n, _lib.raw_stream(dev))
     _lib.check(rc, "ait_packed_attn_fwd")
-    return out, lse
+    return out, lse, rest
 
 
-def packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=False):
+def packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=False):
     """ait_packed_attn_bwd: (dq, dk, dv, d_table f32 [n_buckets, heads] or None)"""
     L = _lib.lib()
     dev = q.device
@@ -884,14 +915,17 @@ def packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=False):
     p.zero_rest = 1
     if p.n_seq == 0:
         dq.zero_(), dk.zero_(), dv.zero_()
-    dt = torch.zeros((p.n_buckets, p.heads), dtype=torch.float32, device=dev) if want_table and (p.n_seq == 0 or p.total_q == 0) else \
-        torch.empty((p.n_buckets, p.heads), dtype=torch.float32, device=dev) if want_table else None
-    with torch.cuda.device(dev):
+    dt = None
+    if want_table:
+        dt = torch.empty((p.n_buckets, p.heads), dtype=torch.float32, device=dev)
+        if p.n_seq == 0 or p.total_q == 0:
+            dt.zero_()
+    with _lib.on_device(dev):
         n = L.ait_packed_attn_bwd_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-        rc = L.ait_packed_attn_bwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(o), *_row_head(d_o), _p(lse),
-                                   *_row_head(dq), *_row_head(dk), *_row_head(dv), _p(dt), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                   _lib.cur_stream(dev))
+        rc = L.ait_packed_attn_bwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(o),
+                                   None if rest is None else rest.data_ptr(), *_row_head(d_o), lse.data_ptr(), *_row_head(dq), *_row_head(dk),
+                                   *_row_head(dv), None if dt is None else dt.data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(dev))
     _lib.check(rc, "ait_packed_attn_bwd")
     return dq, dk, dv, dt
 
@@ -903,47 +937,65 @@ def _rows2d(t):
 
 def gated_norm_desc(x, f, w_post, w_pre, b_post=None, b_pre=None, gate=None, scale=None, layer=False, eps=1e-6, cu_seqlens=None):
     """checks the arguments and returns (ait_gated_norm, the tensors it points at).  x, f [rows, width]"""
-    def need(ok, what):
-        if not ok:
-            raise _lib.AitHipError("gated_norm: " + what)
+    op = "gated_norm"
     for n, t in (("x", x), ("f", f)):
-        need(torch.is_tensor(t) and t.dim() == 2 and t.dtype in _lib.DTYPES, "`%s` must be a float32 or bfloat16 [rows, width] tensor" % n)
-    need(x.shape == f.shape and x.device == f.device, "x and f must have one shape and device (got %s, %s)" % (tuple(x.shape), tuple(f.shape)))
-    need(not (x.dtype == torch.bfloat16 and f.dtype == torch.float32), "a bfloat16 stream takes a bfloat16 branch")
-    rows, W = x.shape
+        if not (torch.is_tensor(t) and t.dim() == 2 and t.dtype in _lib.DTYPES):
+            _refuse(op, "`%s` must be a float32 or bfloat16 [rows, width] tensor", n)
     dev = x.device
-    need(0 < W <= _lib.MAX_NORM_WIDTH, "width %d: 1 to %d expected" % (W, _lib.MAX_NORM_WIDTH))
-    need(rows < 2 ** 31 - 4096, "row counts must fit 31 bits")
+    if x.shape != f.shape or dev != f.device:
+        _refuse(op, "x and f must have one shape and device (got %s, %s)", tuple(x.shape), tuple(f.shape))
+    if x.dtype == torch.bfloat16 and f.dtype == torch.float32:
+        _refuse(op, "a bfloat16 stream takes a bfloat16 branch")
+    rows, W = x.shape
+    if W <= 0 or W > _lib.MAX_NORM_WIDTH:
+        _refuse(op, "width %d: 1 to %d expected", W, _lib.MAX_NORM_WIDTH)
+    if rows >= 2 ** 31 - 4096:
+        _refuse(op, "row counts must fit 31 bits")
     par = []
     for n, t in (("post_weight", w_post), ("post_bias", b_post), ("pre_weight", w_pre), ("pre_bias", b_pre), ("scale", scale)):
-        need(t is not None or n in ("post_bias", "pre_bias", "scale"), "`%s` is missing" % n)
-        need(t is None or (torch.is_tensor(t) and t.dtype == torch.float32 and tuple(t.shape) == (W,) and t.device == dev),
-             "`%s` must be a float32 [%d] tensor on %s" % (n, W, dev))
+        if t is None:
+            if n in ("post_weight", "pre_weight"):
+                _refuse(op, "`%s` is missing", n)
+        elif not (torch.is_tensor(t) and t.dtype == torch.float32 and t.dim() == 1 and t.numel() == W and t.device == dev):
+            _refuse(op, "`%s` must be a float32 [%d] tensor on %s", n, W, dev)
         par.append(None if t is None else t.contiguous())
     n_seq = 0
-    need(cu_seqlens is None or gate is not None, "`cu_seqlens` says whose gate a row takes: there is no gate")
-    if gate is not None:
+    if gate is None:
         if cu_seqlens is not None:
-            need(torch.is_tensor(cu_seqlens) and cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() > 0
-                 and cu_seqlens.device == dev, "`cu_seqlens` must be an int32 tensor on %s" % dev)
-            n_seq, cu_seqlens = cu_seqlens.numel() - 1, cu_seqlens.contiguous()
-        need(torch.is_tensor(gate) and gate.dtype == f.dtype and gate.device == dev
-             and tuple(gate.shape) == ((rows if cu_seqlens is None else n_seq), W),
-             "the gate must be a %s [%d, %d] tensor on %s" % (f.dtype, rows if cu_seqlens is None else n_seq, W, dev))
-        gate = _rows2d(gate)
+            _refuse(op, "`cu_seqlens` says whose gate a row takes: there is no gate")
+    else:
+        if cu_seqlens is not None:
+            if not (torch.is_tensor(cu_seqlens) and cu_seqlens.dim() == 1 and cu_seqlens.numel() > 0):
+                _refuse(op, "`cu_seqlens` must be an int32 tensor of n_seq + 1 values")
+            cu_seqlens = _index(op, "cu_seqlens", cu_seqlens, cu_seqlens.numel(), dev)
+            n_seq = cu_seqlens.numel() - 1
+        n = rows if cu_seqlens is None else n_seq
+        if not (torch.is_tensor(gate) and gate.dtype == f.dtype and gate.device == dev and tuple(gate.shape) == (n, W)):
+            _refuse(op, "the gate must be a %s [%d, %d] tensor on %s", f.dtype, n, W, dev)
     if not x.is_cuda:
         raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % dev)
-    x, f = _rows2d(x), _rows2d(f)
     p = _lib.GatedNorm()
-    ptr = lambda t: None if t is None else t.data_ptr()
-    p.x, p.f, p.gate, p.cu_seqlens, p.x_row, p.f_row = ptr(x), ptr(f), ptr(gate), ptr(cu_seqlens), x.stride(0), f.stride(0)
-    p.gate_row = 0 if gate is None else gate.stride(0)
-    p.w_post, p.b_post, p.w_pre, p.b_pre, p.scale = (ptr(t) for t in par)
     p.rows, p.width, p.n_seq, p.dtype_x, p.dtype_f, p.layer, p.zero_rest, p.eps = rows, W, n_seq, _lib.DTYPES[x.dtype], _lib.DTYPES[f.dtype], \
-        int(bool(layer)), 1, float(eps)
-    if gate is not None and gate.numel() == 0 and p.gate is None:
-        p.gate = p.w_post            # (an empty gate is still a gate; nothing reads it)
-    return p, (x, f, gate, cu_seqlens, *par)
+        1 if layer else 0, 1, float(eps)
+    keep = (_rows2d(x), _rows2d(f), None if gate is None else _rows2d(gate), cu_seqlens, *par)
+    gated_norm_point(p, *keep)
+    return p, keep
+
+
+def gated_norm_point(p, x, f, gate, cu_seqlens, w_post, b_post, w_pre, b_pre, scale):
+    """the descriptor's tensors"""
+    p.x, p.f, p.x_row, p.f_row = x.data_ptr(), f.data_ptr(), x.stride(0), f.stride(0)
+    if gate is not None:
+        p.gate, p.gate_row = gate.data_ptr() or w_post.data_ptr(), gate.stride(0)      # (an empty gate is a gate; nothing reads it)
+        if cu_seqlens is not None:
+            p.cu_seqlens = cu_seqlens.data_ptr()
+    p.w_post, p.w_pre = w_post.data_ptr(), w_pre.data_ptr()
+    if b_post is not None:
+        p.b_post = b_post.data_ptr()
+    if b_pre is not None:
+        p.b_pre = b_pre.data_ptr()
+    if scale is not None:
+        p.scale = scale.data_ptr()
 
 
 def gated_norm_fwd(p, x, f, want_stats=False):
@@ -951,9 +1003,9 @@ def gated_norm_fwd(p, x, f, want_stats=False):
     dev = x.device
     y, h = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(f.shape, dtype=f.dtype, device=dev)
     stats = torch.empty((p.rows, 4), dtype=torch.float32, device=dev) if want_stats else None
-    with torch.cuda.device(dev):
-        rc = _lib.lib().ait_gated_norm_fwd(ctypes.byref(p), ctypes.c_void_p(y.data_ptr()), p.width, ctypes.c_void_p(h.data_ptr()), p.width,
-                                           _p(stats), _lib.cur_stream(dev))
+    with _lib.on_device(dev):
+        rc = _lib.lib().ait_gated_norm_fwd(ctypes.byref(p), y.data_ptr(), p.width, h.data_ptr(), p.width,
+                                           None if stats is None else stats.data_ptr(), _lib.raw_stream(dev))
     _lib.check(rc, "ait_gated_norm_fwd")
     return y, h, stats
 
@@ -971,11 +1023,11 @@ def gated_norm_bwd(p, x, f, gate, stats, dy, dh):
     it = iter(flat)
     dwp, dwq = next(it), next(it)
     ds, dbp, dbq = (next(it) if t is not None else None for t in (p.scale, p.b_post, p.b_pre))
-    vp = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
-    with torch.cuda.device(dev):
+    vp = lambda t: None if t is None else t.data_ptr()
+    with _lib.on_device(dev):
         nb = L.ait_gated_norm_bwd_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
         rc = L.ait_gated_norm_bwd(ctypes.byref(p), vp(stats), vp(dy), dy.stride(0), vp(dh), dh.stride(0), vp(dx), p.width, vp(df), p.width,
-                                  vp(dg), p.width, vp(dwp), vp(dwq), vp(ds), vp(dbp), vp(dbq), vp(ws), ws.numel(), _lib.cur_stream(dev))
+                                  vp(dg), p.width, vp(dwp), vp(dwq), vp(ds), vp(dbp), vp(dbq), vp(ws), ws.numel(), _lib.raw_stream(dev))
     _lib.check(rc, "ait_gated_norm_bwd")
     return dx, df, dg, dwp, dbp, dwq, dbq, ds

@@ -17,29 +17,28 @@ import torch.nn as nn
 from . import _lib, ops
 
 
+def _recorded(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of):
-        table32 = None if table is None else table.float()
-        p, keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table32, bucket_of)
-        grad = any(ctx.needs_input_grad[:4])
-        o, lse = ops.packed_attn_fwd(p, q, k, v, want_lse=grad)
-        if grad:
-            ctx.save_for_backward(q, k, v, o, lse, *[t for t in keep if t is not None])
-            ctx.there = [t is not None for t in keep]
-            ctx.cfg = (max_q, max_k, causal, scale, None if table is None else table.dtype)
+        p, keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, None if table is None else table.float(), bucket_of)
+        o, lse, rest = ops.packed_attn_fwd(p, q, k, v, for_backward=True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, *keep)
+        ctx.p, ctx.table_dtype = p, None if table is None else table.dtype
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
-        q, k, v, o, lse, *keep = ctx.saved_tensors
-        cu_q, cu_k, k_len, table, bucket_of = [keep.pop(0) if t else None for t in ctx.there]
-        max_q, max_k, causal, scale, dt = ctx.cfg
-        p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)
-        dq, dk, dv, d_table = ops.packed_attn_bwd(p, q, k, v, o, d_o, lse, want_table=table is not None and ctx.needs_input_grad[3])
-        n = ctx.needs_input_grad
-        return (dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, None if d_table is None else d_table.to(dt)) + (None,) * 8
+        q, k, v, o, lse, rest, *keep = ctx.saved_tensors
+        p, n = _lib.PackedAttn.from_buffer_copy(ctx.p), ctx.needs_input_grad
+        ops.packed_attn_point(p, *keep)
+        dq, dk, dv, dt = ops.packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=n[3])
+        return dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, None if dt is None else dt.to(ctx.table_dtype), \
+            None, None, None, None, None, None, None, None
 
 
 def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=None, causal=False, scale=None, bias=None):
@@ -60,7 +59,12 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
         table, bucket_of = (bias.weight, bias.bucket_of) if isinstance(bias, RelativePositionBias) else bias
         if not torch.is_tensor(table) or table.dtype not in _lib.DTYPES:
             raise _lib.AitHipError("packed_attn: the bias table must be a float32 or bfloat16 tensor")
-    return _PackedAttention.apply(q, k, v, table, cu_q, cu_q if cu_k is None else cu_k, k_len, max_q, max_k, bool(causal), scale, bucket_of)
+    if cu_k is None:
+        cu_k = cu_q
+    if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded(q, k, v, table):
+        return _PackedAttention.apply(q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of)
+    p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, None if table is None else table.float(), bucket_of)
+    return ops.packed_attn_fwd(p, q, k, v)[0]
 
 
 def relative_buckets(n_buckets, max_distance, two_sided, device=None):
@@ -98,28 +102,27 @@ class RelativePositionBias(nn.Module):
         self.register_buffer("bucket_of", relative_buckets(n_buckets, max_distance, two_sided), persistent=False)
 
 
+def _f32(t):
+    return None if t is None else t.float()
+
+
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, gate, w_post, b_post, w_pre, b_pre, scale, cu_seqlens, layer, eps):
-        f32 = lambda t: None if t is None else t.float()
-        p, keep = ops.gated_norm_desc(x, f, f32(w_post), f32(w_pre), f32(b_post), f32(b_pre), gate, f32(scale), layer, eps, cu_seqlens)
-        grad = any(ctx.needs_input_grad[:8])
-        y, h, stats = ops.gated_norm_fwd(p, x, f, want_stats=grad)
-        if grad:
-            ctx.save_for_backward(stats, *[t for t in keep if t is not None])
-            ctx.there = [t is not None for t in keep]
-            ctx.cfg = (layer, eps, [None if t is None else t.dtype for t in (w_post, b_post, w_pre, b_pre, scale)])
+        p, keep = ops.gated_norm_desc(x, f, _f32(w_post), _f32(w_pre), _f32(b_post), _f32(b_pre), gate, _f32(scale), layer, eps, cu_seqlens)
+        y, h, stats = ops.gated_norm_fwd(p, x, f, want_stats=True)
+        ctx.save_for_backward(stats, *keep)
+        ctx.p, ctx.types = p, [None if t is None else t.dtype for t in (w_post, b_post, w_pre, b_pre, scale)]
         return y, h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
         stats, *keep = ctx.saved_tensors
-        x, f, gate, cu_seqlens, w_post, b_post, w_pre, b_pre, scale = [keep.pop(0) if t else None for t in ctx.there]
-        layer, eps, types = ctx.cfg
-        p, _keep = ops.gated_norm_desc(x, f, w_post, w_pre, b_post, b_pre, gate, scale, layer, eps, cu_seqlens)
-        dx, df, dg, *par = ops.gated_norm_bwd(p, x, f, gate, stats, dy, dh)
-        grads = [dx, df, dg] + [None if t is None else t.to(dt) for t, dt in zip(par, types)]
+        p = _lib.GatedNorm.from_buffer_copy(ctx.p)
+        ops.gated_norm_point(p, *keep)
+        dx, df, dg, *par = ops.gated_norm_bwd(p, keep[0], keep[1], keep[2], stats, dy, dh)
+        grads = [dx, df, dg] + [None if t is None else t.to(dt) for t, dt in zip(par, ctx.types)]
         return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None, None, None)
 
 
@@ -148,5 +151,10 @@ def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, 
         if gate is not None and gate.shape != shape:
             raise _lib.AitHipError("gated_norm: a gate without cu_seqlens has x's shape")
         x, f, gate = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, f, gate))
-    y, h = _GatedNorm.apply(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale, cu_seqlens, kind == "layer", eps)
-    return y.view(shape), h.view(shape)
+    if _recorded(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale):
+        y, h = _GatedNorm.apply(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale, cu_seqlens, kind == "layer", eps)
+    else:
+        p, keep = ops.gated_norm_desc(x, f, _f32(post_weight), _f32(pre_weight), _f32(post_bias), _f32(pre_bias), gate, _f32(scale),
+                                      kind == "layer", eps, cu_seqlens)
+        y, h, _ = ops.gated_norm_fwd(p, x, f)
+    return (y, h) if len(shape) == 2 else (y.view(shape), h.view(shape))

@@ -874,8 +874,7 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *   o_i  = sum_j softmax_j(s_ij) v_j        over the keys j that query i sees: all of its sequence, or with `causal`
  *                                           those with j - i <= len_k - len_q (the last query sees every key)
  *
- * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and lse = -infinity, and
- * takes part in no gradient.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
+ * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and takes part in no gradient.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
  * multiplied, whatever it holds; a key INSIDE the sequence that a causal mask hides from a query must be finite (its value is
  * multiplied by a probability of zero).
  *
@@ -892,7 +891,9 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *   bias_table f32 [n_buckets, heads] or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
  *     table): the bucket of relative position key - query, where the last query is level with the last key; further away the
  *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
- *   lse f32 [heads, total_q] or NULL: log of the sum of exp of a row's scores, which the backward reads.
+ *   For the backward, else NULL: lse f32 [heads, total_q], the binary logarithm of a row's sum of exp (+infinity where a query
+ *     sees no key); o_rest [total_q, heads, d] contiguous, AIT_DTYPE_BF16 only: what rounding took from o, without which the
+ *     gradients of q and k carry o's rounding error.
  *
  * Backward: dq / dk / dv (pitches as given), and with a bias d_table f32 [n_buckets, heads] (overwritten; NULL: not wanted).
  * No atomics on memory: results are the same from run to run, and do not depend on what else runs.
@@ -916,11 +917,11 @@ typedef struct {
 size_t ait_packed_attn_fwd_workspace_bytes(const ait_packed_attn* p);
 int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                         long long k_head, const void* v, long long v_row, long long v_head, void* o, long long o_row,
-                        long long o_head, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                        long long o_head, float* lse, void* o_rest, void* workspace, size_t workspace_bytes, void* stream);
 size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p);
 int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                         long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
-                        long long o_head, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
+                        long long o_head, const void* o_rest, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
                         long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
                         long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -59,8 +59,8 @@ def attn_ref(q, k, v, ql, qs, kl, ks, causal, scale, table=None, bucket_of=None,
             O = p @ V
             o[qa:qa + a, h] = O
             EO = po @ V.abs() + (b + 8) * f * (p @ V.abs())
-            EO = EO + u * (O.abs() + EO)
-            eo[qa:qa + a, h] = EO
+            eo[qa:qa + a, h] = EO + u * (O.abs() + EO)
+            EO = EO + max(u * u, f) * (O.abs() + EO) * 1.01          # ... and the backward has what its rounding took
             if do is None:
                 continue
             G = do[qa:qa + a, h]
@@ -244,11 +244,11 @@ def test_c_entries_refuse_bad_arguments():
 
     def fwd(qptr=4096, qrow=256, qhead=64, **kw):
         p = _lib.PackedAttn(**{**base, **kw})
-        return L.ait_packed_attn_fwd(ctypes.byref(p), qptr, qrow, qhead, *(4096, 128, 64) * 2, 4096, 256, 64, None, None, 0, None)
+        return L.ait_packed_attn_fwd(ctypes.byref(p), qptr, qrow, qhead, *(4096, 128, 64) * 2, 4096, 256, 64, None, None, None, 0, None)
 
     def bwd(ws=4096, n=1 << 30, lse=4096, **kw):
         p = _lib.PackedAttn(**{**base, **kw})
-        return L.ait_packed_attn_bwd(ctypes.byref(p), *(4096, 256, 64), *(4096, 128, 64) * 2, *(4096, 256, 64) * 2, lse, *(4096, 256, 64),
+        return L.ait_packed_attn_bwd(ctypes.byref(p), *(4096, 256, 64), *(4096, 128, 64) * 2, *(4096, 256, 64), None, *(4096, 256, 64), lse, *(4096, 256, 64),
                                      *(4096, 128, 64) * 2, None, ws, n, None)
     EINVAL, EWORKSPACE, EUNSUPPORTED = -1, -2, -4
     for f in (fwd, bwd):
@@ -261,8 +261,8 @@ def test_c_entries_refuse_bad_arguments():
         assert f(n_seq=0) == 0
     assert fwd(qptr=None) == EINVAL and fwd(qptr=4100) == EUNSUPPORTED and fwd(qrow=255) == EUNSUPPORTED and fwd(qhead=65) == EUNSUPPORTED
     assert fwd(qrow=1 << 24) == EUNSUPPORTED
-    assert bwd(lse=None) == EINVAL and bwd(ws=None) == EWORKSPACE and bwd(n=2 * 4 * 5 * 4 - 1) == EWORKSPACE
-    assert L.ait_packed_attn_fwd(None, *(None, 0, 0) * 4, None, None, 0, None) == EINVAL
+    assert bwd(lse=None) == EINVAL and bwd(ws=None) == EWORKSPACE and bwd(n=4 * 5 * 4 - 1) == EWORKSPACE
+    assert L.ait_packed_attn_fwd(None, *(None, 0, 0) * 4, None, None, None, 0, None) == EINVAL
     # a few tokens over a long key axis are cut along it: a workspace is asked for, and a small one refused
     p = dict(n_seq=2, total_q=2, total_k=20000, max_q=1, max_k=10000)
     need = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(_lib.PackedAttn(**{**base, **p})))
