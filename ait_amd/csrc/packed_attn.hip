@@ -83,7 +83,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
   {
     const T* qr = reinterpret_cast<const T*>(a.q) + (long long)(qstart + pos) * a.qs + (long long)head * a.qh;
 #pragma unroll
-    for (int c = 0; c < NCH; c++) qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < rows);
+    for (int c = 0; c < NCH; c++) {
+      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < rows);
+      if (a.scale < 0.f) qf[c] = -qf[c];      // (so that the largest product is the largest score)
+    }
   }
   const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lk, lv;
@@ -109,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
   }
 
   const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
-  const float sc = a.scale * kLog2e;
+  const float sc = fmaxf(fabsf(a.scale * kLog2e), 1e-30f);      // (0 would make NaN of the hidden scores' -infinity)
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; b++)
@@ -126,32 +129,30 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
     const unsigned char* vt = kt + kTile;
     f32x16 s[2];
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
+    for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int r = 0; r < 16; r++) s[x][r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; c++) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);
-    }
+    for (int c = 0; c < NCH; c++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);
+    read_ahead<T, 2 * NCH, 1, 4>();
+    // the block's scores are f * s + add: scaled already where a bias is added value by value
+    float f = sc, add = 0.f;
     if constexpr (BIAS) {
       const int md = a.bias.max_distance;
-      if (k0 + KB - 1 - (wfirst + off) <= -md || k0 - (wlast + off) >= md) {
-        const float f = k0 - (wlast + off) >= md ? far_hi : far_lo;
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) s[x][r] = __builtin_fmaf(s[x][r], sc, f);
+      if (k0 - (wlast + off) >= md) {
+        add = far_hi;
+      } else if (k0 + KB - 1 - (wfirst + off) <= -md) {
+        add = far_lo;
       } else {
         const float* p = bl + (k0 + 4 * h - (pos + off) + md + kPad);
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
           for (int r = 0; r < 16; r++) s[x][r] = __builtin_fmaf(s[x][r], sc, p[32 * x + 8 * (r >> 2) + (r & 3)]);
+        f = 1.f;
       }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 2; x++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) s[x][r] *= sc;
     }
     if (k0 + KB > wsure) {
       const int lim = kmax - k0 - 4 * h;
@@ -162,24 +163,27 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
     }
     float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-    for (int r = 1; r < 16; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
-    top = column_max(top);
-    const float mn = fmaxf(m, top), mu = mn == kNegInf ? 0.f : mn;
-    const float alpha = fast_exp2(m - mu);
-    m = mn;
-    float sum = 0.f;
+    for (int r = 1; r < 16; r++) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+    top = __builtin_fmaf(column_max(top), f, add);
+    // The maximum is only followed where it rises by more than 2^8: what is summed stays below 2^8 and the same bits are
+    // significant, and nearly every block is spared the rescaling of the accumulators
+    if (__any(top > m + 8.f)) {
+      const float mn = fmaxf(m, top), alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[b][r] *= alpha;
+    }
+    const float sub = add - (m == kNegInf ? 0.f : m);
 #pragma unroll
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        s[x][r] = fast_exp2(s[x][r] - mu);
-        sum += s[x][r];
+        s[x][r] = fast_exp2(__builtin_fmaf(s[x][r], f, sub));
+        l += s[x][r];
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) acc[b][r] *= alpha;
 #pragma unroll
     for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -188,6 +192,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
 #pragma unroll
         for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
       }
+    read_ahead<T, 4 * NB, 2, 4>();
   }
 
   if (row >= rows) return;

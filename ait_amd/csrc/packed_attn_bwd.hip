@@ -14,7 +14,14 @@ namespace {
 using namespace ait_packed;
 
 constexpr int NW = 4, NT = NW * 64, BM = NW * 32;
-constexpr int kHist = 96;       // relative positions that a 64 x 32 block spans
+// The bias's gradient wants the sums of a 32 x 32 block of dS along its diagonals (63 relative positions).  Each query writes its
+// column into a row of its own, shifted so that equal relative positions lie below one another, and a lane adds up one of the
+// 64 columns: plain writes and reads of shared memory.  (Added up by f32 atomics in shared memory instead, a block costs about
+// ten times as much: 207 us against 60 for the pass over sequences of 17 to 1024 tokens with a distance of 128.)  Where the
+// tiles leave no room for it (f32 rows of 128 values) the atomics on kHist sums remain.
+constexpr int kHist = 64, kSkew = 32 * 64;
+template <typename T, int D> constexpr bool kSkewed = D == 64 || sizeof(T) == 2;
+template <typename T, int D> constexpr int kSums = kSkewed<T, D> ? kSkew : kHist;      // floats of a wave
 
 struct BwdArgs {
   const void* q;
@@ -38,7 +45,7 @@ struct BwdArgs {
 };
 
 template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_bwd_q_kernel(const BwdArgs a) {
   constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -111,13 +118,13 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
     if (row >= qlen) l2 = -kNegInf;
   }
   float* bl = reinterpret_cast<float*>(lds + 4 * kTile);                 // the head's bias, then per wave: a block's sums by
-  float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kHist + nb);    // relative position, and the sums by bucket
-  float* acc_b = hist + kHist;
+  float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kSums<T, D> + nb);      // relative position, and the sums by bucket
+  float* acc_b = hist + kSums<T, D>;
   float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
   if constexpr (BIAS) {
     fill_bias<NT>(a.bias, a.H, head, 1, bl, tid);
     if (part) {
-      for (int x = lane; x < kHist + nb; x += 64) hist[x] = 0.f;
+      for (int x = lane; x < kSums<T, D> + nb; x += 64) hist[x] = 0.f;
     }
     __syncthreads();
     far_lo = bl[0];
@@ -150,9 +157,11 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; c++) s = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s);
-#pragma unroll
-      for (int c = 0; c < NCH; c++) dp = mma(row_frag<T, D>(vt, rb, x, c), gf[c], dp);
+      for (int c = 0; c < NCH; c++) {
+        s = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s);
+        dp = mma(row_frag<T, D>(vt, rb, x, c), gf[c], dp);
+      }
+      read_ahead<T, 2 * NCH, 1, 4>();
       if (BIAS && near) {
         const float* p = bl + (k0 + 32 * x + 4 * h - (pos + off) + md + kPad);
 #pragma unroll
@@ -172,10 +181,26 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
       if constexpr (BIAS) {
         if (part) {
           if (near) {
-            // key - query over the block, the block's last column (31) at its first key being 0
-            float* p = hist + 32 * x + 4 * h + 31 - (lane & 31);
+            // by key - query + 31 over the block
+            float u = 0.f;
+            if constexpr (kSkewed<T, D>) {
+              float* p = hist + (lane & 31) * 63 + 31 + 4 * h;
 #pragma unroll
-            for (int r = 0; r < 16; r++) __hip_atomic_fetch_add(p + 8 * (r >> 2) + (r & 3), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+              for (int r = 0; r < 16; r++) p[8 * (r >> 2) + (r & 3)] = s[r];
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (this wave's own memory, in order: no barrier)
+#pragma unroll
+              for (int c = 0; c < 32; c++) u += hist[c * 64 + lane];
+            } else {
+              float* p = hist + 31 - (lane & 31) + 4 * h;
+#pragma unroll
+              for (int r = 0; r < 16; r++)
+                __hip_atomic_fetch_add(p + 8 * (r >> 2) + (r & 3), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+              u = hist[lane];
+              hist[lane] = 0.f;
+            }
+            __hip_atomic_fetch_add(acc_b + bucket(a.bias, k0 + 32 * x - (row0 + 31 + off) + lane), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           } else {
             float u = 0.f;
 #pragma unroll
@@ -191,21 +216,7 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
 #pragma unroll
         for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(kt, cb, x, cc, b), df, acc[b]);
       }
-    }
-    if constexpr (BIAS) {
-      if (part && near) {      // this wave's own memory, in order: no barrier
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int i = lane + 64 * x;
-          if (i < kHist) {
-            const float u = hist[i];
-            hist[i] = 0.f;
-            __hip_atomic_fetch_add(acc_b + bucket(a.bias, k0 - (row0 + 31 + off) + i), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-          }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
+      read_ahead<T, 2 * NB, 2, 4>();
     }
   }
 
@@ -229,11 +240,11 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_q_kernel(const
         acc_b[bucket(a.bias, md)] += sum_hi;
       }
       __syncthreads();
-      const float* w0 = bl + bias_row(md) + kHist;
+      const float* w0 = bl + bias_row(md) + kSums<T, D>;
       for (int b = tid; b < nb; b += NT) {
         float u = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) u += w0[w * (kHist + nb) + b];
+        for (int w = 0; w < NW; w++) u += w0[w * (kSums<T, D> + nb) + b];
         part[b] = u;
       }
     }
@@ -257,16 +268,18 @@ __global__ __launch_bounds__(256) void packed_table_kernel(const BwdArgs a) {
   }
 }
 
-template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(const BwdArgs a) {
-  constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+// PARTS: 3 = dK and dV in one pass; 1 / 2: workgroups that form dV alone and workgroups that form dK alone
+template <typename T, int D, bool BIAS, int PART>
+__device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsigned char* lds) {
+  constexpr bool DK = PART & 2, DV = PART & 1;
+  constexpr int XH = 2;
+  constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes, BN = NW / XH * 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int kvh = blockIdx.x % a.Hk, group = a.H / a.Hk, number = (int)(blockIdx.x / a.Hk), md = a.bias.max_distance;
+  const int kvh = index % a.Hk, group = a.H / a.Hk, number = index / a.Hk, md = a.bias.max_distance;
   int seq, block, kstart, kroom, klen;
   // key blocks are numbered by the rows the sequences OCCUPY: keys behind k_len get zeros
-  if (!find_block(a.s.cu_k, a.s.n_seq, a.s.rest, a.s.total_k, 1, BM, number, seq, block, kstart, kroom)) return;
-  const int key0 = block * BM + wave * 32, key = key0 + (lane & 31);
+  if (!find_block(a.s.cu_k, a.s.n_seq, a.s.rest, a.s.total_k, 1, BN, number, seq, block, kstart, kroom)) return;
+  const int kc = wave % (NW / XH), xh = wave / (NW / XH), key0 = block * BN + kc * 32, key = key0 + (lane & 31);
   int qstart = 0, qlen = 0;
   klen = 0;
   if (seq < a.s.n_seq) {
@@ -277,17 +290,17 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
   }
   const int off = klen - qlen;
   // query rows that see a key j: positions >= j - off with a causal mask
-  const int gfirst = a.causal ? max(0, block * BM - off) : 0, wfirst = a.causal ? max(0, key0 - off) : 0;
+  const int gfirst = a.causal ? max(0, block * BN - off) : 0;
   const int wsure = a.causal ? max(0, min(key0 + 31, klen - 1) - off) : 0;          // from here on every key of the wave is seen
-  const int t0 = gfirst / KB, tq = block * BM < klen ? max(0, (qlen + KB - 1) / KB - t0) : 0, total = tq * group;
+  const int t0 = gfirst / KB, tq = block * BN < klen ? max(0, (qlen + KB - 1) / KB - t0) : 0, total = tq * group;
 
   const unsigned qstr = (unsigned)(a.qs * sizeof(T)), gstr = (unsigned)(a.dos * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lq, lg;
   lq.init(tid, qstr, dby);
   lg.init(tid, gstr, dby);
   const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse | delta of KB rows
-  auto fetch = [&](int it, int stage) {
-    const int g = it / tq, t = t0 + it - g * tq, head = kvh * group + g;
+  auto fetch = [&](int g, int t, int stage) {
+    const int head = kvh * group + g;
     const long long r = (long long)t * KB;
     lq.load(reinterpret_cast<const T*>(a.q) + (qstart + r) * a.qs + (long long)head * a.qh, qlen - r, qstr, dby, lds0 + stage * 2 * kTile, wave);
     lg.load(reinterpret_cast<const T*>(a.d_o) + (qstart + r) * a.dos + (long long)head * a.doh, qlen - r, gstr, dby,
@@ -301,7 +314,7 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
     }
   };
   const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile + 1024);
-  if (total > 0) fetch(0, 0);
+  if (total > 0) fetch(0, t0, 0);
 
   Frag<T> kf[NCH], vf[NCH];
   {
@@ -312,7 +325,7 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
       kf[c] = global_frag<T>(kr, 16 * c + 8 * h, a.d, there);
-      vf[c] = global_frag<T>(vr, 16 * c + 8 * h, a.d, there);
+      if (DK) vf[c] = global_frag<T>(vr, 16 * c + 8 * h, a.d, there);
     }
   }
   const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
@@ -324,10 +337,12 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
     for (int r = 0; r < 16; r++) ak[b][r] = av[b][r] = 0.f;
   float far_lo = 0.f, far_hi = 0.f;
 
+  int g = 0, t = t0;                                       // this turn's head and tile,
+  int ng = tq > 1 ? 0 : 1, nt = tq > 1 ? t0 + 1 : t0;      // and the next one's
   for (int it = 0; it < total; it++) {
-    const int stage = it & 1, g = it / tq, t = t0 + it - g * tq, r0 = t * KB;
+    const int stage = it & 1, r0 = t * KB;
     if constexpr (BIAS) {
-      if (it == g * tq) {      // another head: its bias
+      if (t == t0) {      // another head: its bias
         __syncthreads();
         fill_bias<NT>(a.bias, a.H, kvh * group + g, 1, const_cast<float*>(bl), tid);
         __syncthreads();
@@ -336,8 +351,10 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
       }
     }
     loads_done_barrier();
-    if (it + 1 < total) fetch(it + 1, stage ^ 1);
-    if (r0 + KB <= wfirst || key0 >= klen) continue;
+    if (it + 1 < total) fetch(ng, nt, stage ^ 1);
+    g = ng;
+    t = nt;
+    if (++nt == t0 + tq) { nt = t0; ng++; }
     const unsigned char* qt = lds + stage * 2 * kTile;
     const unsigned char* gt = qt + kTile;
     const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * 512);
@@ -348,14 +365,17 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
       near = !right && key0 + 31 - (r0 + off) > -md;
     }
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
+    for (int xx = 0; xx < 2 / XH; xx++) {
+      const int x = XH == 2 ? xh : xx;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; c++) s = mma(row_frag<T, D>(qt, rb, x, c), kf[c], s);
-#pragma unroll
-      for (int c = 0; c < NCH; c++) dp = mma(row_frag<T, D>(gt, rb, x, c), vf[c], dp);
+      for (int c = 0; c < NCH; c++) {
+        s = mma(row_frag<T, D>(qt, rb, x, c), kf[c], s);
+        if (DK) dp = mma(row_frag<T, D>(gt, rb, x, c), vf[c], dp);
+      }
+      read_ahead<T, (DK ? 2 : 1) * NCH, 1, 4>();
       const float far = BIAS ? (right ? far_hi : far_lo) : 0.f;
       const float* p = bl + (key - (r0 + 32 * x + 4 * h + off) + md + kPad);
 #pragma unroll
@@ -363,8 +383,8 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
         const f32x4 l2 = *reinterpret_cast<const f32x4*>(rows + 32 * x + 8 * i + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float f = (BIAS && near) ? p[-8 * i - j] : far;
-          s[4 * i + j] = fast_exp2(__builtin_fmaf(s[4 * i + j], sc, f - l2[j]));
+          const float sub = !BIAS ? -l2[j] : (near ? p[-8 * i - j] : far) - l2[j];
+          s[4 * i + j] = fast_exp2(__builtin_fmaf(s[4 * i + j], sc, sub));
         }
       }
       // a row's first positions do not see the wave's last keys; rows behind the sequence and keys behind k_len are zeros in Q,
@@ -378,12 +398,16 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
           if (!(y >= from && y < qlen && key < klen)) { s[r] = 0.f; dp[r] = 0.f; }
         }
       }
+      if constexpr (DV) {
 #pragma unroll
       for (int cc = 0; cc < 2; cc++) {
         const Frag<T> pf = acc_frag<T>(s, cc);
 #pragma unroll
         for (int b = 0; b < NB; b++) av[b] = mma(col_frag<T, D>(gt, cb, x, cc, b), pf, av[b]);
       }
+      read_ahead<T, 2 * NB, 2, 4>();
+      }
+      if constexpr (DK) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const f32x4 dl = *reinterpret_cast<const f32x4*>(rows + 64 + 32 * x + 8 * i + 4 * h);
@@ -396,9 +420,34 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
 #pragma unroll
         for (int b = 0; b < NB; b++) ak[b] = mma(col_frag<T, D>(qt, cb, x, cc, b), df, ak[b]);
       }
+      read_ahead<T, 2 * NB, 2, 4>();
+      }
     }
   }
 
+  {      // the two waves of a block of keys had half of the query rows each
+    float* p = reinterpret_cast<float*>(lds) + kc * NB * 16 * 64 + lane;
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+      if (!(g ? DV : DK)) continue;
+      f32x16* t = g ? av : ak;
+      loads_done_barrier();
+      if (xh == 1) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) p[(b * 16 + r) * 64] = t[b][r];
+      }
+      loads_done_barrier();
+      if (xh == 0) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) t[b][r] += p[(b * 16 + r) * 64];
+      }
+    }
+    if (xh == 1) return;
+  }
   if (key >= kroom) return;
   T* pk = reinterpret_cast<T*>(a.dk) + (long long)(kstart + key) * a.dks + (long long)kvh * a.dkh;
   T* pv = reinterpret_cast<T*>(a.dv) + (long long)(kstart + key) * a.dvs + (long long)kvh * a.dvh;
@@ -408,28 +457,42 @@ __global__ __launch_bounds__(NT, D == 64 ? 2 : 1) void packed_bwd_kv_kernel(cons
     for (int i = 0; i < 4; i++) {
       const int dd = 32 * b + 8 * i + 4 * h;
       if (dd < a.d) {
-        store4(pk + dd, ak[b][4 * i] * a.scale, ak[b][4 * i + 1] * a.scale, ak[b][4 * i + 2] * a.scale, ak[b][4 * i + 3] * a.scale);
-        store4(pv + dd, av[b][4 * i], av[b][4 * i + 1], av[b][4 * i + 2], av[b][4 * i + 3]);
+        if (DK) store4(pk + dd, ak[b][4 * i] * a.scale, ak[b][4 * i + 1] * a.scale, ak[b][4 * i + 2] * a.scale, ak[b][4 * i + 3] * a.scale);
+        if (DV) store4(pv + dd, av[b][4 * i], av[b][4 * i + 1], av[b][4 * i + 2], av[b][4 * i + 3]);
       }
     }
 }
 
+// SPLIT: dK and dV by workgroups of their own (the keys' gradients, which have three products to dV's two, first)
+template <typename T, int D, bool BIAS, bool SPLIT>
+__global__ __launch_bounds__(NT, D == 128 && sizeof(T) == 4 ? 1 : 2) void packed_bwd_kv_kernel(const BwdArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  if constexpr (SPLIT) {
+    const int n = a.knumbers * a.Hk;
+    if ((int)blockIdx.x < n) bwd_kv<T, D, BIAS, 2>(a, blockIdx.x, lds);
+    else bwd_kv<T, D, BIAS, 1>(a, blockIdx.x - n, lds);
+  } else {
+    bwd_kv<T, D, BIAS, 3>(a, blockIdx.x, lds);
+  }
+}
 template <typename K>
 int set_lds(K kernel, int bytes) {
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? AIT_OK : AIT_ELAUNCH;
 }
 template <typename T, int D, bool BIAS>
-int launch(const BwdArgs& a, hipStream_t st) {
+int launch(BwdArgs a, hipStream_t st) {
   const int bias = BIAS ? bias_row(a.bias.max_distance) * 4 : 0;
-  const int qb = 4 * Tile<T, D>::kBytes + bias + (BIAS ? NW * (kHist + a.bias.n_buckets) * 4 : 0), kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
+  const int qb = 4 * Tile<T, D>::kBytes + bias + (BIAS ? NW * (kSums<T, D> + a.bias.n_buckets) * 4 : 0), kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
   AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS>, qb));
-  AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS>, kb));
+  constexpr bool kSplit = D == 128 && sizeof(T) == 2;
+  AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS, kSplit>, kb));
   if (a.s.total_q > 0) {
     hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS>), dim3((unsigned)(a.qnumbers * a.H)), dim3(NT), qb, st, a);
     AIT_CHECK_LAUNCH();
   }
   if (a.s.total_k > 0) {
-    hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS>), dim3((unsigned)(a.knumbers * a.Hk)), dim3(NT), kb, st, a);
+    a.knumbers = (int)block_numbers(a.s.total_k, 1, NW * 16, a.s.n_seq, a.s.rest);
+    hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS, kSplit>), dim3((unsigned)(a.knumbers * a.Hk * (kSplit ? 2 : 1))), dim3(NT), kb, st, a);
     AIT_CHECK_LAUNCH();
   }
   return AIT_OK;
@@ -474,7 +537,7 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
             p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p),
-            (int)block_numbers(p->total_k, 1, BM, p->n_seq, p->zero_rest ? 1 : 0), p->scale, static_cast<float*>(workspace), nullptr, d_table};
+            0, p->scale, static_cast<float*>(workspace), nullptr, d_table};
   if (p->bias_table && d_table) a.part_table = a.delta + (size_t)p->heads * p->total_q;
   const hipStream_t st = ait_stream(stream);
   AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, st) : launch_t<__bf16>(a, st));

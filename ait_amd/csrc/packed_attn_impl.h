@@ -53,6 +53,22 @@ __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int cc) {
   return f;
 }
 
+// The order of a chain of N products whose left operands come from shared memory by R reads each: AHEAD operands are read before
+// the first product, then one more behind every product.  Left alone, the compiler reads an operand, waits for it and multiplies:
+// a trip to shared memory (over 100 cycles) in front of every 32-cycle product.  (f32: an operand feeds 8 products of 64 cycles.)
+template <typename T, int N, int R, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+  if constexpr (sizeof(T) == 2) {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+  }
+}
+
 // ---- tiles in shared memory: KB rows of D values, 16-byte chunk c of row r at position c ^ swz(r) -------------------------
 // Row operands (16 bytes of 32 consecutive rows) and transposed reads (32 bytes of four consecutive rows) both spread over
 // all 64 banks.  Chunk positions differ from chunks in the low bits only, so every offset below is one base XOR a constant.
