@@ -23,7 +23,7 @@ struct FwdArgs {
   long long qs, qh, ks, kh, vs, vh, os, oh;      // row and head strides in elements
   Seqs s;
   Bias bias;
-  int H, Hk, d, causal, pack, splits, numbers;
+  int H, Hk, d, causal, pack, splits, numbers, stages;
   float scale;
   float* part_o;      // [splits][total_q * H][d] unnormalised, and
   float* part_ml;     // [splits][total_q * H][2] maximum, sum: only where splits > 1
@@ -40,7 +40,7 @@ __device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, in
 }
 
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(const FwdArgs a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(const FwdArgs a) {
   constexpr int NT = NW * 64, BM = NW * 32, NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
     lk.load(kb + r * a.ks, klen - r, kstr, dby, lds0 + stage * 2 * kTile, wave);
     lv.load(vb + r * a.vs, klen - r, vstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
   };
-  const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile);
+  const float* bl = reinterpret_cast<const float*>(lds + 2 * a.stages * kTile);
   float far_lo = 0.f, far_hi = 0.f;
   if (t0 < t1) fetch(t0, 0);
   if constexpr (BIAS) {
@@ -121,10 +121,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
   float m = kNegInf, l = 0.f;
 
   for (int t = t0; t < t1; t++) {
-    const int stage = (t - t0) & 1, k0 = t * KB;
+    const int stage = (t - t0) & (a.stages - 1), k0 = t * KB;
     loads_done_barrier();
-    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
-    if (k0 >= wend) continue;
+    if (a.stages == 2 && t + 1 < t1) fetch(t + 1, stage ^ 1);
+    if (k0 < wend) {
     const unsigned char* kt = lds + stage * 2 * kTile;
     const unsigned char* vt = kt + kTile;
     f32x16 s[2];
@@ -135,7 +135,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
 #pragma unroll
     for (int c = 0; c < NCH; c++)
 #pragma unroll
-      for (int x = 0; x < 2; x++) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);
+      for (int x = 0; x < 2; x++)
+        if (sizeof(T) == 2 || x == 0 || k0 + 32 < wend) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);      // (f32: 512 cycles saved)
     read_ahead<T, 2 * NCH, 1, 4>();
     // the block's scores are f * s + add: scaled already where a bias is added value by value
     float f = sc, add = 0.f;
@@ -188,11 +189,17 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(co
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int cc = 0; cc < 2; cc++) {
+        if (sizeof(T) == 4 && k0 + 32 * x + 16 * cc >= wend) continue;
         const Frag<T> pf = acc_frag<T>(s[x], cc);
 #pragma unroll
         for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
       }
     read_ahead<T, 4 * NB, 2, 4>();
+    }
+    if (a.stages == 1 && t + 1 < t1) {
+      loads_done_barrier();
+      fetch(t + 1, 0);
+    }
   }
 
   if (row >= rows) return;
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
 
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
 int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
-  const int bytes = 4 * Tile<T, D>::kBytes + bias_bytes;
+  const int bytes = 2 * a.stages * Tile<T, D>::kBytes + bias_bytes;
   if (hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           bytes) != hipSuccess)
     return AIT_ELAUNCH;
@@ -273,14 +280,17 @@ int launch_nw(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   if (a.bias.table) return a.splits > 1 ? launch<T, D, NW, true, true>(a, bias_bytes, st) : launch<T, D, NW, true, false>(a, bias_bytes, st);
   return a.splits > 1 ? launch<T, D, NW, false, true>(a, 0, st) : launch<T, D, NW, false, false>(a, 0, st);
 }
+template <typename T, int D>
+int launch_d(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
+  return nw == 1 ? launch_nw<T, D, 1>(a, bias_bytes, st) : nw == 2 ? launch_nw<T, D, 2>(a, bias_bytes, st) : launch_nw<T, D, 4>(a, bias_bytes, st);
+}
 template <typename T>
 int launch_t(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
-  if (a.d <= 64) return nw == 1 ? launch_nw<T, 64, 1>(a, bias_bytes, st) : launch_nw<T, 64, 4>(a, bias_bytes, st);
-  return nw == 1 ? launch_nw<T, 128, 1>(a, bias_bytes, st) : launch_nw<T, 128, 4>(a, bias_bytes, st);
+  return a.d <= 64 ? launch_d<T, 64>(a, nw, bias_bytes, st) : launch_d<T, 128>(a, nw, bias_bytes, st);
 }
 
-// what the sizes decide: heads packed to a position, waves of a workgroup, parts of the key axis
-struct Shape { int pack, nw, splits; };
+// what the sizes decide: heads packed to a position, waves of a workgroup, parts of the key axis, tiles in flight
+struct Shape { int pack, nw, splits, stages; };
 Shape shape_of(const ait_packed_attn& p) {
   Shape r;
   const int group = p.heads / p.kv_heads;
@@ -288,9 +298,13 @@ Shape shape_of(const ait_packed_attn& p) {
   // a few new tokens: the heads of a key head fill the 32 columns of one wave
   const bool few = max_q * group <= 32;
   r.pack = few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
-  r.nw = max_q * r.pack <= 32 ? 1 : 4;
+  r.nw = max_q * r.pack <= 32 ? 1 : max_q * r.pack <= 64 ? 2 : 4;
+  // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another
+  r.stages = max_k <= KB ? 1 : 2;
   const long long wgs = block_numbers(p.total_q, r.pack, r.nw * 32, p.n_seq, 1) * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
-  long long s = r.nw == 1 ? (1024 + wgs - 1) / wgs : 1;
+  const int want = r.nw == 1 ? 1024 : 512;
+  long long s = wgs >= want / 2 ? 1 : (want + wgs - 1) / wgs;
+  if (r.nw == 1 && wgs >= want / 2 && wgs < want) s = 2;
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   r.splits = s < 1 ? 1 : (int)s;
@@ -345,11 +359,12 @@ AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long lo
   const Shape sh = shape_of(*p);
   const size_t need = workspace(*p, sh);
   if (need && (!workspace_ptr || workspace_bytes < need)) return AIT_EWORKSPACE;
+  if ((unsigned long long)workspace_ptr % 16) return AIT_EINVAL;
   FwdArgs a{q, k, v, o, lse, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
-            (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), p->scale, nullptr, nullptr};
+            (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, p->scale, nullptr, nullptr};
   if (need) {
     a.part_o = static_cast<float*>(workspace_ptr);
     a.part_ml = a.part_o + (size_t)sh.splits * p->total_q * p->heads * p->d;

@@ -13,7 +13,7 @@
 namespace {
 using namespace ait_packed;
 
-constexpr int NW = 4, NT = NW * 64, BM = NW * 32;
+constexpr int NW = 4, NT = NW * 64;      // waves of the pass over keys
 // The bias's gradient wants the sums of a 32 x 32 block of dS along its diagonals (63 relative positions).  Each query writes its
 // column into a row of its own, shifted so that equal relative positions lie below one another, and a lane adds up one of the
 // 64 columns: plain writes and reads of shared memory.  (Added up by f32 atomics in shared memory instead, a block costs about
@@ -37,28 +37,29 @@ struct BwdArgs {
   long long qs, qh, ks, kh, vs, vh, os, oh, dos, doh, dqs, dqh, dks, dkh, dvs, dvh;
   Seqs s;
   Bias bias;
-  int H, Hk, d, causal, qnumbers, knumbers;
+  int H, Hk, d, causal, qnumbers, knumbers, splits, stages;
   float scale;
   float* delta;       // [H][total_q]
-  float* part_table;  // [qnumbers][H][n_buckets]; null: the table's gradient is not wanted
+  float* part_dq;     // [splits][total_q * H][d], not yet scaled: only where splits > 1
+  float* part_table;  // [splits * qnumbers][H][n_buckets]; null: the table's gradient is not wanted
   float* d_table;
 };
 
-template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_bwd_q_kernel(const BwdArgs a) {
-  constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
+template <typename T, int D, bool BIAS, int NW>
+__global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_bwd_q_kernel(const BwdArgs a) {
+  constexpr int NT = NW * 64, BM = NW * 32, NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int unit = blockIdx.x % a.H, group = a.H / a.Hk, kvh = unit % a.Hk, head = kvh * group + unit / a.Hk;
   const int number = a.qnumbers - 1 - (int)(blockIdx.x / a.H), nb = a.bias.n_buckets, md = a.bias.max_distance;
-  float* part = BIAS && a.part_table ? a.part_table + ((size_t)number * a.H + head) * nb : nullptr;
+  float* part = BIAS && a.part_table ? a.part_table + (((size_t)blockIdx.y * a.qnumbers + number) * a.H + head) * nb : nullptr;
   int seq, block, qstart, qlen, kstart, klen;
   const bool has = find_block(a.s.cu_q, a.s.n_seq, a.s.rest, a.s.total_q, 1, BM, number, seq, block, qstart, qlen);
   if (!has || seq == a.s.n_seq) {
     if constexpr (BIAS)
       if (part)
         for (int b = tid; b < nb; b += NT) part[b] = 0.f;
-    if (!has) return;
+    if (!has || blockIdx.y) return;
     const int r = block * BM + wave * 32 + (lane & 31);
     if (r < qlen)
       for (int e = 8 * h; e < a.d; e += 16) {
@@ -74,7 +75,8 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
   const int wfirst = min(row0, qlen - 1), wlast = min(row0 + 31, qlen - 1);
   const int wsure = a.causal ? min(klen, wfirst + off + 1) : klen, wend = row0 < qlen ? (a.causal ? min(klen, wlast + off + 1) : klen) : 0;
   const int gend = a.causal ? min(klen, min(block * BM + BM, qlen) + off) : klen;
-  const int t1 = gend > 0 ? (gend + KB - 1) / KB : 0;
+  const int tiles = gend > 0 ? (gend + KB - 1) / KB : 0, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = blockIdx.y * per, t1 = min(tiles, t0 + per);
 
   const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lk, lv;
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
     lk.load(kb + r * a.ks, klen - r, kstr, dby, lds0 + stage * 2 * kTile, wave);
     lv.load(vb + r * a.vs, klen - r, vstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
   };
-  if (t1 > 0) fetch(0, 0);
+  if (t0 < t1) fetch(t0, 0);
 
   Frag<T> qf[NCH], gf[NCH];
   float delta = 0.f, l2;
@@ -114,10 +116,10 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
     }
     delta = column_sum(delta);
     l2 = a.lse[(long long)head * a.s.total_q + at];
-    if (row < qlen && h == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
+    if (row < qlen && h == 0 && blockIdx.y == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
     if (row >= qlen) l2 = -kNegInf;
   }
-  float* bl = reinterpret_cast<float*>(lds + 4 * kTile);                 // the head's bias, then per wave: a block's sums by
+  float* bl = reinterpret_cast<float*>(lds + 2 * a.stages * kTile);      // the head's bias, then per wave: a block's sums by
   float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kSums<T, D> + nb);      // relative position, and the sums by bucket
   float* acc_b = hist + kSums<T, D>;
   float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
@@ -139,11 +141,11 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[b][r] = 0.f;
 
-  for (int t = 0; t < t1; t++) {
-    const int stage = t & 1, k0 = t * KB;
+  for (int t = t0; t < t1; t++) {
+    const int stage = (t - t0) & (a.stages - 1), k0 = t * KB;
     loads_done_barrier();
-    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
-    if (k0 >= wend) continue;
+    if (a.stages == 2 && t + 1 < t1) fetch(t + 1, stage ^ 1);
+    if (k0 < wend) {
     const unsigned char* kt = lds + stage * 2 * kTile;
     const unsigned char* vt = kt + kTile;
     bool near = false, right = false;
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
     }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
+      if (sizeof(T) == 4 && k0 + 32 * x >= wend) continue;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
@@ -218,9 +221,23 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
       }
       read_ahead<T, 2 * NB, 2, 4>();
     }
+    }
+    if (a.stages == 1 && t + 1 < t1) {
+      loads_done_barrier();
+      fetch(t + 1, 0);
+    }
   }
 
-  if (row < qlen) {
+  if (row < qlen && a.splits > 1) {
+    float* p = a.part_dq + (((long long)blockIdx.y * a.s.total_q + qstart + pos) * a.H + head) * a.d;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int dd = 32 * b + 8 * i + 4 * h;
+        if (dd < a.d) store4(p + dd, acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]);
+      }
+  } else if (row < qlen) {
     T* p = reinterpret_cast<T*>(a.dq) + (long long)(qstart + pos) * a.dqs + (long long)head * a.dqh;
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -251,13 +268,27 @@ __global__ __launch_bounds__(NT, D == 64 || sizeof(T) == 2 ? 2 : 1) void packed_
   }
 }
 
+// the parts of a row's dQ in their order: one wave per (query row, head)
+template <typename T>
+__global__ __launch_bounds__(256) void packed_dq_join_kernel(const BwdArgs a) {
+  const int dd = (threadIdx.x & 63) * 4;
+  const long long n = (long long)a.s.total_q * a.H, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= n || dd >= a.d) return;
+  const int at = (int)(id / a.H), head = (int)(id - (long long)at * a.H);
+  if (at < clamped(a.s.cu_q, 0, a.s.total_q) || at >= clamped(a.s.cu_q, a.s.n_seq, a.s.total_q)) return;
+  f32x4 u = *reinterpret_cast<const f32x4*>(a.part_dq + id * a.d + dd);
+  for (int s = 1; s < a.splits; s++) u += *reinterpret_cast<const f32x4*>(a.part_dq + (s * n + id) * a.d + dd);
+  u *= a.scale;
+  store4(reinterpret_cast<T*>(a.dq) + (long long)at * a.dqs + (long long)head * a.dqh + dd, u[0], u[1], u[2], u[3]);
+}
+
 // d table[b][head]: the workgroups' parts in a fixed order
 __global__ __launch_bounds__(256) void packed_table_kernel(const BwdArgs a) {
   __shared__ float sums[256];
   const int head = blockIdx.x, b = blockIdx.y * 16 + (threadIdx.x & 15), nb = a.bias.n_buckets;
   float u = 0.f;
   if (b < nb)
-    for (int n = threadIdx.x >> 4; n < a.qnumbers; n += 16) u += a.part_table[((size_t)n * a.H + head) * nb + b];
+    for (int n = threadIdx.x >> 4; n < a.qnumbers * a.splits; n += 16) u += a.part_table[((size_t)n * a.H + head) * nb + b];
   sums[threadIdx.x] = u;
   __syncthreads();
   if (threadIdx.x < 16 && b < nb) {
@@ -479,16 +510,36 @@ template <typename K>
 int set_lds(K kernel, int bytes) {
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? AIT_OK : AIT_ELAUNCH;
 }
-template <typename T, int D, bool BIAS>
+// what the sizes decide for the pass over query rows: waves of a workgroup, parts of the key axis, tiles in flight
+struct Shape { int nw, splits, stages; };
+Shape shape_of(const ait_packed_attn& p) {
+  const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
+  Shape r;
+  r.nw = max_q <= 64 ? 2 : 4;
+  r.stages = max_k <= KB ? 1 : 2;
+  const long long wgs = block_numbers(p.total_q, 1, r.nw * 32, p.n_seq, 1) * p.heads, tiles = (max_k + KB - 1) / KB;
+  long long s = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+  if (s > tiles / 2) s = tiles / 2;
+  if (s > 64) s = 64;
+  r.splits = s < 1 ? 1 : (int)s;
+  return r;
+}
+
+template <typename T, int D, bool BIAS, int NWQ>
 int launch(BwdArgs a, hipStream_t st) {
   const int bias = BIAS ? bias_row(a.bias.max_distance) * 4 : 0;
-  const int qb = 4 * Tile<T, D>::kBytes + bias + (BIAS ? NW * (kSums<T, D> + a.bias.n_buckets) * 4 : 0), kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
-  AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS>, qb));
+  const int qb = 2 * a.stages * Tile<T, D>::kBytes + bias + (BIAS ? NWQ * (kSums<T, D> + a.bias.n_buckets) * 4 : 0);
+  const int kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
   constexpr bool kSplit = D == 128 && sizeof(T) == 2;
+  AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS, NWQ>, qb));
   AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS, kSplit>, kb));
   if (a.s.total_q > 0) {
-    hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS>), dim3((unsigned)(a.qnumbers * a.H)), dim3(NT), qb, st, a);
+    hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS, NWQ>), dim3((unsigned)(a.qnumbers * a.H), (unsigned)a.splits), dim3(NWQ * 64), qb, st, a);
     AIT_CHECK_LAUNCH();
+    if (a.splits > 1) {
+      hipLaunchKernelGGL(packed_dq_join_kernel<T>, dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
+      AIT_CHECK_LAUNCH();
+    }
   }
   if (a.s.total_k > 0) {
     a.knumbers = (int)block_numbers(a.s.total_k, 1, NW * 16, a.s.n_seq, a.s.rest);
@@ -497,18 +548,26 @@ int launch(BwdArgs a, hipStream_t st) {
   }
   return AIT_OK;
 }
-template <typename T>
-int launch_t(const BwdArgs& a, hipStream_t st) {
-  if (a.bias.table) return a.d <= 64 ? launch<T, 64, true>(a, st) : launch<T, 128, true>(a, st);
-  return a.d <= 64 ? launch<T, 64, false>(a, st) : launch<T, 128, false>(a, st);
+template <typename T, int D>
+int launch_d(const BwdArgs& a, int nw, hipStream_t st) {
+  if (a.bias.table) return nw == 2 ? launch<T, D, true, 2>(a, st) : launch<T, D, true, 4>(a, st);
+  return nw == 2 ? launch<T, D, false, 2>(a, st) : launch<T, D, false, 4>(a, st);
 }
-long long q_numbers(const ait_packed_attn& p) { return block_numbers(p.total_q, 1, BM, p.n_seq, p.zero_rest ? 1 : 0); }
+template <typename T>
+int launch_t(const BwdArgs& a, int nw, hipStream_t st) {
+  return a.d <= 64 ? launch_d<T, 64>(a, nw, st) : launch_d<T, 128>(a, nw, st);
+}
+long long q_numbers(const ait_packed_attn& p, const Shape& s) { return block_numbers(p.total_q, 1, s.nw * 32, p.n_seq, p.zero_rest ? 1 : 0); }
+// floats: delta, the parts of dQ, the parts of the table's gradient
+size_t delta_floats(const ait_packed_attn& p) { return ((size_t)p.heads * p.total_q + 3) / 4 * 4; }
+size_t dq_floats(const ait_packed_attn& p, const Shape& s) { return s.splits > 1 ? (size_t)s.splits * p.total_q * p.heads * p.d : 0; }
 }  // namespace
 
 AIT_API size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p) {
   if (ait_packed::check(p) != AIT_OK) return 0;
-  size_t n = (size_t)p->heads * p->total_q;
-  if (p->bias_table) n += (size_t)q_numbers(*p) * p->heads * p->n_buckets;
+  const Shape s = shape_of(*p);
+  size_t n = delta_floats(*p) + dq_floats(*p, s);
+  if (p->bias_table) n += (size_t)s.splits * q_numbers(*p, s) * p->heads * p->n_buckets;
   return n * sizeof(float);
 }
 
@@ -532,15 +591,17 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
   if ((unsigned long long)o_rest % 16) return AIT_EUNSUPPORTED;
   const size_t need = ait_packed_attn_bwd_workspace_bytes(p);
   if (!workspace || workspace_bytes < need) return AIT_EWORKSPACE;
+  if ((unsigned long long)workspace % 16) return AIT_EINVAL;
+  const Shape sh = shape_of(*p);
   BwdArgs a{q, k, v, o, d_o, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
             dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
-            p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p),
-            0, p->scale, static_cast<float*>(workspace), nullptr, d_table};
-  if (p->bias_table && d_table) a.part_table = a.delta + (size_t)p->heads * p->total_q;
+            p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, p->scale,
+            static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, d_table};
+  if (p->bias_table && d_table) a.part_table = a.part_dq + dq_floats(*p, sh);
   const hipStream_t st = ait_stream(stream);
-  AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, st) : launch_t<__bf16>(a, st));
+  AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, sh.nw, st) : launch_t<__bf16>(a, sh.nw, st));
   if (p->bias_table && d_table) {
     if (p->total_q == 0) a.qnumbers = 0;
     hipLaunchKernelGGL(packed_table_kernel, dim3((unsigned)p->heads, (unsigned)((p->n_buckets + 15) / 16)), dim3(256), 0, st, a);

@@ -171,6 +171,33 @@ def test_relative_position_bias(dtype, lens, H, Hk, d, causal, n, m, two):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ql,kl,H,Hk,d,causal,bias,max_q,max_k", [
+    ([40, 64, 3, 0, 33], None, 4, 2, 64, True, True, 64, 64), ([40, 64, 3, 0, 33], None, 2, 2, 128, False, True, 64, 64),
+    ([64], [1500], 2, 1, 64, False, True, 64, 1500), ([50, 9], [700, 1200], 2, 2, 128, True, True, 50, 1200),
+    ([100], [2500], 1, 1, 32, False, False, 100, 2500), ([130, 70, 300], None, 2, 1, 64, True, True, 1, 1), ([130, 300], None, 2, 1, 128, True, False, 64, 64)])
+def test_how_the_work_is_cut_up_does_not_show(dtype, ql, kl, H, Hk, d, causal, bias, max_q, max_k):
+    """small workgroups, one tile at a time, the key axis in parts -- and hints that are too small"""
+    kl = ql if kl is None else kl
+    q, k, v, do = make(ql, kl, H, Hk, d, dtype, 31)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    b = None
+    if bias:
+        b = (torch.randn(12, H, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True), packed.relative_buckets(12, 50, True, "cuda"))
+        leaves.append(b[0])
+    cq, ck = starts(ql), starts(kl)
+    run = lambda: packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=causal, bias=b, max_q=max_q, max_k=max_k)
+    o = run()
+    grads = torch.autograd.grad(o, leaves, do)
+    want = attn_ref(q, k, v, ql, cq.tolist(), kl, ck.tolist(), causal, d ** -0.5, *(b or (None, None)), do=do)
+    for n, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *grads)):
+        within(t, want[n], n)
+    o2 = run()
+    again = torch.autograd.grad(o2, leaves, do)
+    assert torch.equal(o, o2) and all(torch.equal(x, y) for x, y in zip(grads, again)), "not the same twice"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new,kl,cap,H,Hk,d,bias", [
     ([1] * 4, [30, 1, 0, 77], 80, 8, 8, 64, False), ([1] * 2, [5000, 4097], 5001, 8, 2, 128, False), ([1, 1, 3], [700, 64, 65], 900, 32, 4, 64, True),
     ([7], [3000], 3000, 4, 4, 40, True), ([1], [1], 1, 1, 1, 8, True), ([40, 2], [1500, 2], 1600, 8, 2, 64, True)])
