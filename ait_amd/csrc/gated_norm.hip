@@ -45,9 +45,9 @@ struct NormArgs {
 };
 // which parts there are: w_post, w_pre, then scale, b_post, b_pre where given
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int at, int width, bool vec, float* v) {
-  if (vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T* row, int at, int width, float* v) {
+  if constexpr (VEC) {
     if (at < width) {
       if constexpr (sizeof(T) == 2) {
         const bf16x8 t = *reinterpret_cast<const bf16x8*>(row + at);
@@ -67,9 +67,9 @@ __device__ __forceinline__ void load8(const T* row, int at, int width, bool vec,
     for (int e = 0; e < 8; e++) v[e] = at + e < width ? (float)row[at + e] : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* row, int at, int width, bool vec, const float* v) {
-  if (vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T* row, int at, int width, const float* v) {
+  if constexpr (VEC) {
     if (at >= width) return;
     if constexpr (sizeof(T) == 2) {
       bf16x8 t;
@@ -89,6 +89,9 @@ __device__ __forceinline__ void store8(T* row, int at, int width, bool vec, cons
       if (at + e < width) row[at + e] = (T)v[e];
   }
 }
+
+template <bool VEC>
+__device__ __forceinline__ bool inside(int at, int e, int width) { return VEC ? at < width : at + e < width; }
 
 // sums over the G waves of a row, two at a time; every lane gets them.  `slot` alternates so that one barrier a sum is enough
 template <int G>
@@ -123,10 +126,10 @@ __device__ __forceinline__ int seq_of(const int* cu, int n_seq, int rows, int ro
 }
 
 // G waves a row, V blocks of eight values a lane: a row has up to 64 G * 8 V values.  NT threads: NT / 64 / G rows at a time
-template <int G> struct Block { static constexpr int kWaves = G < 4 ? 4 : G, kThreads = kWaves * 64, kRows = kWaves / G; };
+template <int G> struct Block { static constexpr int kRows = G == 1 ? 4 : G == 2 ? 2 : 1, kWaves = G * kRows, kThreads = kWaves * 64; };
 
-template <typename X, typename F, int G, int V>
-__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(const NormArgs a, const bool vec) {
+template <typename X, typename F, int G, int V, bool VEC>
+__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(const NormArgs a) {
   __shared__ float lds[64];
   const int wave = threadIdx.x >> 6, group = wave / G, gl = threadIdx.x - group * G * 64;
   const int row = blockIdx.x * Block<G>::kRows + group, W = a.width;
@@ -139,9 +142,9 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   const bool write = there && (!dead || a.zero_rest);
   float f[V][8], x[V][8];
 #pragma unroll
-  for (int v = 0; v < V; v++) load8(reinterpret_cast<const F*>(a.f) + rc * a.f_row, (gl + v * G * 64) * 8, W, vec, f[v]);
+  for (int v = 0; v < V; v++) load8<VEC>(reinterpret_cast<const F*>(a.f) + rc * a.f_row, (gl + v * G * 64) * 8, W, f[v]);
 #pragma unroll
-  for (int v = 0; v < V; v++) load8(reinterpret_cast<const X*>(a.x) + rc * a.x_row, (gl + v * G * 64) * 8, W, vec, x[v]);
+  for (int v = 0; v < V; v++) load8<VEC>(reinterpret_cast<const X*>(a.x) + rc * a.x_row, (gl + v * G * 64) * 8, W, x[v]);
   float mean = 0.f, s1 = 0.f, s2 = 0.f;
   if (a.layer) {
 #pragma unroll
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   for (int v = 0; v < V; v++)
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      f[v][e] -= (gl + v * G * 64) * 8 + e < W ? mean : 0.f;
+      f[v][e] -= inside<VEC>((gl + v * G * 64) * 8, e, W) ? mean : 0.f;
       s1 = __builtin_fmaf(f[v][e], f[v][e], s1);
     }
   row_sum2<G>(s1, s2, lds, slot, group * G, wave);
@@ -166,21 +169,21 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   for (int v = 0; v < V; v++) {
     const int at = (gl + v * G * 64) * 8;
     float p[8];
-    load8(a.w_post, at, W, vec, p);
+    load8<VEC>(a.w_post, at, W, p);
 #pragma unroll
     for (int e = 0; e < 8; e++) f[v][e] = f[v][e] * r * p[e];
     if (a.b_post) {
-      load8(a.b_post, at, W, vec, p);
+      load8<VEC>(a.b_post, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) f[v][e] += p[e];
     }
     if (a.gate_kind) {
-      load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, W, vec, p);
+      load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) f[v][e] *= p[e];
     }
     if (a.scale) {
-      load8(a.scale, at, W, vec, p);
+      load8<VEC>(a.scale, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) f[v][e] *= p[e];
     }
@@ -193,7 +196,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
 #pragma unroll
       for (int e = 0; e < 8; e++) x[v][e] = 0.f;
     }
-    if (write) store8(reinterpret_cast<X*>(a.y) + rc * a.y_row, at, W, vec, x[v]);
+    if (write) store8<VEC>(reinterpret_cast<X*>(a.y) + rc * a.y_row, at, W, x[v]);
   }
   mean = 0.f;
   if (a.layer) {
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   for (int v = 0; v < V; v++)
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      x[v][e] -= (gl + v * G * 64) * 8 + e < W ? mean : 0.f;
+      x[v][e] -= inside<VEC>((gl + v * G * 64) * 8, e, W) ? mean : 0.f;
       s1 = __builtin_fmaf(x[v][e], x[v][e], s1);
     }
   row_sum2<G>(s1, s2, lds, slot, group * G, wave);
@@ -214,11 +217,11 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   for (int v = 0; v < V; v++) {
     const int at = (gl + v * G * 64) * 8;
     float p[8];
-    load8(a.w_pre, at, W, vec, p);
+    load8<VEC>(a.w_pre, at, W, p);
 #pragma unroll
     for (int e = 0; e < 8; e++) x[v][e] = x[v][e] * ry * p[e];
     if (a.b_pre) {
-      load8(a.b_pre, at, W, vec, p);
+      load8<VEC>(a.b_pre, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) x[v][e] += p[e];
     }
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
 #pragma unroll
       for (int e = 0; e < 8; e++) x[v][e] = 0.f;
     }
-    if (write) store8(reinterpret_cast<F*>(a.h) + rc * a.h_row, at, W, vec, x[v]);
+    if (write) store8<VEC>(reinterpret_cast<F*>(a.h) + rc * a.h_row, at, W, x[v]);
   }
   if (a.stats && there && gl == 0) {
     f32x4 s;
@@ -236,8 +239,9 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
 }
 
 // one workgroup: `per` rows, one behind another per group of waves (a workgroup's groups take them in turn)
-template <typename X, typename F, int G, int V>
-__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(const NormArgs a, const bool vec) {
+// SUMS_B: also the biases' gradients
+template <typename X, typename F, int G, int V, bool VEC, bool SUMS_B>
+__global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(const NormArgs a) {
   constexpr int R = Block<G>::kRows;
   __shared__ float lds[64];
   const int wave = threadIdx.x >> 6, group = wave / G, gl = threadIdx.x - group * G * 64, W = a.width;
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
       // numbers the pairs that meet without a clash
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        store8(gate_parts + (size_t)(unit + seq) * W, (gl + v * G * 64) * 8, W, vec, cg[v]);
+        store8<VEC>(gate_parts + (size_t)(unit + seq) * W, (gl + v * G * 64) * 8, W, cg[v]);
 #pragma unroll
         for (int e = 0; e < 8; e++) cg[v][e] = 0.f;
       }
@@ -273,39 +277,44 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
     const int L = dead ? 0 : W;             // a dead row is a row of zeros, whatever memory holds
     f32x4 st = *reinterpret_cast<const f32x4*>(a.stats + 4ll * rc);
     if (dead) st[0] = st[1] = st[2] = st[3] = 0.f;
-    float f[V][8], y[V][8], g[V][8], d[V][8];
+    float f[V][8], y[V][8], d[V][8], t[V][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int at = (gl + v * G * 64) * 8;
-      float p[8], q[8];
-      load8(reinterpret_cast<const F*>(a.f) + rc * a.f_row, at, L, vec, f[v]);
-      load8(reinterpret_cast<const X*>(a.x) + rc * a.x_row, at, L, vec, y[v]);
-      load8(reinterpret_cast<const F*>(a.dh) + rc * a.dh_row, at, L, vec, d[v]);
-      load8(a.w_post, at, W, vec, p);
+      load8<VEC>(reinterpret_cast<const F*>(a.f) + rc * a.f_row, at, L, f[v]);
+      load8<VEC>(reinterpret_cast<const X*>(a.x) + rc * a.x_row, at, L, y[v]);
+      load8<VEC>(reinterpret_cast<const F*>(a.dh) + rc * a.dh_row, at, L, d[v]);
+      load8<VEC>(reinterpret_cast<const X*>(a.dy) + rc * a.dy_row, at, L, t[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int at = (gl + v * G * 64) * 8;
+      float p[8], q[8], m[8];
+      load8<VEC>(a.w_post, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        f[v][e] = at + e < W ? (f[v][e] - st[0]) * st[1] : 0.f;       // norm(f)
-        g[v][e] = f[v][e] * p[e];                                    // m
+        f[v][e] = inside<VEC>(at, e, W) ? (f[v][e] - st[0]) * st[1] : 0.f;       // norm(f)
+        m[e] = f[v][e] * p[e];
       }
-      if (a.b_post) {
-        load8(a.b_post, at, W, vec, p);
+      if (SUMS_B && a.b_post) {
+        load8<VEC>(a.b_post, at, W, p);
 #pragma unroll
-        for (int e = 0; e < 8; e++) g[v][e] += p[e];
+        for (int e = 0; e < 8; e++) m[e] += p[e];
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] = 1.f;
-      if (a.gate_kind) load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, vec, p);
+      if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) q[e] = 1.f;
-      if (a.scale) load8(a.scale, at, W, vec, q);
+      if (a.scale) load8<VEC>(a.scale, at, W, q);
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[v][e] = at + e < W ? (y[v][e] + g[v][e] * p[e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
-      load8(a.w_pre, at, W, vec, p);
+      for (int e = 0; e < 8; e++) y[v][e] = inside<VEC>(at, e, W) ? (y[v][e] + m[e] * p[e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
+      load8<VEC>(a.w_pre, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         cq[v][e] = __builtin_fmaf(d[v][e], y[v][e], cq[v][e]);
-        bq[v][e] += d[v][e];
+        if (SUMS_B) bq[v][e] += d[v][e];
         d[v][e] *= p[e];
         s1 = __builtin_fmaf(d[v][e], y[v][e], s1);
         s2 += d[v][e];
@@ -318,31 +327,34 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int at = (gl + v * G * 64) * 8;
-      float p[8], q[8], u[8];
-      load8(reinterpret_cast<const X*>(a.dy) + rc * a.dy_row, at, L, vec, u);
+      float p[8], q[8], m[8], b[8];
+      float* u = t[v];
 #pragma unroll
       for (int e = 0; e < 8; e++) u[e] = u[e] + st[3] * (d[v][e] - s2 - y[v][e] * s1);        // d y
-      if (write) store8(reinterpret_cast<X*>(a.dx) + rc * a.dx_row, at, W, vec, u);
+      if (write) store8<VEC>(reinterpret_cast<X*>(a.dx) + rc * a.dx_row, at, W, u);
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] = q[e] = 1.f;
-      if (a.gate_kind) load8(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, vec, p);
-      if (a.scale) load8(a.scale, at, W, vec, q);
+      if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
+      if (a.scale) load8<VEC>(a.scale, at, W, q);
+      load8<VEC>(a.w_post, at, W, m);
+#pragma unroll
+      for (int e = 0; e < 8; e++) b[e] = 0.f;
+      if (SUMS_B && a.b_post) load8<VEC>(a.b_post, at, W, b);
       float k[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float um = u[e] * g[v][e];
+        const float um = u[e] * (f[v][e] * m[e] + b[e]);
         cs[v][e] = __builtin_fmaf(um, p[e], cs[v][e]);
         k[e] = um * q[e];                                            // d gate
         cg[v][e] += k[e];
         u[e] *= p[e] * q[e];                                         // d m
-        bp[v][e] += u[e];
+        if (SUMS_B) bp[v][e] += u[e];
         cp[v][e] = __builtin_fmaf(u[e], f[v][e], cp[v][e]);
       }
-      if (a.gate_kind == 1 && there) store8(reinterpret_cast<F*>(a.dgate) + rc * a.dg_row, at, W, vec, k);
-      load8(a.w_post, at, W, vec, p);
+      if (a.gate_kind == 1 && there) store8<VEC>(reinterpret_cast<F*>(a.dgate) + rc * a.dg_row, at, W, k);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        d[v][e] = u[e] * p[e];
+        d[v][e] = u[e] * m[e];
         t1 = __builtin_fmaf(d[v][e], f[v][e], t1);
         t2 += d[v][e];
       }
@@ -354,7 +366,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
     for (int v = 0; v < V; v++) {
 #pragma unroll
       for (int e = 0; e < 8; e++) d[v][e] = st[1] * (d[v][e] - t2 - f[v][e] * t1);
-      if (write) store8(reinterpret_cast<F*>(a.df) + rc * a.df_row, (gl + v * G * 64) * 8, W, vec, d[v]);
+      if (write) store8<VEC>(reinterpret_cast<F*>(a.df) + rc * a.df_row, (gl + v * G * 64) * 8, W, d[v]);
     }
   }
   if (unit >= a.units) return;
@@ -363,12 +375,12 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
   for (int v = 0; v < V; v++) {
     const int at = (gl + v * G * 64) * 8;
     float* p = parts;
-    store8(p, at, W, vec, cp[v]);
-    store8(p += W, at, W, vec, cq[v]);
-    if (a.scale) store8(p += W, at, W, vec, cs[v]);
-    if (a.b_post) store8(p += W, at, W, vec, bp[v]);
-    if (a.b_pre) store8(p += W, at, W, vec, bq[v]);
-    if (a.gate_kind == 2 && first < a.rows && seq < a.n_seq) store8(gate_parts + (size_t)(unit + seq) * W, at, W, vec, cg[v]);
+    store8<VEC>(p, at, W, cp[v]);
+    store8<VEC>(p += W, at, W, cq[v]);
+    if (a.scale) store8<VEC>(p += W, at, W, cs[v]);
+    if (SUMS_B && a.b_post) store8<VEC>(p += W, at, W, bp[v]);
+    if (SUMS_B && a.b_pre) store8<VEC>(p += W, at, W, bq[v]);
+    if (a.gate_kind == 2 && first < a.rows && seq < a.n_seq) store8<VEC>(gate_parts + (size_t)(unit + seq) * W, at, W, cg[v]);
   }
 }
 
@@ -382,8 +394,17 @@ __global__ __launch_bounds__(1024) void gated_norm_sum_kernel(const SumArgs a) {
   __shared__ float sums[1024];
   const int t = threadIdx.x, n = a.n_parts * a.width, c = blockIdx.x * 16 + (t & 15);
   float u = 0.f;
-  if (c < n)
-    for (int i = t >> 4; i < a.units; i += 64) u += a.parts[(size_t)i * n + c];
+  if (c < n) {
+    int i = t >> 4;
+    for (; i + 448 < a.units; i += 512) {          // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = a.parts[(size_t)(i + 64 * j) * n + c];
+#pragma unroll
+      for (int j = 0; j < 8; j++) u += v[j];
+    }
+    for (; i < a.units; i += 64) u += a.parts[(size_t)i * n + c];
+  }
   sums[t] = u;
   __syncthreads();
   for (int o = 32; o > 0; o >>= 1) {
@@ -403,30 +424,54 @@ __global__ __launch_bounds__(256) void gated_norm_gate_kernel(const NormArgs a) 
   const int start = clamp_row(a.cu, b, a.rows), end = clamp_row(a.cu, b + 1, a.rows);
   const float* parts = a.parts + (size_t)a.units * a.n_parts * a.width;
   float u = 0.f;
-  if (end > start)
-    for (int i = start / a.per; i <= (end - 1) / a.per; i++) u += parts[(size_t)(i + b) * a.width + c];
+  if (end > start) {
+    int i = start / a.per;
+    const int last = (end - 1) / a.per;
+    for (; i + 7 <= last; i += 8) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = parts[(size_t)(i + j + b) * a.width + c];
+#pragma unroll
+      for (int j = 0; j < 8; j++) u += v[j];
+    }
+    for (; i <= last; i++) u += parts[(size_t)(i + b) * a.width + c];
+  }
   reinterpret_cast<F*>(a.dgate)[(long long)b * a.dg_row + c] = (F)u;
 }
 
 constexpr int kMaxWidth = 8192;
 bool aligned(const void* p, long long row, int es) { return !p || ((unsigned long long)p % 16 == 0 && (row * es) % 16 == 0); }
 
-template <typename X, typename F, bool BWD, int G, int V>
-int launch_gv(const NormArgs& a, bool vec, hipStream_t st) {
+template <typename X, typename F, bool BWD, bool VEC, int G, int V>
+int launch_gv(const NormArgs& a, hipStream_t st) {
   const int rows = BWD ? a.units : a.rows;
   const dim3 grid((unsigned)((rows + Block<G>::kRows - 1) / Block<G>::kRows)), block(Block<G>::kThreads);
-  if constexpr (BWD) hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V>), grid, block, 0, st, a, vec);
-  else hipLaunchKernelGGL((gated_norm_fwd_kernel<X, F, G, V>), grid, block, 0, st, a, vec);
+  if constexpr (BWD) {
+    if (a.b_post || a.b_pre) hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V, VEC, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V, VEC, false>), grid, block, 0, st, a);
+  } else hipLaunchKernelGGL((gated_norm_fwd_kernel<X, F, G, V, VEC>), grid, block, 0, st, a);
   AIT_CHECK_LAUNCH();
   return AIT_OK;
 }
 template <typename X, typename F, bool BWD>
 int launch_xf(const NormArgs& a, bool vec, hipStream_t st) {
-  if (a.width <= 512) return launch_gv<X, F, BWD, 1, 1>(a, vec, st);
-  if (a.width <= 1024) return launch_gv<X, F, BWD, 2, 1>(a, vec, st);
-  if (a.width <= 2048) return launch_gv<X, F, BWD, 4, 1>(a, vec, st);
-  if (a.width <= 4096) return launch_gv<X, F, BWD, 8, 1>(a, vec, st);
-  return launch_gv<X, F, BWD, 8, 2>(a, vec, st);
+  // as many waves as the row fills: one block of eight values a lane up to 4096, two beyond
+  if (!vec) {
+    if (a.width <= 512) return launch_gv<X, F, BWD, false, 1, 1>(a, st);
+    if (a.width <= 2048) return launch_gv<X, F, BWD, false, 4, 1>(a, st);
+    return a.width <= 4096 ? launch_gv<X, F, BWD, false, 8, 1>(a, st) : launch_gv<X, F, BWD, false, 8, 2>(a, st);
+  }
+  switch ((a.width + 511) / 512) {
+    case 1: return launch_gv<X, F, BWD, true, 1, 1>(a, st);
+    case 2: return launch_gv<X, F, BWD, true, 2, 1>(a, st);
+    case 3: return launch_gv<X, F, BWD, true, 3, 1>(a, st);
+    case 4: return launch_gv<X, F, BWD, true, 4, 1>(a, st);
+    case 5: case 6: return launch_gv<X, F, BWD, true, 6, 1>(a, st);
+    case 7: case 8: return launch_gv<X, F, BWD, true, 8, 1>(a, st);
+    case 9: case 10: return launch_gv<X, F, BWD, true, 5, 2>(a, st);
+    case 11: case 12: return launch_gv<X, F, BWD, true, 6, 2>(a, st);
+    default: return launch_gv<X, F, BWD, true, 8, 2>(a, st);
+  }
 }
 template <bool BWD>
 int launch(const ait_gated_norm& p, const NormArgs& a, bool vec, hipStream_t st) {
@@ -463,7 +508,7 @@ bool inputs_aligned(const ait_gated_norm& p) {
 }
 // units of the backward: about two workgroups' groups a CU, each with a run of rows
 void units_of(const ait_gated_norm& p, int& units, int& per) {
-  const int groups = p.width <= 512 ? 2048 : p.width <= 1024 ? 1024 : p.width <= 2048 ? 512 : 256;
+  const int groups = p.width <= 512 ? 2048 : p.width <= 1024 ? 1024 : 512;
   per = p.rows > 0 ? (p.rows + groups - 1) / groups : 1;
   units = (p.rows + per - 1) / per;
 }

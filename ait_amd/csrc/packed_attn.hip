@@ -104,11 +104,14 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
   float far_lo = 0.f, far_hi = 0.f;
   if (t0 < t1) fetch(t0, 0);
   if constexpr (BIAS) {
-    fill_bias<NT>(a.bias, a.H, head0, a.pack, const_cast<float*>(bl), tid);
-    __syncthreads();
-    bl += (head - head0) * bias_row(a.bias.max_distance);
-    far_lo = bl[0];
-    far_hi = bl[2 * (a.bias.max_distance + kPad)];
+    const int md = a.bias.max_distance, first = block * BM / a.pack, last = (min(block * BM + BM, rows) - 1) / a.pack;
+    far_lo = bias_log2(a.bias.table[(size_t)bucket(a.bias, -md) * a.H + head]);
+    far_hi = bias_log2(a.bias.table[(size_t)bucket(a.bias, md) * a.H + head]);
+    if (t1 * KB - 1 - (first + off) > -md && t0 * KB - (last + off) < md) {      // (else every key is in the outermost buckets)
+      fill_bias<NT>(a.bias, a.H, head0, a.pack, const_cast<float*>(bl), tid);
+      __syncthreads();
+      bl += (head - head0) * bias_row(md);
+    }
   }
 
   const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
@@ -233,8 +236,10 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
   }
 }
 
-// the splits of a row joined, in their order: one wave per (query row, head)
-template <typename T>
+// The parts of a row joined: one wave per (query row, head).  A lane has one part's maximum and sum (there are at most 64); then
+// LD lanes take four values each and 64 / LD parts go at a time, added up in a fixed order.
+constexpr int kMaxSplits = 64;
+template <typename T, int LD>
 __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
   const int lane = threadIdx.x & 63;
   const long long n = (long long)a.s.total_q * a.H, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -242,22 +247,28 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
   const int at = (int)(id / a.H);
   const bool in = at >= clamped(a.s.cu_q, 0, a.s.total_q) && at < clamped(a.s.cu_q, a.s.n_seq, a.s.total_q);
   if (!in && !a.s.rest) return;                          // no sequence's row: left as it is, or set to zero
-  const int head = (int)(id - (long long)at * a.H), dd = lane * 4, splits = in ? a.splits : 0;
-  float m = kNegInf;
-  for (int s = 0; s < splits; s++) m = fmaxf(m, a.part_ml[2 * (s * n + id)]);
-  const float mu = m == kNegInf ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-  for (int s = 0; s < splits; s++) {
-    const float w = fast_exp2(a.part_ml[2 * (s * n + id)] - mu), ls = a.part_ml[2 * (s * n + id) + 1];
-    l += w * ls;
-    if (dd < a.d) {
-      const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (s * n + id) * a.d + dd);
-      o0 += w * p[0]; o1 += w * p[1]; o2 += w * p[2]; o3 += w * p[3];
-    }
+  const int head = (int)(id - (long long)at * a.H), dd = (lane % LD) * 4, splits = in ? a.splits : 0;
+  float m = kNegInf, l = 0.f;
+  if (lane < splits) {
+    m = a.part_ml[2 * (lane * n + id)];
+    l = a.part_ml[2 * (lane * n + id) + 1];
   }
+  const float top = wave_max(m), w = fast_exp2(m - (top == kNegInf ? 0.f : top));      // (NaN scores leave m alone and make l NaN)
+  l = wave_sum(lane < splits ? l * w : 0.f);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < splits; s0 += 64 / LD) {
+    const int s = s0 + lane / LD;
+    const float ws = __shfl(w, s & 63, 64);
+    if (s < splits && dd < a.d) o += *reinterpret_cast<const f32x4*>(a.part_o + (s * n + id) * a.d + dd) * ws;
+  }
+#pragma unroll
+  for (int x = LD; x < 64; x *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], x, 64);
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (a.lse && lane == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? -kNegInf : m + __builtin_amdgcn_logf(l);
-  if (dd < a.d) store_o<T>(a, reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, at, head, dd, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+  if (a.lse && lane == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? -kNegInf : top + __builtin_amdgcn_logf(l);
+  if (lane < LD && dd < a.d)
+    store_o<T>(a, reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, at, head, dd, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
@@ -270,7 +281,7 @@ int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
                      bytes, st, a);
   AIT_CHECK_LAUNCH();
   if constexpr (SPLIT) {
-    hipLaunchKernelGGL((packed_join_kernel<T>), dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((packed_join_kernel<T, D / 4>), dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
     AIT_CHECK_LAUNCH();
   }
   return AIT_OK;
@@ -306,7 +317,7 @@ Shape shape_of(const ait_packed_attn& p) {
   long long s = wgs >= want / 2 ? 1 : (want + wgs - 1) / wgs;
   if (r.nw == 1 && wgs >= want / 2 && wgs < want) s = 2;
   if (s > tiles / 2) s = tiles / 2;
-  if (s > 64) s = 64;
+  if (s > kMaxSplits) s = kMaxSplits;
   r.splits = s < 1 ? 1 : (int)s;
   return r;
 }

@@ -249,15 +249,25 @@ __device__ __forceinline__ int clamped(const int* cu, int i, int total) {
 // With `rest` the rows behind the last sequence count as one more, number n_seq: the blocks that set them to zero.
 __device__ __forceinline__ bool find_block(const int* cu, int n_seq, int rest, int total, int mul, int bm, int number, int& seq, int& block,
                                            int& start, int& len) {
-  int lo = 0, hi = n_seq - 1 + rest;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int)((long long)clamped(cu, mid, total) * mul / bm) + mid <= number) lo = mid;
-    else hi = mid - 1;
+  // 64 candidates at a time, one per lane: up to 64 sequences cost one trip to memory
+  const int lane = threadIdx.x & 63;
+  int lo = 0, count = n_seq + rest, begin = 0, end = 0;
+  while (true) {
+    const int step = (count + 63) / 64, b = lo + lane * step;
+    const bool there = lane * step < count;
+    const int c = there ? clamped(cu, b, total) : 0, e = !there ? 0 : b < n_seq ? clamped(cu, b + 1, total) : total;
+    // (the first candidate counts in any case; what follows a later one is later, in a table that ascends)
+    const unsigned long long ok = __ballot(there && (lane == 0 || (int)((long long)c * mul / bm) + b <= number));
+    const int t = 63 - __builtin_clzll(ok);
+    lo += t * step;
+    count = min(step, count - t * step);
+    begin = __builtin_amdgcn_readlane(c, t);
+    end = __builtin_amdgcn_readlane(e, t);
+    if (step == 1) break;
   }
   seq = lo;
-  start = clamped(cu, lo, total);
-  len = (lo < n_seq ? clamped(cu, lo + 1, total) : total) - start;
+  start = begin;
+  len = end - begin;
   block = number - (int)((long long)start * mul / bm) - lo;
   return block >= 0 && (long long)block * bm < (long long)len * mul;
 }
@@ -304,9 +314,10 @@ __device__ __forceinline__ float bias_log2(float t) {
 template <int NT>
 __device__ __forceinline__ void fill_bias(const Bias& b, int H, int head0, int heads, float* lds, int tid) {
   const int w = bias_row(b.max_distance);
-  for (int g = 0; g < heads; g++)
-    for (int x = tid; x < w; x += NT)
-      lds[g * w + x] = bias_log2(b.table[(size_t)bucket(b, x - b.max_distance - kPad) * H + head0 + g]);
+  for (int x = tid; x < w; x += NT) {
+    const float* t = b.table + (size_t)bucket(b, x - b.max_distance - kPad) * H + head0;
+    for (int g = 0; g < heads; g++) lds[g * w + x] = bias_log2(t[g]);
+  }
 }
 
 int check(const ait_packed_attn* p);
