@@ -141,6 +141,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
       for (int x = 0; x < 2; x++)
         if (sizeof(T) == 2 || x == 0 || k0 + 32 < wend) s[x] = mma(row_frag<T, D>(kt, rb, x, c), qf[c], s[x]);      // (f32: 512 cycles saved)
     read_ahead<T, 2 * NCH, 1, 4>();
+    const FirstCols<T, D> first(vt, cb, 0);
     // the block's scores are f * s + add: scaled already where a bias is added value by value
     float f = sc, add = 0.f;
     if constexpr (BIAS) {
@@ -195,9 +196,9 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
         if (sizeof(T) == 4 && k0 + 32 * x + 16 * cc >= wend) continue;
         const Frag<T> pf = acc_frag<T>(s[x], cc);
 #pragma unroll
-        for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
+        for (int b = 0; b < NB; b++) acc[b] = mma(x == 0 ? first.get(vt, cb, x, cc, b) : col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
       }
-    read_ahead<T, 4 * NB, 2, 4>();
+    read_ahead<T, 4 * NB, 2, 4, true>();
     }
     if (a.stages == 1 && t + 1 < t1) {
       loads_done_barrier();

@@ -165,6 +165,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
         dp = mma(row_frag<T, D>(vt, rb, x, c), gf[c], dp);
       }
       read_ahead<T, 2 * NCH, 1, 4>();
+      const FirstCols<T, D> first(kt, cb, x);
       if (BIAS && near) {
         const float* p = bl + (k0 + 32 * x + 4 * h - (pos + off) + md + kPad);
 #pragma unroll
@@ -217,9 +218,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
       for (int cc = 0; cc < 2; cc++) {
         const Frag<T> df = acc_frag<T>(s, cc);
 #pragma unroll
-        for (int b = 0; b < NB; b++) acc[b] = mma(col_frag<T, D>(kt, cb, x, cc, b), df, acc[b]);
+        for (int b = 0; b < NB; b++) acc[b] = mma(first.get(kt, cb, x, cc, b), df, acc[b]);
       }
-      read_ahead<T, 2 * NB, 2, 4>();
+      read_ahead<T, 2 * NB, 2, 4, true>();
     }
     }
     if (a.stages == 1 && t + 1 < t1) {
@@ -330,22 +331,40 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   lq.init(tid, qstr, dby);
   lg.init(tid, gstr, dby);
   const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse | delta of KB rows
-  auto fetch = [&](int g, int t, int stage) {
-    const int head = kvh * group + g;
-    const long long r = (long long)t * KB;
-    lq.load(reinterpret_cast<const T*>(a.q) + (qstart + r) * a.qs + (long long)head * a.qh, qlen - r, qstr, dby, lds0 + stage * 2 * kTile, wave);
-    lg.load(reinterpret_cast<const T*>(a.d_o) + (qstart + r) * a.dos + (long long)head * a.doh, qlen - r, gstr, dby,
-            lds0 + stage * 2 * kTile + kTile, wave);
+  // the next tile to load: its head, number, rows and rows left (pointers run on: a head's tiles lie one behind another)
+  const T *pq = nullptr, *pg = nullptr;
+  const float* ps = nullptr;
+  int nt = t0, nhead = kvh * group, left = 0;
+  auto to_head = [&]() {
+    const long long r = qstart + (long long)t0 * KB;
+    pq = reinterpret_cast<const T*>(a.q) + r * a.qs + (long long)nhead * a.qh;
+    pg = reinterpret_cast<const T*>(a.d_o) + r * a.dos + (long long)nhead * a.doh;
+    ps = (wave ? a.delta : a.lse) + (long long)nhead * a.s.total_q + r;
+    left = qlen - t0 * KB;
+  };
+  auto fetch = [&](int stage) {
+    lq.load(pq, left, qstr, dby, lds0 + stage * 2 * kTile, wave);
+    lg.load(pg, left, gstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
     if (wave < 2) {
-      const float* src = (wave ? a.delta : a.lse) + (long long)head * a.s.total_q + qstart + r;
-      const int n = (int)min((long long)KB, qlen - r);
-      const i32x4 rsrc = tile_rsrc(src, n * 4);
+      const i32x4 rsrc = tile_rsrc(ps, min(KB, left) * 4);
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
-                   : : "v"(lane * 4), "s"(rsrc), "s"((unsigned)__builtin_amdgcn_readfirstlane((int)(rows0 + stage * 512 + wave * 256))) : "m0", "memory");
+                   : : "v"(lane * 4), "s"(rsrc), "s"(rows0 + stage * 512 + wave * 256) : "m0", "memory");
+    }
+    pq += KB * a.qs;
+    pg += KB * a.dos;
+    ps += KB;
+    left -= KB;
+    if (++nt == t0 + tq) {
+      nt = t0;
+      nhead++;
+      to_head();
     }
   };
   const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile + 1024);
-  if (total > 0) fetch(0, t0, 0);
+  if (total > 0) {
+    to_head();
+    fetch(0);
+  }
 
   Frag<T> kf[NCH], vf[NCH];
   {
@@ -368,8 +387,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     for (int r = 0; r < 16; r++) ak[b][r] = av[b][r] = 0.f;
   float far_lo = 0.f, far_hi = 0.f;
 
-  int g = 0, t = t0;                                       // this turn's head and tile,
-  int ng = tq > 1 ? 0 : 1, nt = tq > 1 ? t0 + 1 : t0;      // and the next one's
+  int g = 0, t = t0;
   for (int it = 0; it < total; it++) {
     const int stage = it & 1, r0 = t * KB;
     if constexpr (BIAS) {
@@ -382,10 +400,8 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       }
     }
     loads_done_barrier();
-    if (it + 1 < total) fetch(ng, nt, stage ^ 1);
-    g = ng;
-    t = nt;
-    if (++nt == t0 + tq) { nt = t0; ng++; }
+    if (it + 1 < total) fetch(stage ^ 1);
+    if (++t == t0 + tq) { t = t0; g++; }
     const unsigned char* qt = lds + stage * 2 * kTile;
     const unsigned char* gt = qt + kTile;
     const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * 512);
@@ -395,9 +411,8 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       right = key0 - (last + off) >= md;
       near = !right && key0 + 31 - (r0 + off) > -md;
     }
-#pragma unroll
-    for (int xx = 0; xx < 2 / XH; xx++) {
-      const int x = XH == 2 ? xh : xx;
+    const int x = xh;
+    {
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
@@ -407,6 +422,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
         if (DK) dp = mma(row_frag<T, D>(gt, rb, x, c), vf[c], dp);
       }
       read_ahead<T, (DK ? 2 : 1) * NCH, 1, 4>();
+      const FirstCols<T, D> first(DV ? gt : qt, cb, x);
       const float far = BIAS ? (right ? far_hi : far_lo) : 0.f;
       const float* p = bl + (key - (r0 + 32 * x + 4 * h + off) + md + kPad);
 #pragma unroll
@@ -420,8 +436,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       }
       // a row's first positions do not see the wave's last keys; rows behind the sequence and keys behind k_len are zeros in Q,
       // dO, K and V, but their "probabilities" are not
-      const bool edge = r0 < wsure || r0 + KB > qlen || key0 + 32 > klen;
-      if (edge) {
+      if (r0 < wsure || r0 + KB > qlen || key0 + 32 > klen) {
         const int from = a.causal ? key - off : 0;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
@@ -434,9 +449,9 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       for (int cc = 0; cc < 2; cc++) {
         const Frag<T> pf = acc_frag<T>(s, cc);
 #pragma unroll
-        for (int b = 0; b < NB; b++) av[b] = mma(col_frag<T, D>(gt, cb, x, cc, b), pf, av[b]);
+        for (int b = 0; b < NB; b++) av[b] = mma(first.get(gt, cb, x, cc, b), pf, av[b]);
       }
-      read_ahead<T, 2 * NB, 2, 4>();
+      read_ahead<T, 2 * NB, 2, 4, true>();
       }
       if constexpr (DK) {
 #pragma unroll
@@ -449,9 +464,9 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       for (int cc = 0; cc < 2; cc++) {
         const Frag<T> df = acc_frag<T>(s, cc);
 #pragma unroll
-        for (int b = 0; b < NB; b++) ak[b] = mma(col_frag<T, D>(qt, cb, x, cc, b), df, ak[b]);
+        for (int b = 0; b < NB; b++) ak[b] = mma(DV ? col_frag<T, D>(qt, cb, x, cc, b) : first.get(qt, cb, x, cc, b), df, ak[b]);
       }
-      read_ahead<T, 2 * NB, 2, 4>();
+      read_ahead<T, 2 * NB, 2, 4, !DV>();
       }
     }
   }

@@ -56,10 +56,11 @@ __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int cc) {
 // The order of a chain of N products whose left operands come from shared memory by R reads each: AHEAD operands are read before
 // the first product, then one more behind every product.  Left alone, the compiler reads an operand, waits for it and multiplies:
 // a trip to shared memory (over 100 cycles) in front of every 32-cycle product.  (f32: an operand feeds 8 products of 64 cycles.)
-template <typename T, int N, int R, int AHEAD>
+// READ: the first AHEAD operands are there already.
+template <typename T, int N, int R, int AHEAD, bool READ = false>
 __device__ __forceinline__ void read_ahead() {
   if constexpr (sizeof(T) == 2) {
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
+    if constexpr (!READ) __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
 #pragma unroll
     for (int i = 0; i < N - AHEAD; i++) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -138,6 +139,27 @@ __device__ __forceinline__ Frag<T> col_frag(const unsigned char* tile, int base,
     return f;
   }
 }
+
+// The first four transposed operands of a product, read before what comes between it and the product in front (exponentials,
+// selects, branches: the compiler moves no read across them).  f32 operands are eight reads each and feed 512 cycles: not kept.
+template <typename T, int D>
+struct FirstCols {
+  static constexpr int NB = D / 32;
+  Frag<T> f[sizeof(T) == 2 ? 4 : 1];
+  __device__ __forceinline__ FirstCols(const unsigned char* tile, int base, int rt) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) f[i] = col_frag<T, D>(tile, base, rt, i / NB, i % NB);
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+    }
+  }
+  __device__ __forceinline__ Frag<T> get(const unsigned char* tile, int base, int rt, int cc, int b) const {
+    if constexpr (sizeof(T) == 2) {
+      if (cc * NB + b < 4) return f[(cc * NB + b) & 3];
+    }
+    return col_frag<T, D>(tile, base, rt, cc, b);
+  }
+};
 
 // ---- global -> shared memory -----------------------------------------------------------------------------------------------
 // 16 bytes a lane straight into shared memory.  The buffer descriptor ends behind the sequence's last row (tile by tile: a
