@@ -225,7 +225,7 @@ class PackedAttn(ctypes.Structure):
     """ait_packed_attn."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("cu_q", "cu_k", "k_len", "bias_table", "bucket_of")] + \
         [(n, ctypes.c_int) for n in ("n_seq", "total_q", "total_k", "max_q", "max_k", "heads", "kv_heads", "d", "dtype", "causal",
-                                     "n_buckets", "max_distance", "zero_rest")] + [("scale", ctypes.c_float)]
+                                     "n_buckets", "max_distance", "table_dtype", "zero_rest")] + [("scale", ctypes.c_float)]
 
 
 class GatedNorm(ctypes.Structure):

@@ -105,8 +105,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
   if (t0 < t1) fetch(t0, 0);
   if constexpr (BIAS) {
     const int md = a.bias.max_distance, first = block * BM / a.pack, last = (min(block * BM + BM, rows) - 1) / a.pack;
-    far_lo = bias_log2(a.bias.table[(size_t)bucket(a.bias, -md) * a.H + head]);
-    far_hi = bias_log2(a.bias.table[(size_t)bucket(a.bias, md) * a.H + head]);
+    far_lo = bias_log2(a.bias, (size_t)bucket(a.bias, -md) * a.H + head);
+    far_hi = bias_log2(a.bias, (size_t)bucket(a.bias, md) * a.H + head);
     if (t1 * KB - 1 - (first + off) > -md && t0 * KB - (last + off) < md) {      // (else every key is in the outermost buckets)
       fill_bias<NT>(a.bias, a.H, head0, a.pack, const_cast<float*>(bl), tid);
       __syncthreads();
@@ -275,7 +275,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
 int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   const int bytes = 2 * a.stages * Tile<T, D>::kBytes + bias_bytes;
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+  if (bytes > 65536 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           bytes) != hipSuccess)
     return AIT_ELAUNCH;
   hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), dim3((unsigned)(a.numbers * (a.H / a.pack)), (unsigned)a.splits), dim3(NW * 64),
@@ -313,10 +314,10 @@ Shape shape_of(const ait_packed_attn& p) {
   r.nw = max_q * r.pack <= 32 ? 1 : max_q * r.pack <= 64 ? 2 : 4;
   // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another
   r.stages = max_k <= KB ? 1 : 2;
-  const long long wgs = block_numbers(p.total_q, r.pack, r.nw * 32, p.n_seq, 1) * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
-  const int want = r.nw == 1 ? 1024 : 512;
-  long long s = wgs >= want / 2 ? 1 : (want + wgs - 1) / wgs;
-  if (r.nw == 1 && wgs >= want / 2 && wgs < want) s = 2;
+  // few rows leave most of the chip idle: the key axis is cut until there are about 2048 waves, two tiles at least to a part
+  const long long rows = (long long)p.total_q * r.pack, blocks = rows / (r.nw * 32) > p.n_seq ? rows / (r.nw * 32) : p.n_seq;
+  const long long wgs = blocks * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB, want = 2048 / (r.nw == 4 ? 4 : r.nw == 2 ? 2 : 1);
+  long long s = wgs > want / 2 ? 1 : (want + wgs - 1) / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > kMaxSplits) s = kMaxSplits;
   r.splits = s < 1 ? 1 : (int)s;
@@ -336,6 +337,7 @@ int check(const ait_packed_attn* p) {
   if (p->d > 128 || p->d % 8) return AIT_EUNSUPPORTED;
   if (p->bias_table) {
     if (!p->bucket_of || p->n_buckets <= 0 || p->max_distance < 0) return AIT_EINVAL;
+    if (p->table_dtype != AIT_DTYPE_F32 && p->table_dtype != AIT_DTYPE_BF16) return AIT_EINVAL;
     if (p->n_buckets > AIT_MAX_BUCKETS || p->max_distance > AIT_MAX_BIAS_DISTANCE) return AIT_EUNSUPPORTED;
   }
   if ((p->n_seq > 0 && p->total_q > 0) && (!p->cu_q || !p->cu_k)) return AIT_EINVAL;
@@ -374,7 +376,7 @@ AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long lo
   if ((unsigned long long)workspace_ptr % 16) return AIT_EINVAL;
   FwdArgs a{q, k, v, o, lse, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
-            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
+            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
             (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, p->scale, nullptr, nullptr};
   if (need) {

@@ -42,7 +42,7 @@ struct BwdArgs {
   float* delta;       // [H][total_q]
   float* part_dq;     // [splits][total_q * H][d], not yet scaled: only where splits > 1
   float* part_table;  // [splits * qnumbers][H][n_buckets]; null: the table's gradient is not wanted
-  float* d_table;
+  void* d_table;
 };
 
 template <typename T, int D, bool BIAS, int NW>
@@ -296,7 +296,9 @@ __global__ __launch_bounds__(256) void packed_table_kernel(const BwdArgs a) {
     u = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i++) u += sums[threadIdx.x + 16 * i];
-    a.d_table[(size_t)b * a.H + head] = u;
+    const size_t at = (size_t)b * a.H + head;
+    if (a.bias.bf16) static_cast<__bf16*>(a.d_table)[at] = (__bf16)u;
+    else static_cast<float*>(a.d_table)[at] = u;
   }
 }
 
@@ -523,6 +525,7 @@ __global__ __launch_bounds__(NT, D == 128 && sizeof(T) == 4 ? 1 : 2) void packed
 }
 template <typename K>
 int set_lds(K kernel, int bytes) {
+  if (bytes <= 65536) return AIT_OK;
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? AIT_OK : AIT_ELAUNCH;
 }
 // what the sizes decide for the pass over query rows: waves of a workgroup, parts of the key axis, tiles in flight
@@ -532,8 +535,10 @@ Shape shape_of(const ait_packed_attn& p) {
   Shape r;
   r.nw = max_q <= 64 ? 2 : 4;
   r.stages = max_k <= KB ? 1 : 2;
-  const long long wgs = block_numbers(p.total_q, 1, r.nw * 32, p.n_seq, 1) * p.heads, tiles = (max_k + KB - 1) / KB;
-  long long s = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+  // (as in the forward)
+  const long long blocks = p.total_q / (r.nw * 32) > p.n_seq ? p.total_q / (r.nw * 32) : p.n_seq;
+  const long long wgs = blocks * p.heads, tiles = (max_k + KB - 1) / KB, want = 2048 / r.nw;
+  long long s = wgs > want / 2 ? 1 : (want + wgs - 1) / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   r.splits = s < 1 ? 1 : (int)s;
@@ -590,7 +595,7 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
                                 long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
                                 long long o_head, const void* o_rest, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
                                 long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
-                                long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream) {
+                                long long dv_row, long long dv_head, void* d_table, void* workspace, size_t workspace_bytes, void* stream) {
   AIT_TRY_RC(ait_packed::check(p));
   if (p->n_seq == 0 || (p->total_q == 0 && p->total_k == 0)) return AIT_OK;
   if (!p->cu_q || !p->cu_k) return AIT_EINVAL;
@@ -611,7 +616,7 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
   BwdArgs a{q, k, v, o, d_o, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
             dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
-            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance},
+            {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, p->scale,
             static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, d_table};
   if (p->bias_table && d_table) a.part_table = a.part_dq + dq_floats(*p, sh);

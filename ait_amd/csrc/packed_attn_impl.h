@@ -317,9 +317,9 @@ __device__ __forceinline__ void keys_of(const Seqs& s, int seq, int& start, int&
 // A workgroup keeps the values of its heads in shared memory, kPad of the outermost ones on either side: a 64 x 32 block that
 // touches the inner range reads them at one address per lane plus constants; a block that does not adds one constant.
 struct Bias {
-  const float* table;      // [n_buckets, H]; null: no bias
+  const void* table;       // [n_buckets, H], f32 or bf16; null: no bias
   const int* bucket_of;    // [2 max_distance + 1], by key - query + max_distance
-  int n_buckets, max_distance;
+  int n_buckets, max_distance, bf16;
 };
 constexpr int kPad = 96;
 __host__ __device__ static inline int bias_row(int max_distance) { return 2 * (max_distance + kPad) + 1; }
@@ -328,8 +328,8 @@ __device__ __forceinline__ int bucket(const Bias& b, int rel) {
   return v < 0 ? 0 : v >= b.n_buckets ? b.n_buckets - 1 : v;
 }
 // in units of the exponent to base 2.  The lowest finite values stay finite: a row that sees nothing else still has its softmax
-__device__ __forceinline__ float bias_log2(float t) {
-  const float v = t * kLog2e;
+__device__ __forceinline__ float bias_log2(const Bias& b, size_t at) {
+  const float t = b.bf16 ? (float)static_cast<const __bf16*>(b.table)[at] : static_cast<const float*>(b.table)[at], v = t * kLog2e;
   return (v == kNegInf && t != kNegInf) ? -3.402823466e38f : v;
 }
 
@@ -337,8 +337,8 @@ template <int NT>
 __device__ __forceinline__ void fill_bias(const Bias& b, int H, int head0, int heads, float* lds, int tid) {
   const int w = bias_row(b.max_distance);
   for (int x = tid; x < w; x += NT) {
-    const float* t = b.table + (size_t)bucket(b, x - b.max_distance - kPad) * H + head0;
-    for (int g = 0; g < heads; g++) lds[g * w + x] = bias_log2(t[g]);
+    const size_t at = (size_t)bucket(b, x - b.max_distance - kPad) * H + head0;
+    for (int g = 0; g < heads; g++) lds[g * w + x] = bias_log2(b, at + g);
   }
 }
 

@@ -843,16 +843,16 @@ def packed_attn_desc(q, k, v, cu_q, cu_k, k_len=None, max_q=None, max_k=None, ca
     if k_len is not None:
         k_len = _index(op, "k_len", k_len, n, dev)
     if table is not None:
-        if not (torch.is_tensor(table) and table.dim() == 2 and table.shape[1] == H and table.shape[0] > 0 and table.dtype == torch.float32
+        if not (torch.is_tensor(table) and table.dim() == 2 and table.shape[1] == H and table.shape[0] > 0 and table.dtype in _lib.DTYPES
                 and table.device == dev):
-            _refuse(op, "the bias table must be a float32 [n_buckets, %d] tensor on %s", H, dev)
+            _refuse(op, "the bias table must be a float32 or bfloat16 [n_buckets, %d] tensor on %s", H, dev)
         if not (torch.is_tensor(bucket_of) and bucket_of.dim() == 1 and bucket_of.numel() % 2 == 1):
             _refuse(op, "`bucket_of` must have 2 * max_distance + 1 values")
         bucket_of = _index(op, "bucket_of", bucket_of, bucket_of.numel(), dev)
         if table.shape[0] > _lib.MAX_BUCKETS or bucket_of.numel() // 2 > _lib.MAX_BIAS_DISTANCE:
             _refuse(op, "at most %d buckets and a distance of %d", _lib.MAX_BUCKETS, _lib.MAX_BIAS_DISTANCE)
         table = table.contiguous()
-        p.n_buckets, p.max_distance = table.shape[0], bucket_of.numel() // 2
+        p.n_buckets, p.max_distance, p.table_dtype = table.shape[0], bucket_of.numel() // 2, _lib.DTYPES[table.dtype]
     if not q.is_cuda:
         raise _lib.AitHipError("tensor must live on a GPU (got %s): the hot path has no CPU fallback" % dev)
     p.n_seq, p.total_q, p.total_k, p.heads, p.kv_heads, p.d = n, tq, tk, H, Hk, d
@@ -882,7 +882,7 @@ def packed_attn_fwd(p, q, k, v, out=None, for_backward=False):
     dev = q.device
     q, k, v = _fit(q), _fit(k), _fit(v)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         p.zero_rest = 1
         if p.n_seq == 0:
             out.zero_()
@@ -895,7 +895,7 @@ def packed_attn_fwd(p, q, k, v, out=None, for_backward=False):
     if for_backward:
         lse = torch.empty((p.heads, p.total_q), dtype=torch.float32, device=dev)
         if q.dtype == torch.bfloat16:
-            rest = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            rest = torch.empty_like(q, memory_format=torch.contiguous_format)
     with _lib.on_device(dev):
         n = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -907,17 +907,17 @@ def packed_attn_fwd(p, q, k, v, out=None, for_backward=False):
 
 
 def packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=False):
-    """ait_packed_attn_bwd: (dq, dk, dv, d_table f32 [n_buckets, heads] or None)"""
+    """ait_packed_attn_bwd: (dq, dk, dv, d_table as the table or None)"""
     L = _lib.lib()
     dev = q.device
     q, k, v, o, d_o = _fit(q), _fit(k), _fit(v), _fit(o), _fit(d_o)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     p.zero_rest = 1
     if p.n_seq == 0:
         dq.zero_(), dk.zero_(), dv.zero_()
     dt = None
     if want_table:
-        dt = torch.empty((p.n_buckets, p.heads), dtype=torch.float32, device=dev)
+        dt = torch.empty((p.n_buckets, p.heads), dtype=torch.bfloat16 if p.table_dtype else torch.float32, device=dev)
         if p.n_seq == 0 or p.total_q == 0:
             dt.zero_()
     with _lib.on_device(dev):
@@ -1001,7 +1001,7 @@ def gated_norm_point(p, x, f, gate, cu_seqlens, w_post, b_post, w_pre, b_pre, sc
 def gated_norm_fwd(p, x, f, want_stats=False):
     """ait_gated_norm_fwd: y as x, h as f, stats [rows, 4] or None"""
     dev = x.device
-    y, h = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(f.shape, dtype=f.dtype, device=dev)
+    y, h = torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty_like(f, memory_format=torch.contiguous_format)
     stats = torch.empty((p.rows, 4), dtype=torch.float32, device=dev) if want_stats else None
     with _lib.on_device(dev):
         rc = _lib.lib().ait_gated_norm_fwd(ctypes.byref(p), y.data_ptr(), p.width, h.data_ptr(), p.width,
@@ -1016,7 +1016,7 @@ def gated_norm_bwd(p, x, f, gate, stats, dy, dh):
     L = _lib.lib()
     dev = x.device
     dy, dh = _rows2d(dy), _rows2d(dh)
-    e = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+    e = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
     dx, df, dg = e(x), e(f), e(gate)
     n = 2 + sum(t is not None for t in (p.scale, p.b_post, p.b_pre))
     flat = torch.empty((n, p.width), dtype=torch.float32, device=dev)

@@ -24,10 +24,10 @@ def _recorded(*tensors):
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of):
-        p, keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, None if table is None else table.float(), bucket_of)
+        p, keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)
         o, lse, rest = ops.packed_attn_fwd(p, q, k, v, for_backward=True)
         ctx.save_for_backward(q, k, v, o, lse, rest, *keep)
-        ctx.p, ctx.table_dtype = p, None if table is None else table.dtype
+        ctx.p = p
         return o
 
     @staticmethod
@@ -37,8 +37,8 @@ class _PackedAttention(torch.autograd.Function):
         p, n = _lib.PackedAttn.from_buffer_copy(ctx.p), ctx.needs_input_grad
         ops.packed_attn_point(p, *keep)
         dq, dk, dv, dt = ops.packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=n[3])
-        return dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, None if dt is None else dt.to(ctx.table_dtype), \
-            None, None, None, None, None, None, None, None
+        return dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, dt, None, None, None, None, \
+            None, None, None, None
 
 
 def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=None, causal=False, scale=None, bias=None):
@@ -57,13 +57,11 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
     table = bucket_of = None
     if bias is not None:
         table, bucket_of = (bias.weight, bias.bucket_of) if isinstance(bias, RelativePositionBias) else bias
-        if not torch.is_tensor(table) or table.dtype not in _lib.DTYPES:
-            raise _lib.AitHipError("packed_attn: the bias table must be a float32 or bfloat16 tensor")
     if cu_k is None:
         cu_k = cu_q
     if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded(q, k, v, table):
         return _PackedAttention.apply(q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of)
-    p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, None if table is None else table.float(), bucket_of)
+    p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)
     return ops.packed_attn_fwd(p, q, k, v)[0]
 
 

@@ -888,14 +888,15 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *     but the order of sums depends on them.
  *   dtype AIT_DTYPE_F32 (exact f32 products) or AIT_DTYPE_BF16 (f32 scores, statistics and sums; probabilities and dS are
  *     rounded to bf16 where they enter a product) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
- *   bias_table f32 [n_buckets, heads] or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
+ *   bias_table [n_buckets, heads] of table_dtype (AIT_DTYPE_*), or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
  *     table): the bucket of relative position key - query, where the last query is level with the last key; further away the
  *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
  *   For the backward, else NULL: lse f32 [heads, total_q], the binary logarithm of a row's sum of exp (+infinity where a query
  *     sees no key); o_rest [total_q, heads, d] contiguous, AIT_DTYPE_BF16 only: what rounding took from o, without which the
  *     gradients of q and k carry o's rounding error.
  *
- * Backward: dq / dk / dv (pitches as given), and with a bias d_table f32 [n_buckets, heads] (overwritten; NULL: not wanted).
+ * Backward: dq / dk / dv (pitches as given), and with a bias d_table [n_buckets, heads] of table_dtype
+ * (overwritten; summed in f32; NULL: not wanted).
  * No atomics on memory: results are the same from run to run, and do not depend on what else runs.
  * Workspaces: the caller's, used by one call at a time.
  * ------------------------------------------------------------------------------------- */
@@ -907,11 +908,11 @@ typedef struct {
   const int32_t* cu_q;
   const int32_t* cu_k;
   const int32_t* k_len;
-  const float* bias_table;
+  const void* bias_table;
   const int32_t* bucket_of;
   int n_seq, total_q, total_k, max_q, max_k;
   int heads, kv_heads, d, dtype, causal;
-  int n_buckets, max_distance, zero_rest;
+  int n_buckets, max_distance, table_dtype, zero_rest;
   float scale;
 } ait_packed_attn;
 size_t ait_packed_attn_fwd_workspace_bytes(const ait_packed_attn* p);
@@ -923,7 +924,7 @@ int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row
                         long long k_head, const void* v, long long v_row, long long v_head, const void* o, long long o_row,
                         long long o_head, const void* o_rest, const void* d_o, long long do_row, long long do_head, const float* lse, void* dq,
                         long long dq_row, long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
-                        long long dv_row, long long dv_head, float* d_table, void* workspace, size_t workspace_bytes, void* stream);
+                        long long dv_row, long long dv_head, void* d_table, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * The norm behind a block, its gate and residual scale, the residual, and the norm in front of the next block, fused: the rows

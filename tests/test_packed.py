@@ -29,7 +29,7 @@ def attn_ref(q, k, v, ql, qs, kl, ks, causal, scale, table=None, bucket_of=None,
     z = lambda t: torch.zeros_like(t)
     o, eo, dq, edq, dk, edk, dv, edv = z(q), z(q), z(q), z(q), z(k), z(k), z(v), z(v)
     if table is not None:
-        table, bucket_of = table.detach().cpu().to(F8), bucket_of.cpu().long()
+        table_type, table, bucket_of = table.dtype, table.detach().cpu().to(F8), bucket_of.cpu().long()
         m = bucket_of.numel() // 2
         dt, edt = z(table), z(table)
     do = None if do is None else do.detach().cpu().to(F8)
@@ -87,7 +87,8 @@ def attn_ref(q, k, v, ql, qs, kl, ks, causal, scale, table=None, bucket_of=None,
         r = lambda x, e: (x, e + u * (x.abs() + e))
         out.update(dq=r(dq, edq), dk=r(dk, edk), dv=r(dv, edv))
         if table is not None:
-            out["dt"] = (dt, edt + 64 * f * dt.abs())
+            edt = edt + 64 * f * dt.abs()
+            out["dt"] = (dt, edt + torch.finfo(table_type).eps / 2 * (dt.abs() + edt))
     return out
 
 
@@ -157,7 +158,7 @@ def test_queries_and_keys_of_different_lengths(dtype, ql, kl, H, Hk, d, causal):
     ([500], 1, 1, 32, True, 16, 9, False), ([40, 64, 3], 8, 8, 64, False, 16, 2000, True)])
 def test_relative_position_bias(dtype, lens, H, Hk, d, causal, n, m, two):
     q, k, v, do = make(lens, lens, H, Hk, d, dtype, 11 + m)
-    bias = packed.RelativePositionBias(H, n, m, two).cuda()
+    bias = packed.RelativePositionBias(H, n, m, two).to("cuda", dtype if H > 1 else torch.float32)
     with torch.no_grad():
         bias.weight.copy_(torch.randn(n, H, generator=torch.Generator().manual_seed(5)))
     leaves = [t.requires_grad_(True) for t in (q, k, v)] + [bias.weight]
@@ -167,6 +168,7 @@ def test_relative_position_bias(dtype, lens, H, Hk, d, causal, n, m, two):
     want = attn_ref(q, k, v, lens, cu.tolist(), lens, cu.tolist(), causal, d ** -0.5, bias.weight, bias.bucket_of, do)
     for name, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *grads)):
         within(t, want[name], name)
+    assert grads[3].dtype == bias.weight.dtype
 
 
 @pytest.mark.gpu
