@@ -314,10 +314,12 @@ Shape shape_of(const ait_packed_attn& p) {
   r.nw = max_q * r.pack <= 32 ? 1 : max_q * r.pack <= 64 ? 2 : 4;
   // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another
   r.stages = max_k <= KB ? 1 : 2;
-  // few rows leave most of the chip idle: the key axis is cut until there are about 2048 waves, two tiles at least to a part
+  // Few rows leave most of the chip idle: the key axis is cut, two tiles at least to a part.  As many parts as fit the chip at
+  // once with two workgroups a CU (a round more costs as much as all of them: 64 queries against 2394 keys in f32 took
+  // 37 us in 19 parts, 608 workgroups); of the single waves of new tokens twice as many, whose time is their loads'
   const long long rows = (long long)p.total_q * r.pack, blocks = rows / (r.nw * 32) > p.n_seq ? rows / (r.nw * 32) : p.n_seq;
-  const long long wgs = blocks * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB, want = 2048 / (r.nw == 4 ? 4 : r.nw == 2 ? 2 : 1);
-  long long s = wgs > want / 2 ? 1 : (want + wgs - 1) / wgs;
+  const long long wgs = blocks * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
+  long long s = r.nw == 1 ? (1024 + wgs - 1) / wgs : 512 / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > kMaxSplits) s = kMaxSplits;
   r.splits = s < 1 ? 1 : (int)s;

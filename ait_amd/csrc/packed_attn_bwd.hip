@@ -537,8 +537,8 @@ Shape shape_of(const ait_packed_attn& p) {
   r.stages = max_k <= KB ? 1 : 2;
   // (as in the forward)
   const long long blocks = p.total_q / (r.nw * 32) > p.n_seq ? p.total_q / (r.nw * 32) : p.n_seq;
-  const long long wgs = blocks * p.heads, tiles = (max_k + KB - 1) / KB, want = 2048 / r.nw;
-  long long s = wgs > want / 2 ? 1 : (want + wgs - 1) / wgs;
+  const long long wgs = blocks * p.heads, tiles = (max_k + KB - 1) / KB;
+  long long s = 512 / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   r.splits = s < 1 ? 1 : (int)s;
