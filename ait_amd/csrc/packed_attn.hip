@@ -308,8 +308,8 @@ Shape shape_of(const ait_packed_attn& p) {
   Shape r;
   const int group = p.heads / p.kv_heads;
   const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
-  // a few new tokens: the heads of a key head fill the 32 columns of one wave
-  const bool few = max_q * group <= 32;
+  // a few new tokens: the heads of a key head share a workgroup's columns, and its keys are read once
+  const bool few = max_q * group <= 128;
   r.pack = few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
   r.nw = max_q * r.pack <= 32 ? 1 : max_q * r.pack <= 64 ? 2 : 4;
   // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another
@@ -318,7 +318,7 @@ Shape shape_of(const ait_packed_attn& p) {
   // once with two workgroups a CU (a round more costs as much as all of them: 64 queries against 2394 keys in f32 took
   // 37 us in 19 parts, 608 workgroups); of the single waves of new tokens twice as many, whose time is their loads'
   const long long rows = (long long)p.total_q * r.pack, blocks = rows / (r.nw * 32) > p.n_seq ? rows / (r.nw * 32) : p.n_seq;
-  const long long wgs = blocks * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
+  const long long wgs = (blocks > 0 ? blocks : 1) * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
   long long s = r.nw == 1 ? (1024 + wgs - 1) / wgs : 512 / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > kMaxSplits) s = kMaxSplits;

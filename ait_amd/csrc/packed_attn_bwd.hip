@@ -117,7 +117,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
     delta = column_sum(delta);
     l2 = a.lse[(long long)head * a.s.total_q + at];
     if (row < qlen && h == 0 && blockIdx.y == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
-    if (row >= qlen) l2 = -kNegInf;
+    // (a query that sees one key has no gradient of its scores: exactly zero, not the rounding of dP - delta)
+    if (row >= qlen || kmax <= 1) l2 = -kNegInf;
   }
   float* bl = reinterpret_cast<float*>(lds + 2 * a.stages * kTile);      // the head's bias, then per wave: a block's sums by
   float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kSums<T, D> + nb);      // relative position, and the sums by bucket
@@ -436,14 +437,24 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
           s[4 * i + j] = fast_exp2(__builtin_fmaf(s[4 * i + j], sc, sub));
         }
       }
+      if constexpr (DK) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(rows + 64 + 32 * x + 8 * i + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; j++) dp[4 * i + j] -= dl[j];
+        }
+      }
       // a row's first positions do not see the wave's last keys; rows behind the sequence and keys behind k_len are zeros in Q,
-      // dO, K and V, but their "probabilities" are not
+      // dO, K and V, but their "probabilities" are not; a query that sees one key has no gradient of its scores
       if (r0 < wsure || r0 + KB > qlen || key0 + 32 > klen) {
-        const int from = a.causal ? key - off : 0;
+        const int from = a.causal ? key - off : 0, one = klen <= 1 ? qlen : a.causal ? -off : -1;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int y = r0 + 32 * x + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (!(y >= from && y < qlen && key < klen)) { s[r] = 0.f; dp[r] = 0.f; }
+          const bool seen = y >= from && y < qlen && key < klen;
+          if (!seen) s[r] = 0.f;
+          if (!seen || y <= one) dp[r] = 0.f;
         }
       }
       if constexpr (DV) {
@@ -457,11 +468,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       }
       if constexpr (DK) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(rows + 64 + 32 * x + 8 * i + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[4 * i + j] *= dp[4 * i + j] - dl[j];
-      }
+      for (int r = 0; r < 16; r++) s[r] *= dp[r];
 #pragma unroll
       for (int cc = 0; cc < 2; cc++) {
         const Frag<T> df = acc_frag<T>(s, cc);
@@ -537,7 +544,7 @@ Shape shape_of(const ait_packed_attn& p) {
   r.stages = max_k <= KB ? 1 : 2;
   // (as in the forward)
   const long long blocks = p.total_q / (r.nw * 32) > p.n_seq ? p.total_q / (r.nw * 32) : p.n_seq;
-  const long long wgs = blocks * p.heads, tiles = (max_k + KB - 1) / KB;
+  const long long wgs = (blocks > 0 ? blocks : 1) * p.heads, tiles = (max_k + KB - 1) / KB;
   long long s = 512 / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;

@@ -806,7 +806,7 @@ def _fit(t):
     v = 16 // es
     (rows, heads, _), (sr, sh, se) = t.shape, t.stride()
     ok = se == 1 and t.data_ptr() % 16 == 0 and (rows < 2 or (sr % v == 0 and sr * es < 2 ** 25)) and (heads < 2 or sh % v == 0)
-    return t if ok or t.numel() == 0 else t.contiguous()
+    return t if ok or t.numel() == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _row_head(t):

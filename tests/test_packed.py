@@ -296,6 +296,13 @@ def test_c_entries_refuse_bad_arguments():
     p = dict(n_seq=2, total_q=2, total_k=20000, max_q=1, max_k=10000)
     need = L.ait_packed_attn_fwd_workspace_bytes(ctypes.byref(_lib.PackedAttn(**{**base, **p})))
     assert need > 0 and fwd(**p) == EWORKSPACE
+    # sizes of nothing are sizes too
+    for kw in (dict(n_seq=0), dict(n_seq=0, total_q=0, total_k=0), dict(total_q=0), dict(total_k=0), dict(total_q=1, max_q=1, total_k=0)):
+        for f in (L.ait_packed_attn_fwd_workspace_bytes, L.ait_packed_attn_bwd_workspace_bytes):
+            assert f(ctypes.byref(_lib.PackedAttn(**{**base, **kw}))) < 1 << 20
+    assert L.ait_packed_attn_fwd_workspace_bytes(None) == 0 and L.ait_packed_attn_bwd_workspace_bytes(None) == 0
+    assert L.ait_gated_norm_bwd_workspace_bytes(None) == 0
+    assert L.ait_gated_norm_bwd_workspace_bytes(ctypes.byref(_lib.GatedNorm(w_post=4096, w_pre=4096, rows=0, width=8))) == 0
 
 
 # ------------------------------------------------------------------------------------------
@@ -450,3 +457,287 @@ def test_gated_norm_refuses_what_it_does_not_take():
             assert f(**kw) == -4, kw
     assert fwd(y=None) == -1 and fwd(yr=31) == -1
     assert bwd(ws=None) == -2 and bwd(n=64) == -2 and bwd(scale=4096) == -1 and bwd(gate=4096, gate_row=32) == -1
+
+
+# ------------------------------------------------------------------------------------------
+# what calls may do
+# ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_key_has_no_gradient_of_its_score(dtype):
+    ql, kl = [3, 0, 70, 1], [1, 1, 1, 0]
+    q, k, v, do = make(ql, kl, 4, 2, 96, dtype, 3)
+    table, of = torch.randn(8, 4).cuda().requires_grad_(True), packed.relative_buckets(8, 20, True, "cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)] + [table]
+    o = packed.packed_attention(q, k, v, starts(ql).cuda(), starts(kl).cuda(), bias=(table, of))
+    dq, dk, dv, dt = torch.autograd.grad(o, leaves, do)
+    assert all(bool((t == 0).all()) for t in (dq, dk, dt))
+    want = attn_ref(q, k, v, ql, starts(ql).tolist(), kl, starts(kl).tolist(), False, 96 ** -0.5, table, of, do)
+    within(o, want["o"], "o")
+    within(dv, want["dv"], "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+def test_any_scale(scale):
+    lens = [70, 130]
+    q, k, v, do = make(lens, lens, 2, 1, 64, torch.float32, 5)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    cu = starts(lens)
+    o = packed.packed_attention(q, k, v, cu.cuda(), causal=True, scale=scale)
+    want = attn_ref(q, k, v, lens, cu.tolist(), lens, cu.tolist(), True, scale, do=do)
+    for n, t in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, do))):
+        within(t, want[n], n)
+
+
+@pytest.mark.gpu
+def test_many_short_sequences():
+    """more sequences than one look at 64 starts, and than two"""
+    g = torch.Generator().manual_seed(9)
+    lens = torch.randint(0, 4, (4300,), generator=g).tolist()
+    q, k, v, do = make(lens, lens, 1, 1, 16, torch.float32, 9)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    cu = starts(lens)
+    o = packed.packed_attention(q, k, v, cu.cuda(), causal=True, max_q=3, max_k=3)
+    want = attn_ref(q, k, v, lens, cu.tolist(), lens, cu.tolist(), True, 0.25, do=do)
+    for n, t in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, do))):
+        within(t, want[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["heads first", "one key head for all", "odd rows", "unaligned", "backwards gradient"])
+def test_layouts(layout):
+    lens, dt = [37, 90], torch.bfloat16
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    n, H, d = sum(lens), 4, 64
+    q, k, v, do = r(n, H, d), r(n, H, d), r(n, H, d), r(n, H, d)
+    if layout == "heads first":
+        q, k, v, do = (t.permute(1, 0, 2).contiguous().permute(1, 0, 2) for t in (q, k, v, do))
+    if layout == "one key head for all":
+        k, v = k[:, :1].expand(n, H, d), v[:, :1].expand(n, H, d)
+    if layout == "odd rows":
+        q, k, v = (torch.cat([t.reshape(n, -1), t.reshape(n, -1)[:, :3]], 1)[:, :H * d].view(n, H, d) for t in (q, k, v))
+    if layout == "unaligned":
+        q, k, v = (torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(n, H, d) for t in (q, k, v))
+    if layout == "backwards gradient":
+        do = do.flip(2)[:, :, ::2].repeat_interleave(2, 2)[..., :d].transpose(0, 2).contiguous().transpose(0, 2)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    cu = starts(lens)
+    o = packed.packed_attention(*leaves, cu.cuda(), causal=True)
+    want = attn_ref(q, k, v, lens, cu.tolist(), lens, cu.tolist(), True, d ** -0.5, do=do)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, do))):
+        within(t, want[name], name)
+
+
+@pytest.mark.gpu
+def test_offsets_past_four_gibibytes():
+    """a cache of 2.2 million rows: a sequence far behind the start, and one that is itself longer than 32-bit offsets"""
+    rows, Hk, d, dt = 2200000, 8, 128, torch.bfloat16
+    k, v = torch.zeros(rows, Hk, d, dtype=dt, device="cuda"), torch.zeros(rows, Hk, d, dtype=dt, device="cuda")
+    g = torch.Generator().manual_seed(4)
+    k[-200:], v[-200:] = torch.randn(200, Hk, d, generator=g).to(dt).cuda(), torch.randn(200, Hk, d, generator=g).to(dt).cuda()
+    q = torch.randn(2, Hk, d, generator=g).to(dt).cuda()
+    cu = torch.tensor([0, rows - 200, rows], dtype=torch.int32).cuda()
+    o = packed.packed_attention(q, k, v, starts([1, 1]).cuda(), cu, k_len=torch.tensor([3, 200], dtype=torch.int32).cuda(), causal=True, max_q=1, max_k=200)
+    want = attn_ref(q, k[-200:], v[-200:], [0, 1], [0, 1], [0, 200], [0, 0], True, d ** -0.5)["o"]
+    within(o[1], tuple(t[1] for t in want), "o")
+    assert bool((o[0] == 0).all())
+    # all keys before the last 200 are zero, and so are their values: they only add exp(-top) each to the sums
+    q = q[:1] * 4
+    o = packed.packed_attention(q, k, v, starts([1]).cuda(), torch.tensor([0, rows], dtype=torch.int32).cuda(), causal=True, max_q=1, max_k=rows)
+    s = torch.einsum("hd,khd->hk", q[0].cpu().to(F8), k[-200:].cpu().to(F8)) * d ** -0.5
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    p = p / (p.sum(1, keepdim=True) + (rows - 200) * torch.exp(-s.amax(1, keepdim=True)))
+    vv = v[-200:].cpu().to(F8).permute(1, 0, 2)
+    ref, size = torch.matmul(p[:, None], vv)[:, 0], torch.matmul(p[:, None], vv.abs())[:, 0]
+    # u for a probability, u for the result; 2^-11 for a sum of 2.2 million equal terms, 34000 a lane at worst
+    within(o[0], (ref, size * (2 ** -8 + 2 ** -11) + 2 ** -8 * ref.abs()), "o")
+
+
+@pytest.mark.gpu
+def test_a_given_output_keeps_its_other_rows():
+    lens = [20, 45]
+    q, k, v, _ = make(lens, lens, 2, 2, 64, torch.bfloat16, 6)
+    cu = starts(lens).cuda()
+    out = torch.full((q.shape[0], 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    p, keep = ops.packed_attn_desc(q, k, v, cu, cu, causal=True)
+    got, _, _ = ops.packed_attn_fwd(p, q, k, v, out=out[:, 1:3])
+    assert got.data_ptr() == out[:, 1:3].data_ptr()
+    assert torch.equal(got[:65], packed.packed_attention(q, k, v, cu, causal=True)[:65])
+    assert bool((out[65:] == 7).all()) and bool((out[:, 0] == 7).all()) and bool((out[:, 3] == 7).all())
+    for bad in (out[:, :2].float(), out[:-1, :2], out[:, :1].expand(-1, 2, -1), out[:, 1:3, :].transpose(1, 2).contiguous().transpose(1, 2)):
+        with pytest.raises(_lib.AitHipError):
+            ops.packed_attn_fwd(p, q, k, v, out=bad)
+    empty = packed.packed_attention(q[:0], k[:0], v[:0], torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert empty.shape == (0, 2, 64)
+    none = packed.packed_attention(q, k, v, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert bool((none == 0).all())
+
+
+def _step(x, w, cu, table, of):
+    """a training step's operators on packed rows, everything a gradient flows to returned"""
+    q, k, v = (x @ w[i] for i in range(3))
+    n, H = x.shape[0], 2
+    o = packed.packed_attention(q.view(n, H, -1), k.view(n, H, -1), v.view(n, H, -1), cu, causal=True, bias=(table, of))
+    y, h = packed.gated_norm(x, o.reshape(n, -1), post_weight=w[3, 0], pre_weight=w[3, 1], scale=w[3, 2], kind="rms")
+    return [y.detach(), h.detach(), *torch.autograd.grad([y, h], [x, w, table], [y.detach() * 0.5, h.detach()])]
+
+
+@pytest.mark.gpu
+def test_streams_threads_and_graphs():
+    import threading
+    lens = [70, 1, 200]
+    cu = starts(lens).cuda()
+    g = torch.Generator().manual_seed(1)
+    of = packed.relative_buckets(16, 60, False, "cuda")
+    x, w, t = (torch.randn(*s, generator=g).cuda().mul_(f).requires_grad_(True) for s, f in (((sum(lens), 64), 1.0), ((4, 64, 64), 0.2), ((16, 2), 1.0)))
+    want = _step(x, w, cu, t, of)
+    # two streams at once, and a thread each
+    got = {}
+
+    def work(i):
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(st):
+            got[i] = [_step(x, w, cu, t, of) for _ in range(3)][-1]
+        st.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [th.start() for th in threads]
+    [th.join() for th in threads]
+    assert len(got) == 3
+    for r in got.values():
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+    # forward and backward in a graph, replayed on other values between eager work
+    static = [a.detach().clone().requires_grad_(True) for a in (x, w, t)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(static[0], static[1], cu, static[2], of)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, _step(static[0], static[1], cu, static[2], of)))
+    for i in range(4):
+        new = [a.detach() * (1 + 0.1 * i) for a in (x, w, t)]
+        with torch.no_grad():
+            for s, a in zip(static, new):
+                s.copy_(a)
+        eager = _step(*[a.clone().requires_grad_(True) for a in new[:2]], cu, new[2].clone().requires_grad_(True), of)
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, eager)), "replay %d" % i
+
+
+@pytest.mark.gpu
+def test_new_tokens_in_a_graph_as_the_caches_grow():
+    """lengths are read on the device: one captured call serves every step"""
+    cap, B, H, Hk, d = 700, 3, 8, 2, 64
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(B * cap, Hk, d, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q = torch.randn(B, H, d, generator=g).to(torch.bfloat16).cuda()
+    cq, ck = starts([1] * B).cuda(), starts([cap] * B).cuda()
+    kl = torch.tensor([1, 1, 1], dtype=torch.int32, device="cuda")
+    call = lambda: packed.packed_attention(q, k, v, cq, ck, k_len=kl, causal=True, max_q=1, max_k=cap)
+    with torch.no_grad():
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        for lens in ([1, 5, 0], [64, 65, 63], [700, 1, 300], [699, 128, 129]):
+            kl.copy_(torch.tensor(lens, dtype=torch.int32))
+            graph.replay()
+            want = attn_ref(q, k, v, [1] * B, [0, 1, 2], lens, ck.tolist(), True, d ** -0.5)
+            within(out, want["o"], str(lens))
+
+
+def _norm64(t, w, layer):
+    t = t - t.mean(1, keepdim=True) if layer else t
+    return t * (t.pow(2).mean(1, keepdim=True) + 1e-6) ** -0.5 * w
+
+
+@pytest.mark.gpu
+def test_a_block_of_them_together():
+    """norm - projections - attention with a bias - projection - gated norm, twice over, against the same in 64 bits"""
+    lens, W, H, Hk, d = [50, 3, 81], 96, 6, 2, 16
+    n = sum(lens)
+    g = torch.Generator().manual_seed(12)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=F8)
+    par = dict(x=r(n, W), f=r(n, W), wq=r(2, W, H * d) * W ** -0.5, wk=r(2, W, Hk * d) * W ** -0.5, wv=r(2, W, Hk * d) * W ** -0.5,
+               wo=r(2, H * d, W) * (H * d) ** -0.5, table=r(8, H), post=1 + 0.1 * r(3, W), pre=1 + 0.1 * r(3, W), gate=torch.sigmoid(r(len(lens), W)),
+               scale=0.5 + 0.1 * r(W))
+    cu, of = starts(lens), packed.relative_buckets(8, 24, False)
+    seq = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+
+    def model(p, norm, attend, of, cu):
+        y, h = norm(p["x"], p["f"], p, 0)
+        for i in range(2):
+            q, k, v = (h @ p[m][i] for m in ("wq", "wk", "wv"))
+            o = attend(q.view(n, H, d), k.view(n, Hk, d), v.view(n, Hk, d), p["table"], of, cu)
+            y, h = norm(y, o.reshape(n, H * d) @ p["wo"][i], p, i + 1)
+        return (y * h).sum() / n + h.pow(2).sum() / n
+
+    def norm64(x, f, p, i):
+        y = x + p["scale"] * p["gate"][seq] * _norm64(f, p["post"][i], True)
+        return y, _norm64(y, p["pre"][i], True)
+
+    def attend64(q, k, v, table, of, cu):
+        out = []
+        m = of.numel() // 2
+        for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+            rel = torch.arange(b - a)[None] - torch.arange(b - a)[:, None]
+            s = torch.einsum("ihd,jhd->hij", q[a:b], k[a:b].repeat_interleave(H // Hk, 1)) * d ** -0.5 + table[of.long()[rel.clamp(-m, m) + m]].permute(2, 0, 1)
+            out.append(torch.einsum("hij,jhd->ihd", torch.softmax(s.masked_fill(rel > 0, -math.inf), 2), v[a:b].repeat_interleave(H // Hk, 1)))
+        return torch.cat(out)
+
+    def norm_hip(x, f, p, i):
+        return packed.gated_norm(x, f, post_weight=p["post"][i], pre_weight=p["pre"][i], gate=p["gate"], scale=p["scale"], kind="layer", cu_seqlens=cu_d)
+    ref = {m: t.clone().requires_grad_(True) for m, t in par.items()}
+    loss = model(ref, norm64, attend64, of, cu)
+    want = torch.autograd.grad(loss, list(ref.values()))
+    cu_d = cu.cuda()
+    hip = {m: t.float().cuda().requires_grad_(True) for m, t in par.items()}
+    got_loss = model(hip, norm_hip, lambda q, k, v, table, of, cu: packed.packed_attention(q, k, v, cu, causal=True, bias=(table, of)), of.cuda(), cu_d)
+    got = torch.autograd.grad(got_loss, list(hip.values()))
+    # f32 throughout: every stage (five norms' worth of rows, six products of 96 terms, two softmaxes, and their backwards) adds at
+    # most about 16 units of 2^-24, in random directions over some 30 stages, and a norm's 1 / deviation amplifies by up to 4
+    tol = 4 * 16 * 30 ** 0.5 * 2.0 ** -24
+    assert abs(float(got_loss) - float(loss)) < tol * abs(float(loss))
+    for m, a, b in zip(par, got, want):
+        assert float((a.cpu().to(F8) - b).norm()) < tol * float(b.norm()), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["attention", "norm"])
+def test_gradients_against_differences(what):
+    lens = [40, 75]
+    cu = starts(lens).cuda()
+    g = torch.Generator().manual_seed(21)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()
+    n = sum(lens)
+    if what == "attention":
+        of = packed.relative_buckets(8, 30, True, "cuda")
+        leaves = [r(n, 4, 32), r(n, 2, 32), r(n, 2, 32), r(8, 4)]
+        f = lambda a: [packed.packed_attention(a[0], a[1], a[2], cu, causal=True, bias=(a[3], of))]
+        weight = [r(n, 4, 32)]
+    else:
+        leaves = [r(n, 72), r(n, 72), 1 + 0.2 * r(72), 1 + 0.2 * r(72), torch.sigmoid(r(2, 72)), r(72), 0.3 * r(72)]
+        f = lambda a: list(packed.gated_norm(a[0], a[1], post_weight=a[2], pre_weight=a[3], gate=a[4], scale=a[5], post_bias=a[6], kind="layer", cu_seqlens=cu))
+        weight = [r(n, 72), r(n, 72)]
+    loss = lambda a: float(sum((o.double() * w.double()).sum() for o, w in zip(f(a), weight)))
+    at = [t.clone().requires_grad_(True) for t in leaves]
+    outs = f(at)
+    grads = torch.autograd.grad(outs, at, weight)
+    noise = 2.0 ** -20 * float(sum((o.double() * w.double()).pow(2).sum() for o, w in zip(outs, weight))) ** 0.5      # of a sum of values off by 2^-20
+    for i, t in enumerate(leaves):
+        d = r(*t.shape)
+        slope = lambda e: (loss(leaves[:i] + [t + e * d] + leaves[i + 1:]) - loss(leaves[:i] + [t - e * d] + leaves[i + 1:])) / (2 * e)
+        e = 2.0 ** -7
+        near, far = slope(e), slope(2 * e)
+        # the steps' error falls by four from 2 e to e: what is left at e is a third of what they differ by
+        assert abs(float((grads[i].double() * d.double()).sum()) - near) <= abs(near - far) / 3 * 1.5 + 4 * noise / e, (what, i)
