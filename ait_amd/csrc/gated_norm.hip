@@ -39,8 +39,8 @@ struct NormArgs {
   void* dx;
   void* df;
   void* dgate;
-  float* parts;        // [units][n_parts][width] of the parameters, then [units + n_seq][width] of the sequences' gates
-  int units, per, n_parts;      // a unit: a group of waves and its `per` consecutive rows
+  float* parts;        // [blocks][n_parts][width] of the parameters, then [units + n_seq][width] of the sequences' gates
+  int units, per, blocks, n_parts;      // a unit: a group of waves and its `per` consecutive rows; blocks: workgroups
   int zero_rest;
 };
 // which parts there are: w_post, w_pre, then scale, b_post, b_pre where given
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
 #pragma unroll
     for (int e = 0; e < 8; e++) cp[v][e] = cq[v][e] = cs[v][e] = bp[v][e] = bq[v][e] = cg[v][e] = 0.f;
   const int unit = blockIdx.x * R + group, first = unit * a.per, last = min(first + a.per, a.rows);
-  float* gate_parts = a.parts + (size_t)a.units * a.n_parts * W;
+  float* gate_parts = a.parts + (size_t)a.blocks * a.n_parts * W;
   int seq = 0;
   if (a.gate_kind == 2 && first < a.rows) seq = seq_of(a.cu, a.n_seq, a.rows, first);
   for (int i = 0; i < a.per; i++) {          // (every group makes every turn: the sums meet at barriers)
@@ -369,19 +369,40 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
       if (write) store8<VEC>(reinterpret_cast<F*>(a.df) + rc * a.df_row, (gl + v * G * 64) * 8, W, d[v]);
     }
   }
-  if (unit >= a.units) return;
-  float* parts = a.parts + (size_t)unit * a.n_parts * W;
+  // the parameters' sums: those of a workgroup's groups added in order, one part of a workgroup to memory
+  __shared__ float join[R > 1 ? R * G * 512 : 1];
+  float* out = a.parts + (size_t)blockIdx.x * a.n_parts * W;
+  auto part = [&](float (*c)[8]) {
+    if constexpr (R > 1) {
+      __syncthreads();
+      float* mine = join + group * G * 512;
 #pragma unroll
-  for (int v = 0; v < V; v++) {
-    const int at = (gl + v * G * 64) * 8;
-    float* p = parts;
-    store8<VEC>(p, at, W, cp[v]);
-    store8<VEC>(p += W, at, W, cq[v]);
-    if (a.scale) store8<VEC>(p += W, at, W, cs[v]);
-    if (SUMS_B && a.b_post) store8<VEC>(p += W, at, W, bp[v]);
-    if (SUMS_B && a.b_pre) store8<VEC>(p += W, at, W, bq[v]);
-    if (a.gate_kind == 2 && first < a.rows && seq < a.n_seq) store8<VEC>(gate_parts + (size_t)(unit + seq) * W, at, W, cg[v]);
-  }
+      for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) mine[(gl + v * G * 64) * 8 + e] = c[v][e];
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int g = 1; g < R; g++) c[v][e] += join[g * G * 512 + (gl + v * G * 64) * 8 + e];
+      }
+    }
+    if (group == 0)
+#pragma unroll
+      for (int v = 0; v < V; v++) store8<VEC>(out, (gl + v * G * 64) * 8, W, c[v]);
+    out += W;
+  };
+  part(cp);
+  part(cq);
+  if (a.scale) part(cs);
+  if (SUMS_B && a.b_post) part(bp);
+  if (SUMS_B && a.b_pre) part(bq);
+  if (a.gate_kind == 2 && first < a.rows && seq < a.n_seq)
+#pragma unroll
+    for (int v = 0; v < V; v++) store8<VEC>(gate_parts + (size_t)(unit + seq) * W, (gl + v * G * 64) * 8, W, cg[v]);
 }
 
 // the units' parts of the parameters' gradients added in order: 16 values and 64 rows of units to a workgroup
@@ -419,10 +440,10 @@ __global__ __launch_bounds__(1024) void gated_norm_sum_kernel(const SumArgs a) {
 // a sequence's gate: the parts of the units that have rows of it
 template <typename F>
 __global__ __launch_bounds__(256) void gated_norm_gate_kernel(const NormArgs a) {
-  const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+  const int nx = (a.width + 255) / 256, b = blockIdx.x / nx, c = (blockIdx.x - b * nx) * 256 + threadIdx.x;
   if (c >= a.width) return;
   const int start = clamp_row(a.cu, b, a.rows), end = clamp_row(a.cu, b + 1, a.rows);
-  const float* parts = a.parts + (size_t)a.units * a.n_parts * a.width;
+  const float* parts = a.parts + (size_t)a.blocks * a.n_parts * a.width;
   float u = 0.f;
   if (end > start) {
     int i = start / a.per;
@@ -446,6 +467,7 @@ template <typename X, typename F, bool BWD, bool VEC, int G, int V>
 int launch_gv(const NormArgs& a, hipStream_t st) {
   const int rows = BWD ? a.units : a.rows;
   const dim3 grid((unsigned)((rows + Block<G>::kRows - 1) / Block<G>::kRows)), block(Block<G>::kThreads);
+  if ((unsigned long long)grid.x * block.x >= (1ull << 32)) return AIT_EUNSUPPORTED;      // a launch's work items are counted in 32 bits
   if constexpr (BWD) {
     if (a.b_post || a.b_pre) hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V, VEC, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((gated_norm_bwd_kernel<X, F, G, V, VEC, false>), grid, block, 0, st, a);
@@ -455,7 +477,7 @@ int launch_gv(const NormArgs& a, hipStream_t st) {
 }
 template <typename X, typename F, bool BWD>
 int launch_xf(const NormArgs& a, bool vec, hipStream_t st) {
-  // as many waves as the row fills: one block of eight values a lane up to 4096, two beyond
+  // as many waves as the row fills: one block of eight values a lane up to 6144, two beyond
   if (!vec) {
     if (a.width <= 512) return launch_gv<X, F, BWD, false, 1, 1>(a, st);
     if (a.width <= 2048) return launch_gv<X, F, BWD, false, 4, 1>(a, st);
@@ -468,8 +490,8 @@ int launch_xf(const NormArgs& a, bool vec, hipStream_t st) {
     case 4: return launch_gv<X, F, BWD, true, 4, 1>(a, st);
     case 5: case 6: return launch_gv<X, F, BWD, true, 6, 1>(a, st);
     case 7: case 8: return launch_gv<X, F, BWD, true, 8, 1>(a, st);
-    case 9: case 10: return launch_gv<X, F, BWD, true, 5, 2>(a, st);
-    case 11: case 12: return launch_gv<X, F, BWD, true, 6, 2>(a, st);
+    case 9: case 10: return launch_gv<X, F, BWD, true, 10, 1>(a, st);
+    case 11: case 12: return launch_gv<X, F, BWD, true, 12, 1>(a, st);
     default: return launch_gv<X, F, BWD, true, 8, 2>(a, st);
   }
 }
@@ -484,7 +506,7 @@ int check(const ait_gated_norm* p) {
   if (!p || p->rows < 0 || p->width <= 0 || p->n_seq < 0 || !(p->eps >= 0.f)) return AIT_EINVAL;
   if ((p->dtype_x != AIT_DTYPE_F32 && p->dtype_x != AIT_DTYPE_BF16) || (p->dtype_f != AIT_DTYPE_F32 && p->dtype_f != AIT_DTYPE_BF16)) return AIT_EINVAL;
   if (p->width > kMaxWidth || (p->dtype_x == AIT_DTYPE_BF16 && p->dtype_f == AIT_DTYPE_F32)) return AIT_EUNSUPPORTED;
-  if ((long long)p->rows + 4096 >= (1ll << 31)) return AIT_EUNSUPPORTED;
+  if ((long long)p->rows + 4096 >= (1ll << 31) || (p->width + 255) / 256 * 256ll * p->n_seq >= (1ll << 32)) return AIT_EUNSUPPORTED;
   if (!p->w_post || !p->w_pre) return AIT_EINVAL;
   if (p->rows > 0 && (!p->x || !p->f)) return AIT_EINVAL;
   if (p->x_row < 0 || p->f_row < 0 || p->gate_row < 0) return AIT_EINVAL;
@@ -508,10 +530,13 @@ bool inputs_aligned(const ait_gated_norm& p) {
 }
 // units of the backward: about two workgroups' groups a CU, each with a run of rows
 void units_of(const ait_gated_norm& p, int& units, int& per) {
-  const int groups = p.width <= 512 ? 2048 : p.width <= 1024 ? 1024 : 512;
+  const int groups = p.width <= 512 ? 2048 : p.width <= 1024 ? 1024 : p.width <= 4096 ? 512 : 256;
   per = p.rows > 0 ? (p.rows + groups - 1) / groups : 1;
   units = (p.rows + per - 1) / per;
 }
+// rows that a workgroup of the backward has side by side (Block<G>::kRows of the launch)
+int groups_of(const ait_gated_norm& p, bool vec) { return p.width <= 512 ? 4 : vec && p.width <= 1024 ? 2 : 1; }
+int blocks_of(const ait_gated_norm& p, int units, bool vec) { return (units + groups_of(p, vec) - 1) / groups_of(p, vec); }
 int parts_of(const ait_gated_norm& p) { return 2 + (p.scale ? 1 : 0) + (p.b_post ? 1 : 0) + (p.b_pre ? 1 : 0); }
 }  // namespace
 
@@ -529,7 +554,7 @@ AIT_API size_t ait_gated_norm_bwd_workspace_bytes(const ait_gated_norm* p) {
   if (check(p) != AIT_OK) return 0;
   int units, per;
   units_of(*p, units, per);
-  return ((size_t)units * parts_of(*p) + (p->cu_seqlens ? (size_t)units + p->n_seq : 0)) * p->width * sizeof(float);
+  return ((size_t)blocks_of(*p, units, false) * parts_of(*p) + (p->cu_seqlens ? (size_t)units + p->n_seq : 0)) * p->width * sizeof(float);
 }
 
 AIT_API int ait_gated_norm_bwd(const ait_gated_norm* p, const float* stats, const void* dy, long long dy_row, const void* dh, long long dh_row,
@@ -555,8 +580,9 @@ AIT_API int ait_gated_norm_bwd(const ait_gated_norm* p, const float* stats, cons
   const int xs = p->dtype_x == AIT_DTYPE_F32 ? 4 : 2, fs = p->dtype_f == AIT_DTYPE_F32 ? 4 : 2;
   const bool vec = inputs_aligned(*p) && aligned(dy, dy_row, xs) && aligned(dh, dh_row, fs) && aligned(dx, dx_row, xs) && aligned(df, df_row, fs) &&
                    aligned(d_gate, dg_row, fs);
+  a.blocks = blocks_of(*p, a.units, vec);
   if (p->rows > 0) AIT_TRY_RC(launch<true>(*p, a, vec, st));
-  SumArgs s{a.parts, {d_w_post, d_w_pre, nullptr, nullptr, nullptr}, a.units, a.n_parts, p->width};
+  SumArgs s{a.parts, {d_w_post, d_w_pre, nullptr, nullptr, nullptr}, a.blocks, a.n_parts, p->width};
   int n = 2;
   if (p->scale) s.out[n++] = d_scale;
   if (p->b_post) s.out[n++] = d_b_post;
@@ -564,7 +590,7 @@ AIT_API int ait_gated_norm_bwd(const ait_gated_norm* p, const float* stats, cons
   hipLaunchKernelGGL(gated_norm_sum_kernel, dim3((unsigned)((a.n_parts * p->width + 15) / 16)), dim3(1024), 0, st, s);
   AIT_CHECK_LAUNCH();
   if (a.gate_kind == 2 && p->n_seq > 0) {
-    const dim3 grid((unsigned)((p->width + 255) / 256), (unsigned)p->n_seq);
+    const dim3 grid((unsigned)((p->width + 255) / 256) * (unsigned)p->n_seq);
     if (p->dtype_f == AIT_DTYPE_F32) hipLaunchKernelGGL(gated_norm_gate_kernel<float>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(gated_norm_gate_kernel<__bf16>, grid, dim3(256), 0, st, a);
     AIT_CHECK_LAUNCH();

@@ -275,6 +275,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
 int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   const int bytes = 2 * a.stages * Tile<T, D>::kBytes + bias_bytes;
+  if (!launchable((long long)a.numbers * (a.H / a.pack), NW * 64) || (SPLIT && !launchable(((long long)a.s.total_q * a.H + 3) / 4, 256)))
+    return AIT_EUNSUPPORTED;
   if (bytes > 65536 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           bytes) != hipSuccess)

@@ -558,6 +558,11 @@ int launch(BwdArgs a, hipStream_t st) {
   const int qb = 2 * a.stages * Tile<T, D>::kBytes + bias + (BIAS ? NWQ * (kSums<T, D> + a.bias.n_buckets) * 4 : 0);
   const int kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
   constexpr bool kSplit = D == 128 && sizeof(T) == 2;
+  const long long knumbers = block_numbers(a.s.total_k, 1, NW * 16, a.s.n_seq, a.s.rest);
+  if (!launchable((long long)a.qnumbers * a.H, NWQ * 64) || !launchable(knumbers * a.Hk * (kSplit ? 2 : 1), NT) ||
+      (a.splits > 1 && !launchable(((long long)a.s.total_q * a.H + 3) / 4, 256)))
+    return AIT_EUNSUPPORTED;
+  a.knumbers = (int)knumbers;
   AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS, NWQ>, qb));
   AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS, kSplit>, kb));
   if (a.s.total_q > 0) {
@@ -569,7 +574,6 @@ int launch(BwdArgs a, hipStream_t st) {
     }
   }
   if (a.s.total_k > 0) {
-    a.knumbers = (int)block_numbers(a.s.total_k, 1, NW * 16, a.s.n_seq, a.s.rest);
     hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS, kSplit>), dim3((unsigned)(a.knumbers * a.Hk * (kSplit ? 2 : 1))), dim3(NT), kb, st, a);
     AIT_CHECK_LAUNCH();
   }

@@ -343,6 +343,8 @@ __device__ __forceinline__ void fill_bias(const Bias& b, int H, int head0, int h
 }
 
 int check(const ait_packed_attn* p);
+// a launch's work items are counted in 32 bits
+static inline bool launchable(long long workgroups, int threads) { return workgroups * threads < (1LL << 32) && workgroups < (1LL << 31); }
 int check_strides(const ait_packed_attn* p, const void* base, long long row, long long head, long long rows);
 
 }  // namespace ait_packed

@@ -155,7 +155,7 @@ def test_queries_and_keys_of_different_lengths(dtype, ql, kl, H, Hk, d, causal):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lens,H,Hk,d,causal,n,m,two", [
     (RAGGED, 2, 2, 64, False, 8, 20, True), (LONG, 4, 1, 64, True, 32, 128, False), (LONG, 2, 1, 128, False, 32, 100, True),
-    ([500], 1, 1, 32, True, 16, 9, False), ([40, 64, 3], 8, 8, 64, False, 16, 2000, True)])
+    ([500], 1, 1, 32, True, 16, 9, False), ([40, 64, 3], 8, 8, 64, False, 16, 2000, True), ([300, 33], 2, 1, 128, False, 512, 2048, True)])
 def test_relative_position_bias(dtype, lens, H, Hk, d, causal, n, m, two):
     q, k, v, do = make(lens, lens, H, Hk, d, dtype, 11 + m)
     bias = packed.RelativePositionBias(H, n, m, two).to("cuda", dtype if H > 1 else torch.float32)
@@ -284,7 +284,7 @@ def test_c_entries_refuse_bad_arguments():
         for kw in (dict(heads=0), dict(kv_heads=3), dict(n_seq=-1), dict(total_q=-1), dict(d=0), dict(dtype=2), dict(cu_q=None), dict(cu_k=None),
                    dict(max_q=-1), dict(scale=float("nan")), dict(bias_table=4096), dict(bias_table=4096, bucket_of=4096, n_buckets=0)):
             assert f(**kw) == EINVAL, kw
-        for kw in (dict(d=136), dict(d=12), dict(bias_table=4096, bucket_of=4096, n_buckets=513), dict(total_q=2 ** 30),
+        for kw in (dict(d=136), dict(d=12), dict(n_seq=1 << 27), dict(bias_table=4096, bucket_of=4096, n_buckets=513), dict(total_q=2 ** 30),
                    dict(bias_table=4096, bucket_of=4096, n_buckets=4, max_distance=2049)):
             assert f(**kw) == EUNSUPPORTED, kw
         assert f(n_seq=0) == 0
@@ -383,7 +383,8 @@ def norm_ref(x, f, post, pre, post_b, pre_b, gate, scale, layer, eps, cu, dy, dh
     (1, 8, "rms", "row", True, False), (37, 512, "layer", "none", True, False), (300, 512, "rms", "sequence", True, False), (5, 17, "layer", "row", False, False),
     (64, 513, "layer", "sequence", True, False), (130, 1024, "rms", "row", True, True), (9, 2048, "layer", "sequence", False, False),
     (21, 4096, "rms", "sequence", True, True), (17, 8192, "layer", "row", True, False), (600, 100, "layer", "sequence", True, False), (3, 5120, "rms", "none", False, False),
-    (2100, 40, "layer", "sequence", True, True), (5, 1, "rms", "row", True, False)])
+    (2100, 40, "layer", "sequence", True, True), (5, 1, "rms", "row", True, False), (0, 64, "layer", "sequence", True, False), (30, 1536, "rms", "row", True, False),
+    (11, 2600, "layer", "none", True, True), (9, 6144, "layer", "row", True, False), (40, 5120, "layer", "sequence", True, False)])
 def test_gated_norm(types, rows, width, kind, gate, scale, odd):
     xt, ft = (getattr(torch, t) for t in types)
     g = torch.Generator().manual_seed(rows + width)
@@ -453,9 +454,9 @@ def test_gated_norm_refuses_what_it_does_not_take():
         for kw in (dict(rows=-1), dict(width=0), dict(dtype_x=2), dict(dtype_f=-1), dict(w_post=None), dict(w_pre=None), dict(x=None), dict(f=None),
                    dict(eps=-1.0), dict(cu_seqlens=4096), dict(x_row=-1), dict(n_seq=-1)):
             assert f(**kw) == -1, kw
-        for kw in (dict(width=8193), dict(dtype_x=1, dtype_f=0)):
+        for kw in (dict(width=8193), dict(dtype_x=1, dtype_f=0), dict(rows=2 ** 31 - 4096)):
             assert f(**kw) == -4, kw
-    assert fwd(y=None) == -1 and fwd(yr=31) == -1
+    assert fwd(y=None) == -1 and fwd(yr=31) == -1 and fwd(rows=1 << 27) == -4
     assert bwd(ws=None) == -2 and bwd(n=64) == -2 and bwd(scale=4096) == -1 and bwd(gate=4096, gate_row=32) == -1
 
 
