@@ -45,12 +45,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int units = a.H / a.pack, unit = blockIdx.x % units, group = a.H / a.Hk;
-  // key heads run fastest (workgroups 8 apart share an L2: they read the same key head where there are 8, 4, 2 or 1 of them),
-  // a sequence's last rows first (with a causal mask they have the most to do)
+  // key heads run fastest (workgroups 8 apart share an L2: they read the same key head where there are 8, 4, 2 or 1 of them)
   const int kvh = unit % a.Hk, head0 = kvh * group + (unit / a.Hk) * a.pack;
-  int seq, block, qstart, qlen, kstart, klen;
-  if (!find_block(a.s.cu_q, a.s.n_seq, a.s.rest, a.s.total_q, a.pack, BM, a.numbers - 1 - (int)(blockIdx.x / units), seq, block, qstart, qlen))
-    return;
+  Place place;
+  if (!find_place<false>(a.s, a.pack, BM, (int)(blockIdx.x / units), a.numbers, a.causal, place)) return;
+  const int seq = place.seq, block = place.block, qstart = place.qstart, qlen = place.qlen;
   if (seq == a.s.n_seq) {          // rows of no sequence
     if constexpr (!SPLIT) {
       const int r = block * BM + wave * 32 + (lane & 31), n = r / a.pack;
@@ -64,8 +63,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
     }
     return;
   }
-  keys_of(a.s, seq, kstart, klen);
-  const int rows = qlen * a.pack, off = klen - qlen;
+  const int kstart = place.kstart, klen = place.klen, rows = qlen * a.pack, off = klen - qlen;
   const int row0 = block * BM + wave * 32, row = row0 + (lane & 31);
   const int rowc = row < rows ? row : rows - 1, pos = rowc / a.pack, head = head0 + rowc - pos * a.pack;
   const int kmax = a.causal ? min(klen, pos + off + 1) : klen;                           // this lane's query sees keys below it
@@ -379,7 +377,7 @@ AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long lo
   if (need && (!workspace_ptr || workspace_bytes < need)) return AIT_EWORKSPACE;
   if ((unsigned long long)workspace_ptr % 16) return AIT_EINVAL;
   FwdArgs a{q, k, v, o, lse, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
-            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
+            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.nw > 1 && sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
             (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, p->scale, nullptr, nullptr};

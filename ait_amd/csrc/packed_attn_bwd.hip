@@ -51,10 +51,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int unit = blockIdx.x % a.H, group = a.H / a.Hk, kvh = unit % a.Hk, head = kvh * group + unit / a.Hk;
-  const int number = a.qnumbers - 1 - (int)(blockIdx.x / a.H), nb = a.bias.n_buckets, md = a.bias.max_distance;
+  const int number = (int)(blockIdx.x / a.H), nb = a.bias.n_buckets, md = a.bias.max_distance;
   float* part = BIAS && a.part_table ? a.part_table + (((size_t)blockIdx.y * a.qnumbers + number) * a.H + head) * nb : nullptr;
-  int seq, block, qstart, qlen, kstart, klen;
-  const bool has = find_block(a.s.cu_q, a.s.n_seq, a.s.rest, a.s.total_q, 1, BM, number, seq, block, qstart, qlen);
+  Place place;
+  const bool has = find_place<false>(a.s, 1, BM, number, a.qnumbers, a.causal, place);
+  const int seq = place.seq, block = place.block, qstart = place.qstart, qlen = place.qlen;
   if (!has || seq == a.s.n_seq) {
     if constexpr (BIAS)
       if (part)
@@ -69,8 +70,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
       }
     return;
   }
-  keys_of(a.s, seq, kstart, klen);
-  const int off = klen - qlen, row0 = block * BM + wave * 32, row = row0 + (lane & 31), pos = min(row, qlen - 1);
+  const int kstart = place.kstart, klen = place.klen, off = klen - qlen, row0 = block * BM + wave * 32, row = row0 + (lane & 31), pos = min(row, qlen - 1);
   const int kmax = a.causal ? min(klen, pos + off + 1) : klen;
   const int wfirst = min(row0, qlen - 1), wlast = min(row0 + 31, qlen - 1);
   const int wsure = a.causal ? min(klen, wfirst + off + 1) : klen, wend = row0 < qlen ? (a.causal ? min(klen, wlast + off + 1) : klen) : 0;
@@ -311,19 +311,10 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes, BN = NW / XH * 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int kvh = index % a.Hk, group = a.H / a.Hk, number = index / a.Hk, md = a.bias.max_distance;
-  int seq, block, kstart, kroom, klen;
-  // key blocks are numbered by the rows the sequences OCCUPY: keys behind k_len get zeros
-  if (!find_block(a.s.cu_k, a.s.n_seq, a.s.rest, a.s.total_k, 1, BN, number, seq, block, kstart, kroom)) return;
-  const int kc = wave % (NW / XH), xh = wave / (NW / XH), key0 = block * BN + kc * 32, key = key0 + (lane & 31);
-  int qstart = 0, qlen = 0;
-  klen = 0;
-  if (seq < a.s.n_seq) {
-    int ks;
-    keys_of(a.s, seq, ks, klen);
-    qstart = clamped(a.s.cu_q, seq, a.s.total_q);
-    qlen = max(0, clamped(a.s.cu_q, seq + 1, a.s.total_q) - qstart);
-  }
-  const int off = klen - qlen;
+  Place place;
+  if (!find_place<true>(a.s, 1, BN, number, 0, a.causal, place)) return;
+  const int block = place.block, qstart = place.qstart, qlen = place.qlen, kstart = place.kstart, klen = place.klen, kroom = place.kroom;
+  const int kc = wave % (NW / XH), xh = wave / (NW / XH), key0 = block * BN + kc * 32, key = key0 + (lane & 31), off = klen - qlen;
   // query rows that see a key j: positions >= j - off with a causal mask
   const int gfirst = a.causal ? max(0, block * BN - off) : 0;
   const int wsure = a.causal ? max(0, min(key0 + 31, klen - 1) - off) : 0;          // from here on every key of the wave is seen
@@ -626,7 +617,7 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
   const Shape sh = shape_of(*p);
   BwdArgs a{q, k, v, o, d_o, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, lse, dq, dk, dv, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head,
             dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
-            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0},
+            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, p->scale,
             static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, d_table};

@@ -293,6 +293,51 @@ __device__ __forceinline__ bool find_block(const int* cu, int n_seq, int rest, i
   block = number - (int)((long long)start * mul / bm) - lo;
   return block >= 0 && (long long)block * bm < (long long)len * mul;
 }
+// inclusive sum over the lanes
+__device__ __forceinline__ int lane_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: inside 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);      // the last lane of rows 0 and 2 to rows 1 and 3,
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);      // of the first half to the second
+  return v;
+}
+// The same blocks in another order: those with the most turns first, whatever their sequence, so that a launch does not end on
+// the long ones (7 prompts of 33 to 4096 tokens: see packed_attn.hip).  At most 64 sequences, `rest` among them.
+// A block of rows j (of ROWS rows) of a sequence takes turns(j) = ceil(min(all, (j + 1) rows_per + off) / KB) turns if it
+// ascends, ceil((all - max(0, j rows_per - off)) / KB) if not -- the key tiles of a query block, the query tiles of a key block;
+// `flat`: every block takes ceil(all / KB).  The blocks with more than L turns are counted in closed form and L is found by
+// bisection; among those with L + 1 turns the order is by sequence.
+struct Turns { int blocks, all, off, rows_per; bool flat, ascends; };
+__device__ __forceinline__ int blocks_over(const Turns& s, int L) {      // blocks with more than L >= 0 turns
+  const int need = L * KB;
+  if (s.all <= need) return 0;
+  if (s.flat) return s.blocks;
+  if (s.ascends) {      // (j + 1) rows_per + off > need
+    const int first = need - s.off;
+    return s.blocks - min(s.blocks, first > 0 ? first / s.rows_per : 0);
+  }
+  const int room = s.all - need - 1 + s.off;      // all - max(0, j rows_per - off) > need: j rows_per <= room
+  return room < 0 ? 0 : min(s.blocks, room / s.rows_per + 1);
+}
+__device__ __forceinline__ bool heaviest_first(const Turns& s, int number, int most, int& seq, int& block) {
+  if (__builtin_amdgcn_readlane(lane_scan(s.blocks), 63) <= number) return false;
+  int lo = -1, hi = most;      // over(lo) > number >= over(hi); over(-1): all blocks
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__builtin_amdgcn_readlane(lane_scan(blocks_over(s, mid)), 63) > number) lo = mid;
+    else hi = mid;
+  }
+  const int more = blocks_over(s, lo + 1), here = (lo < 0 ? s.blocks : blocks_over(s, lo)) - more;      // this lane's with lo + 1 turns
+  const int skip = number - __builtin_amdgcn_readlane(lane_scan(more), 63), upto = lane_scan(here);
+  seq = __builtin_ctzll(__ballot(upto > skip));
+  const int k = skip - __builtin_amdgcn_readlane(upto - here, seq);
+  // the k-th of them: in an ascending sequence the blocks with more turns are the last ones, else the first
+  const int m = __builtin_amdgcn_readlane(more, seq), n = __builtin_amdgcn_readlane(here, seq), b = __builtin_amdgcn_readlane(s.blocks, seq);
+  block = __builtin_amdgcn_readlane((int)(s.ascends && !s.flat), seq) ? b - m - n + k : m + k;
+  return true;
+}
 static inline long long block_numbers(long long total, int mul, int bm, int n_seq, int rest) {
   return total * mul / bm + n_seq + rest;
 }
@@ -302,6 +347,7 @@ struct Seqs {
   const int* cu_k;
   const int* k_len;        // may be null: the keys of a sequence end where the next one's begin
   int n_seq, total_q, total_k, rest;
+  int ordered;             // blocks in the order of heaviest_first
 };
 __device__ __forceinline__ void keys_of(const Seqs& s, int seq, int& start, int& len) {
   start = clamped(s.cu_k, seq, s.total_k);
@@ -311,6 +357,49 @@ __device__ __forceinline__ void keys_of(const Seqs& s, int seq, int& start, int&
     const int l = s.k_len[seq];
     len = l < 0 ? 0 : l < len ? l : len;
   }
+}
+
+// A workgroup's place: block `number` of the query rows (mul rows to a position, bm to a block) or, KEYS, of the key rows (bm to a
+// block, counted over the rows that the sequences occupy: keys behind k_len get zeros), and its sequence's queries and keys.
+struct Place { int seq, block, qstart, qlen, kstart, klen, kroom; };
+template <bool KEYS>
+__device__ __forceinline__ bool find_place(const Seqs& s, int mul, int bm, int number, int numbers, bool causal, Place& p) {
+  if (s.ordered) {
+    const int lane = threadIdx.x & 63, n = s.n_seq + s.rest, b = lane < n ? lane : n - 1;
+    const bool seq = b < s.n_seq;
+    const int qs = clamped(s.cu_q, b, s.total_q), qe = seq ? clamped(s.cu_q, b + 1, s.total_q) : s.total_q;
+    const int ks = clamped(s.cu_k, b, s.total_k), ke = seq ? clamped(s.cu_k, b + 1, s.total_k) : s.total_k;
+    const int len = max(0, qe - qs), room = max(0, ke - ks);
+    int kl = seq ? room : 0;
+    if (s.k_len && seq) kl = max(0, min(kl, s.k_len[b]));
+    const int off = kl - len, rows = KEYS ? room : len * mul, per = KEYS || mul == 1 ? bm : max(1, bm / mul);
+    const Turns t{lane < n && rows > 0 ? (rows - 1) / bm + 1 : 0, KEYS ? (kl > 0 ? len : 0) : kl, off, per, !causal, !KEYS};
+    if (!heaviest_first(t, number, (KEYS ? s.total_q : s.total_k) / KB + 1, p.seq, p.block)) return false;
+    p.qstart = __builtin_amdgcn_readlane(qs, p.seq);
+    p.qlen = __builtin_amdgcn_readlane(len, p.seq);
+    p.kstart = __builtin_amdgcn_readlane(ks, p.seq);
+    p.klen = __builtin_amdgcn_readlane(kl, p.seq);
+    p.kroom = __builtin_amdgcn_readlane(room, p.seq);
+    return true;
+  }
+  if constexpr (KEYS) {
+    if (!find_block(s.cu_k, s.n_seq, s.rest, s.total_k, 1, bm, number, p.seq, p.block, p.kstart, p.kroom)) return false;
+    p.qstart = p.qlen = p.klen = 0;
+    if (p.seq < s.n_seq) {
+      int ks;
+      keys_of(s, p.seq, ks, p.klen);
+      p.qstart = clamped(s.cu_q, p.seq, s.total_q);
+      p.qlen = max(0, clamped(s.cu_q, p.seq + 1, s.total_q) - p.qstart);
+    }
+  } else {      // a sequence's last rows first: with a causal mask they have the most to do
+    if (!find_block(s.cu_q, s.n_seq, s.rest, s.total_q, mul, bm, numbers - 1 - number, p.seq, p.block, p.qstart, p.qlen)) return false;
+    if (p.seq < s.n_seq) keys_of(s, p.seq, p.kstart, p.klen);
+  }
+  return true;
+}
+static inline int order_blocks(const ait_packed_attn& p) {
+  const long long max_k = p.max_k > 0 ? p.max_k : p.total_k;
+  return p.n_seq < 64 && max_k > 4 * KB && p.total_q < (1 << 24) && p.total_k < (1 << 24);
 }
 
 // ---- the bias: one value per relative position and head, constant beyond max_distance on either side --------------------------
