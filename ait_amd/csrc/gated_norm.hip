@@ -255,25 +255,20 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
     for (int e = 0; e < 8; e++) cp[v][e] = cq[v][e] = cs[v][e] = bp[v][e] = bq[v][e] = cg[v][e] = 0.f;
   const int unit = blockIdx.x * R + group, first = unit * a.per, last = min(first + a.per, a.rows);
   float* gate_parts = a.parts + (size_t)a.blocks * a.n_parts * W;
-  // the parameters of a lane's values, read once where registers allow it (one block of eight a lane)
+  // The parameters of a lane's values, read once for all rows where registers allow it: one block of eight a lane and up to
+  // eight waves (f32 rows of 512: 161 -> 153 us; ten and twelve waves have 168 registers a lane, which spill, and gain nothing)
+  constexpr bool HELD = V == 1 && G <= 8;
   float w1[1][8], w2[1][8], w3[1][8];
-  if constexpr (V == 1) {
+  if constexpr (HELD) {
     load8<VEC>(a.w_post, gl * 8, W, w1[0]);
     load8<VEC>(a.w_pre, gl * 8, W, w2[0]);
 #pragma unroll
     for (int e = 0; e < 8; e++) w3[0][e] = 1.f;
     if (a.scale) load8<VEC>(a.scale, gl * 8, W, w3[0]);
   }
-  auto take = [&](const float* from, const float (&held)[1][8], int at, float* to) {
-    if constexpr (V == 1) {
+  auto held = [&](const float (&w)[1][8], float* to) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) to[e] = held[0][e];
-    } else if (from) {
-      load8<VEC>(from, at, W, to);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) to[e] = 1.f;
-    }
+    for (int e = 0; e < 8; e++) to[e] = w[0][e];
   };
   int seq = 0;
   if (a.gate_kind == 2 && first < a.rows) seq = seq_of(a.cu, a.n_seq, a.rows, first);
@@ -311,7 +306,8 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
     for (int v = 0; v < V; v++) {
       const int at = (gl + v * G * 64) * 8;
       float p[8], q[8], m[8];
-      take(a.w_post, w1, at, p);
+      if constexpr (HELD) held(w1, p);
+      else load8<VEC>(a.w_post, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         f[v][e] = inside<VEC>(at, e, W) ? (f[v][e] - st[0]) * st[1] : 0.f;       // norm(f)
@@ -325,10 +321,17 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] = 1.f;
       if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
-      take(a.scale, w3, at, q);
+      if constexpr (HELD) {
+        held(w3, q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = 1.f;
+        if (a.scale) load8<VEC>(a.scale, at, W, q);
+      }
 #pragma unroll
       for (int e = 0; e < 8; e++) y[v][e] = inside<VEC>(at, e, W) ? (y[v][e] + m[e] * p[e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
-      take(a.w_pre, w2, at, p);
+      if constexpr (HELD) held(w2, p);
+      else load8<VEC>(a.w_pre, at, W, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         cq[v][e] = __builtin_fmaf(d[v][e], y[v][e], cq[v][e]);
@@ -353,8 +356,15 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] = 1.f;
       if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
-      take(a.scale, w3, at, q);
-      take(a.w_post, w1, at, m);
+      if constexpr (HELD) {
+        held(w3, q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = 1.f;
+        if (a.scale) load8<VEC>(a.scale, at, W, q);
+      }
+      if constexpr (HELD) held(w1, m);
+      else load8<VEC>(a.w_post, at, W, m);
 #pragma unroll
       for (int e = 0; e < 8; e++) b[e] = 0.f;
       if (SUMS_B && a.b_post) load8<VEC>(a.b_post, at, W, b);
