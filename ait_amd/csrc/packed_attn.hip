@@ -8,6 +8,13 @@
 // go straight into shared memory while this one is multiplied, one barrier a tile.  The rows of a workgroup are (position,
 // head) pairs of one key head: `pack` heads to a position, so that a single new token still fills the block's columns with the
 // heads that share its keys.
+//
+// What bounds it.  Long sequences: the matrix unit and the exponentials beside it, at the clock the chip holds under them: 7
+// causal prompts of 33 to 4096 tokens, 16 heads on 4 of 128, bf16: 175 GFLOP in 220 us, 800 TFLOP/s (a large bf16 product
+// reaches 1244 here); the loads alone taken out of it 214, the exponentials alone 219, so neither is in the way.  Matrix unit
+// 42 % busy at 1.7 GHz, no bank conflicts.  (Tried: eight waves a workgroup 247 against 227, two 322 against 231, the next
+// tile's scores under this one's exponentials 255 against 227.)  New tokens: memory: 16 caches of 5000 to 8191, 32 heads on 8 of
+// 128: 432 MB in 84.5 us, 5.1 TB/s, and 4.8 us to join the parts.
 #include "packed_attn_impl.h"
 
 namespace {
@@ -30,7 +37,8 @@ struct FwdArgs {
 };
 
 // four values of o; for a backward also what their rounding takes away.  The backward's delta = dO . O is subtracted from
-// scores' gradients of like size, so O's rounding to bf16 would be the largest error of dQ and dK
+// scores' gradients of like size, so O's rounding to bf16 would be the largest error of dQ and dK.  (Measured against 64 bits: dQ
+// off by 0.0025 to 0.0039 of its norm without the rest, 0.0024 with it; bf16 outputs alone are off by 0.0017.)
 template <typename T>
 __device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, int head, int dd, float v0, float v1, float v2, float v3) {
   store4(p, v0, v1, v2, v3);
@@ -39,8 +47,13 @@ __device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, in
       store4(reinterpret_cast<T*>(a.rest) + (at * a.H + head) * a.d + dd, v0 - (float)(T)v0, v1 - (float)(T)v1, v2 - (float)(T)v2, v3 - (float)(T)v3);
 }
 
-template <typename T, int D, int NW, bool BIAS, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(const FwdArgs a) {
+// REST (bf16 forwards that a backward follows): the probabilities enter the second product as two operands, their bf16 value and
+// what that rounding took, so that delta belongs to the probabilities and not to their rounding: the bias's gradient, a sum over
+// all pairs in which P dP and P delta cancel, is off by 0.0013 to 0.0017 instead of 0.0019 to 0.0023, dQ by 0.0024 instead of up
+// to 0.0026.  It costs a half more products of this pass (long documents 165 -> 212 us of 950 in all); an inference call, which
+// nothing is subtracted from, rounds them once.
+template <typename T, int D, int NW, bool BIAS, bool SPLIT, bool REST>
+__global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a) {
   constexpr int NT = NW * 64, BM = NW * 32, NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -194,9 +207,13 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? 2 : 1) void packed_fwd_kernel(con
         if (sizeof(T) == 4 && k0 + 32 * x + 16 * cc >= wend) continue;
         const Frag<T> pf = acc_frag<T>(s[x], cc);
 #pragma unroll
-        for (int b = 0; b < NB; b++) acc[b] = mma(x == 0 ? first.get(vt, cb, x, cc, b) : col_frag<T, D>(vt, cb, x, cc, b), pf, acc[b]);
+        for (int b = 0; b < NB; b++) {
+          const Frag<T> vf = x == 0 ? first.get(vt, cb, x, cc, b) : col_frag<T, D>(vt, cb, x, cc, b);
+          acc[b] = mma(vf, pf, acc[b]);
+          if constexpr (REST) acc[b] = mma(vf, acc_rest<T>(s[x], cc, pf), acc[b]);
+        }
       }
-    read_ahead<T, 4 * NB, 2, 4, true>();
+    read_ahead<T, 4 * NB, 2, 4, true, REST ? 2 : 1>();
     }
     if (a.stages == 1 && t + 1 < t1) {
       loads_done_barrier();
@@ -270,16 +287,16 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
     store_o<T>(a, reinterpret_cast<T*>(a.o) + (long long)at * a.os + (long long)head * a.oh + dd, at, head, dd, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
-template <typename T, int D, int NW, bool BIAS, bool SPLIT>
+template <typename T, int D, int NW, bool BIAS, bool SPLIT, bool REST>
 int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   const int bytes = 2 * a.stages * Tile<T, D>::kBytes + bias_bytes;
   if (!launchable((long long)a.numbers * (a.H / a.pack), NW * 64) || (SPLIT && !launchable(((long long)a.s.total_q * a.H + 3) / 4, 256)))
     return AIT_EUNSUPPORTED;
   if (bytes > 65536 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+      hipFuncSetAttribute(reinterpret_cast<const void*>(packed_fwd_kernel<T, D, NW, BIAS, SPLIT, REST>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           bytes) != hipSuccess)
     return AIT_ELAUNCH;
-  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, BIAS, SPLIT>), dim3((unsigned)(a.numbers * (a.H / a.pack)), (unsigned)a.splits), dim3(NW * 64),
+  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, BIAS, SPLIT, REST>), dim3((unsigned)(a.numbers * (a.H / a.pack)), (unsigned)a.splits), dim3(NW * 64),
                      bytes, st, a);
   AIT_CHECK_LAUNCH();
   if constexpr (SPLIT) {
@@ -288,14 +305,20 @@ int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   }
   return AIT_OK;
 }
+template <typename T, int D, int NW, bool BIAS, bool SPLIT>
+int launch_rest(const FwdArgs& a, int bias_bytes, hipStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (a.rest) return launch<T, D, NW, BIAS, SPLIT, true>(a, bias_bytes, st);
+  return launch<T, D, NW, BIAS, SPLIT, false>(a, bias_bytes, st);
+}
 template <typename T, int D, int NW>
 int launch_nw(const FwdArgs& a, int bias_bytes, hipStream_t st) {
-  if (a.bias.table) return a.splits > 1 ? launch<T, D, NW, true, true>(a, bias_bytes, st) : launch<T, D, NW, true, false>(a, bias_bytes, st);
-  return a.splits > 1 ? launch<T, D, NW, false, true>(a, 0, st) : launch<T, D, NW, false, false>(a, 0, st);
+  if (a.bias.table) return a.splits > 1 ? launch_rest<T, D, NW, true, true>(a, bias_bytes, st) : launch_rest<T, D, NW, true, false>(a, bias_bytes, st);
+  return a.splits > 1 ? launch_rest<T, D, NW, false, true>(a, 0, st) : launch_rest<T, D, NW, false, false>(a, 0, st);
 }
 template <typename T, int D>
 int launch_d(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
-  return nw == 1 ? launch_nw<T, D, 1>(a, bias_bytes, st) : nw == 2 ? launch_nw<T, D, 2>(a, bias_bytes, st) : launch_nw<T, D, 4>(a, bias_bytes, st);
+  return nw == 2 ? launch_nw<T, D, 2>(a, bias_bytes, st) : launch_nw<T, D, 4>(a, bias_bytes, st);
 }
 template <typename T>
 int launch_t(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
@@ -308,18 +331,22 @@ Shape shape_of(const ait_packed_attn& p) {
   Shape r;
   const int group = p.heads / p.kv_heads;
   const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
-  // a few new tokens: the heads of a key head share a workgroup's columns, and its keys are read once
+  // a few new tokens: the heads of a key head share a workgroup's columns, and its keys are read once (16 long caches, 4 heads to
+  // a key head: 86 us, 185 with a workgroup to a head; with a bias, whose heads each want a row in shared memory, 13.3 and 20.9)
   const bool few = max_q * group <= 128;
   r.pack = few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
-  r.nw = max_q * r.pack <= 32 ? 1 : max_q * r.pack <= 64 ? 2 : 4;
-  // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another
+  // up to 64 rows in two waves, in four what is longer (sequences of 1 to 49 in f32: 36.3 us against 43.5 in four; prompts: 322 us
+  // in two, 231 in four); for single tokens two measure as four and better than one (with bias 11.3, 11.7, 13.3 us)
+  r.nw = max_q * r.pack <= 64 ? 2 : 4;
+  // sequences of one tile have no second one to load ahead: half the memory, twice the workgroups beside one another (sequences
+  // of 1 to 49 in f32: 36.3 us, 55.1 with room for two)
   r.stages = max_k <= KB ? 1 : 2;
   // Few rows leave most of the chip idle: the key axis is cut, two tiles at least to a part.  As many parts as fit the chip at
-  // once with two workgroups a CU (a round more costs as much as all of them: 64 queries against 2394 keys in f32 took
-  // 37 us in 19 parts, 608 workgroups); of the single waves of new tokens twice as many, whose time is their loads'
+  // once with two workgroups a CU: a round more costs as much as all of them (64 queries against 2394 keys in f32: 37 us in 19
+  // parts, 608 workgroups, 33.6 in 16; forward and backward 465 us uncut, 172 cut); twice as many gain new tokens nothing (84.2 us against 84.0)
   const long long rows = (long long)p.total_q * r.pack, blocks = rows / (r.nw * 32) > p.n_seq ? rows / (r.nw * 32) : p.n_seq;
   const long long wgs = (blocks > 0 ? blocks : 1) * (p.heads / r.pack), tiles = (max_k + KB - 1) / KB;
-  long long s = r.nw == 1 ? (1024 + wgs - 1) / wgs : 512 / wgs;
+  long long s = 512 / wgs;
   if (s > tiles / 2) s = tiles / 2;
   if (s > kMaxSplits) s = kMaxSplits;
   r.splits = s < 1 ? 1 : (int)s;
@@ -377,7 +404,7 @@ AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long lo
   if (need && (!workspace_ptr || workspace_bytes < need)) return AIT_EWORKSPACE;
   if ((unsigned long long)workspace_ptr % 16) return AIT_EINVAL;
   FwdArgs a{q, k, v, o, lse, p->dtype == AIT_DTYPE_BF16 ? o_rest : nullptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
-            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.nw > 1 && sh.splits == 1 && ait_packed::order_blocks(*p)},
+            {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
             (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, p->scale, nullptr, nullptr};

@@ -44,7 +44,9 @@ __device__ __forceinline__ f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) 
 
 // eight accumulator values (registers 8 cc .. 8 cc + 7) as an operand: reduction index 16 cc + 8 (e / 4) + 4 (lane >> 5) + e % 4
 // of the 32 the block has.  bf16: rounded to nearest even here -- the one rounding of the probabilities (and of dS in the
-// backward), to the type of the tensor they are multiplied with, as the matrix unit asks; sums stay in f32.
+// backward), to the type of the tensor they are multiplied with, as the matrix unit asks; sums stay in f32.  Against 64 bits it
+// leaves o off by 0.0021 and the gradients by 0.0024 of their norm, where the outputs' own rounding to bf16 makes 0.0017; a
+// second operand with what it took (acc_rest) would cost every product that has one of them as much again.
 template <typename T>
 __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int cc) {
   Frag<T> f;
@@ -53,20 +55,29 @@ __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int cc) {
   return f;
 }
 
+// what that rounding took, as a second operand
+template <typename T>
+__device__ __forceinline__ Frag<T> acc_rest(const f32x16& c, int cc, const Frag<T>& f) {
+  Frag<T> r;
+#pragma unroll
+  for (int e = 0; e < 8; e++) r[e] = (T)(c[8 * cc + e] - (float)f[e]);
+  return r;
+}
+
 // The order of a chain of N products whose left operands come from shared memory by R reads each: AHEAD operands are read before
 // the first product, then one more behind every product.  Left alone, the compiler reads an operand, waits for it and multiplies:
 // a trip to shared memory (over 100 cycles) in front of every 32-cycle product.  (f32: an operand feeds 8 products of 64 cycles.)
-// READ: the first AHEAD operands are there already.
-template <typename T, int N, int R, int AHEAD, bool READ = false>
+// READ: the first AHEAD operands are there already.  M: products that share a left operand.
+template <typename T, int N, int R, int AHEAD, bool READ = false, int M = 1>
 __device__ __forceinline__ void read_ahead() {
   if constexpr (sizeof(T) == 2) {
     if constexpr (!READ) __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
 #pragma unroll
     for (int i = 0; i < N - AHEAD; i++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * M, 0);
   }
 }
 
@@ -304,7 +315,7 @@ __device__ __forceinline__ int lane_scan(int v) {
   return v;
 }
 // The same blocks in another order: those with the most turns first, whatever their sequence, so that a launch does not end on
-// the long ones (7 prompts of 33 to 4096 tokens: see packed_attn.hip).  At most 64 sequences, `rest` among them.
+// the long ones (7 prompts of 33 to 4096 tokens: 217 us against 227, sequences of 17 to 1024 with a bias 61 against 73 in the pass over query rows).  At most 64 sequences, `rest` among them.
 // A block of rows j (of ROWS rows) of a sequence takes turns(j) = ceil(min(all, (j + 1) rows_per + off) / KB) turns if it
 // ascends, ceil((all - max(0, j rows_per - off)) / KB) if not -- the key tiles of a query block, the query tiles of a key block;
 // `flat`: every block takes ceil(all / KB).  The blocks with more than L turns are counted in closed form and L is found by

@@ -893,7 +893,7 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
  *   For the backward, else NULL: lse f32 [heads, total_q], the binary logarithm of a row's sum of exp (+infinity where a query
  *     sees no key); o_rest [total_q, heads, d] contiguous, AIT_DTYPE_BF16 only: what rounding took from o, without which the
- *     gradients of q and k carry o's rounding error.
+ *     gradients of q and k carry o's rounding error; with it the forward multiplies unrounded probabilities (bf16 value + rest).
  *
  * Backward: dq / dk / dv (pitches as given), and with a bias d_table [n_buckets, heads] of table_dtype
  * (overwritten; summed in f32; NULL: not wanted).
