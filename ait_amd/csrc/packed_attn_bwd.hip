@@ -45,10 +45,11 @@ struct BwdArgs {
   long long qs, qh, ks, kh, vs, vh, os, oh, dos, doh, dqs, dqh, dks, dkh, dvs, dvh;
   Seqs s;
   Bias bias;
-  int H, Hk, d, causal, qnumbers, knumbers, splits, stages;
+  int H, Hk, d, causal, qnumbers, knumbers, splits, stages, kparts;
   float scale;
   float* delta;       // [H][total_q]
   float* part_dq;     // [splits][total_q * H][d], not yet scaled: only where splits > 1
+  float* part_kv;     // [kparts][dK, dV][total_k][Hk][d], dK not yet scaled: only where kparts > 1
   float* part_table;  // [splits * qnumbers][H][n_buckets]; null: the table's gradient is not wanted
   void* d_table;
 };
@@ -312,13 +313,13 @@ __global__ __launch_bounds__(256) void packed_table_kernel(const BwdArgs a) {
 }
 
 // PARTS: 3 = dK and dV in one pass; 1 / 2: workgroups that form dV alone and workgroups that form dK alone
-template <typename T, int D, bool BIAS, int PART>
+// XH: 2 = the waves of a pair have the same 32 keys and half of a tile's queries each; 1 = every wave has keys of its own
+template <typename T, int D, bool BIAS, int PART, int XH>
 __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsigned char* lds) {
   constexpr bool DK = PART & 2, DV = PART & 1;
-  constexpr int XH = 2;
   constexpr int NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes, BN = NW / XH * 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int kvh = index % a.Hk, group = a.H / a.Hk, number = index / a.Hk, md = a.bias.max_distance;
+  const int kvh = index % a.Hk, group = a.H / a.Hk, part = index / a.Hk % a.kparts, number = index / a.Hk / a.kparts, md = a.bias.max_distance;
   Place place;
   if (!find_place<true>(a.s, 1, BN, number, 0, a.causal, place)) return;
   const int block = place.block, qstart = place.qstart, qlen = place.qlen, kstart = place.kstart, klen = place.klen, kroom = place.kroom;
@@ -326,7 +327,10 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   // query rows that see a key j: positions >= j - off with a causal mask
   const int gfirst = a.causal ? max(0, block * BN - off) : 0;
   const int wsure = a.causal ? max(0, min(key0 + 31, klen - 1) - off) : 0;          // from here on every key of the wave is seen
-  const int t0 = gfirst / KB, tq = block * BN < klen ? max(0, (qlen + KB - 1) / KB - t0) : 0, total = tq * group;
+  const int t0 = gfirst / KB, tq = block * BN < klen ? max(0, (qlen + KB - 1) / KB - t0) : 0, all = tq * group;
+  // this part's share of the turns, which run over the query tiles of one head after another's
+  const int first = (int)((long long)all * part / a.kparts), total = (int)((long long)all * (part + 1) / a.kparts) - first;
+  int g = total > 0 ? first / tq : 0, t = t0 + first - g * tq;
 
   const unsigned qstr = (unsigned)(a.qs * sizeof(T)), gstr = (unsigned)(a.dos * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lq, lg;
@@ -336,13 +340,13 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   // the next tile to load: its head, number, rows and rows left (pointers run on: a head's tiles lie one behind another)
   const T *pq = nullptr, *pg = nullptr;
   const float* ps = nullptr;
-  int nt = t0, nhead = kvh * group, left = 0;
+  int nt = t, nhead = kvh * group + g, left = 0;
   auto to_head = [&]() {
-    const long long r = qstart + (long long)t0 * KB;
+    const long long r = qstart + (long long)nt * KB;
     pq = reinterpret_cast<const T*>(a.q) + r * a.qs + (long long)nhead * a.qh;
     pg = reinterpret_cast<const T*>(a.d_o) + r * a.dos + (long long)nhead * a.doh;
     ps = (wave ? a.delta : a.lse) + (long long)nhead * a.s.total_q + r;
-    left = qlen - t0 * KB;
+    left = qlen - nt * KB;
   };
   auto fetch = [&](int stage) {
     lq.load(pq, left, qstr, dby, lds0 + stage * 2 * kTile, wave);
@@ -389,11 +393,10 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     for (int r = 0; r < 16; r++) ak[b][r] = av[b][r] = 0.f;
   float far_lo = 0.f, far_hi = 0.f;
 
-  int g = 0, t = t0;
   for (int it = 0; it < total; it++) {
     const int stage = it & 1, r0 = t * KB;
     if constexpr (BIAS) {
-      if (t == t0) {      // another head: its bias
+      if (it == 0 || t == t0) {      // another head: its bias
         __syncthreads();
         fill_bias<NT>(a.bias, a.H, kvh * group + g, 1, const_cast<float*>(bl), tid);
         __syncthreads();
@@ -413,8 +416,9 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       right = key0 - (last + off) >= md;
       near = !right && key0 + 31 - (r0 + off) > -md;
     }
-    const int x = xh;
-    {
+#pragma unroll
+    for (int xx = 0; xx < 2 / XH; xx++) {
+      const int x = XH == 1 ? xx : xh;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
@@ -479,7 +483,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     }
   }
 
-  {      // the two waves of a block of keys had half of the query rows each
+  if constexpr (XH == 2) {      // the two waves of a block of keys had half of the query rows each
     float* p = reinterpret_cast<float*>(lds) + kc * NB * 16 * 64 + lane;
 #pragma unroll
     for (int g = 0; g < 2; g++) {
@@ -503,6 +507,21 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     if (xh == 1) return;
   }
   if (key >= kroom) return;
+  if (a.kparts > 1) {
+    float* p = a.part_kv + (((long long)part * 2 * a.s.total_k + kstart + key) * a.Hk + kvh) * a.d;
+    const long long dv = (long long)a.s.total_k * a.Hk * a.d;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int dd = 32 * b + 8 * i + 4 * h;
+        if (dd < a.d) {
+          if (DK) store4(p + dd, ak[b][4 * i], ak[b][4 * i + 1], ak[b][4 * i + 2], ak[b][4 * i + 3]);
+          if (DV) store4(p + dv + dd, av[b][4 * i], av[b][4 * i + 1], av[b][4 * i + 2], av[b][4 * i + 3]);
+        }
+      }
+    return;
+  }
   T* pk = reinterpret_cast<T*>(a.dk) + (long long)(kstart + key) * a.dks + (long long)kvh * a.dkh;
   T* pv = reinterpret_cast<T*>(a.dv) + (long long)(kstart + key) * a.dvs + (long long)kvh * a.dvh;
 #pragma unroll
@@ -518,16 +537,36 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
 }
 
 // SPLIT: dK and dV by workgroups of their own (the keys' gradients, which have three products to dV's two, first)
-template <typename T, int D, bool BIAS, bool SPLIT>
+template <typename T, int D, bool BIAS, bool SPLIT, int XH>
 __global__ __launch_bounds__(NT, D == 128 && sizeof(T) == 4 ? 1 : 2) void packed_bwd_kv_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   if constexpr (SPLIT) {
-    const int n = a.knumbers * a.Hk;
-    if ((int)blockIdx.x < n) bwd_kv<T, D, BIAS, 2>(a, blockIdx.x, lds);
-    else bwd_kv<T, D, BIAS, 1>(a, blockIdx.x - n, lds);
+    const int n = a.knumbers * a.Hk * a.kparts;
+    if ((int)blockIdx.x < n) bwd_kv<T, D, BIAS, 2, XH>(a, blockIdx.x, lds);
+    else bwd_kv<T, D, BIAS, 1, XH>(a, blockIdx.x - n, lds);
   } else {
-    bwd_kv<T, D, BIAS, 3>(a, blockIdx.x, lds);
+    bwd_kv<T, D, BIAS, 3, XH>(a, blockIdx.x, lds);
   }
+}
+
+// the parts of dK and dV in their order: a thread has four values of a row and head
+template <typename T>
+__global__ __launch_bounds__(256) void packed_kv_join_kernel(const BwdArgs a) {
+  const int vecs = a.d / 4;
+  const long long n = (long long)a.s.total_k * a.Hk * vecs, id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n) return;
+  const long long rh = id / vecs;
+  const int dd = (int)(id - rh * vecs) * 4, row = (int)(rh / a.Hk), head = (int)(rh - (long long)row * a.Hk);
+  if (row < clamped(a.s.cu_k, 0, a.s.total_k) || (row >= clamped(a.s.cu_k, a.s.n_seq, a.s.total_k) && !a.s.rest)) return;
+  f32x4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
+  for (int s = 0; s < a.kparts; s++) {
+    const float* p = a.part_kv + (2 * s * n + id) * 4;
+    k += *reinterpret_cast<const f32x4*>(p);
+    v += *reinterpret_cast<const f32x4*>(p + n * 4);
+  }
+  k *= a.scale;
+  store4(reinterpret_cast<T*>(a.dk) + (long long)row * a.dks + (long long)head * a.dkh + dd, k[0], k[1], k[2], k[3]);
+  store4(reinterpret_cast<T*>(a.dv) + (long long)row * a.dvs + (long long)head * a.dvh + dd, v[0], v[1], v[2], v[3]);
 }
 template <typename K>
 int set_lds(K kernel, int bytes) {
@@ -535,7 +574,7 @@ int set_lds(K kernel, int bytes) {
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? AIT_OK : AIT_ELAUNCH;
 }
 // what the sizes decide for the pass over query rows: waves of a workgroup, parts of the key axis, tiles in flight
-struct Shape { int nw, splits, stages; };
+struct Shape { int nw, splits, stages, kwide, kparts; };
 Shape shape_of(const ait_packed_attn& p) {
   const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
   Shape r;
@@ -550,55 +589,75 @@ Shape shape_of(const ait_packed_attn& p) {
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   r.splits = s < 1 ? 1 : (int)s;
+  const bool split = p.dtype == AIT_DTYPE_BF16 && p.d > 64;
+  r.kwide = split && !p.bias_table && max_k >= 512;
+  const int bn = r.kwide ? NW * 32 : NW * 16;
+  const long long kblocks = p.total_k / bn > p.n_seq ? p.total_k / bn : p.n_seq, turns = (max_q + KB - 1) / KB * (p.heads / p.kv_heads);
+  const long long kw = (kblocks > 0 ? kblocks : 1) * p.kv_heads * (split ? 2 : 1);
+  s = r.kwide ? (1024 + kw - 1) / kw : 512 / kw;
+  if (s > turns / 8) s = turns / 8;
+  if (s > 16) s = 16;
+  r.kparts = s < 1 ? 1 : (int)s;
   return r;
 }
 
-template <typename T, int D, bool BIAS, int NWQ>
-int launch(BwdArgs a, hipStream_t st) {
-  const int bias = BIAS ? bias_row(a.bias.max_distance) * 4 : 0;
-  const int qb = 2 * a.stages * Tile<T, D>::kBytes + bias + (BIAS ? NWQ * (kSums<T, D> + a.bias.n_buckets) * 4 : 0);
-  const int kb = 4 * Tile<T, D>::kBytes + 1024 + bias;
+template <typename T, int D, bool BIAS, int XH>
+int launch_kv(BwdArgs a, hipStream_t st) {
+  const int bytes = 4 * Tile<T, D>::kBytes + 1024 + (BIAS ? bias_row(a.bias.max_distance) * 4 : 0);
   constexpr bool kSplit = D == 128 && sizeof(T) == 2;
-  const long long knumbers = block_numbers(a.s.total_k, 1, NW * 16, a.s.n_seq, a.s.rest);
-  if (!launchable((long long)a.qnumbers * a.H, NWQ * 64) || !launchable(knumbers * a.Hk * (kSplit ? 2 : 1), NT) ||
-      (a.splits > 1 && !launchable(((long long)a.s.total_q * a.H + 3) / 4, 256)))
-    return AIT_EUNSUPPORTED;
-  a.knumbers = (int)knumbers;
-  AIT_TRY_RC(set_lds(packed_bwd_q_kernel<T, D, BIAS, NWQ>, qb));
-  AIT_TRY_RC(set_lds(packed_bwd_kv_kernel<T, D, BIAS, kSplit>, kb));
-  if (a.s.total_q > 0) {
-    hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS, NWQ>), dim3((unsigned)(a.qnumbers * a.H), (unsigned)a.splits), dim3(NWQ * 64), qb, st, a);
-    AIT_CHECK_LAUNCH();
-    if (a.splits > 1) {
-      hipLaunchKernelGGL(packed_dq_join_kernel<T>, dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
-      AIT_CHECK_LAUNCH();
-    }
-  }
-  if (a.s.total_k > 0) {
-    hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS, kSplit>), dim3((unsigned)(a.knumbers * a.Hk * (kSplit ? 2 : 1))), dim3(NT), kb, st, a);
+  const long long numbers = block_numbers(a.s.total_k, 1, NW / XH * 32, a.s.n_seq, a.s.rest), wgs = numbers * a.Hk * a.kparts * (kSplit ? 2 : 1);
+  const long long vecs = (long long)a.s.total_k * a.Hk * (a.d / 4);
+  if (!launchable(wgs, NT) || (a.kparts > 1 && !launchable((vecs + 255) / 256, 256))) return AIT_EUNSUPPORTED;
+  a.knumbers = (int)numbers;
+  AIT_TRY_RC((set_lds(packed_bwd_kv_kernel<T, D, BIAS, kSplit, XH>, bytes)));
+  if (a.s.total_k == 0) return AIT_OK;
+  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, D, BIAS, kSplit, XH>), dim3((unsigned)wgs), dim3(NT), bytes, st, a);
+  AIT_CHECK_LAUNCH();
+  if (a.kparts > 1) {
+    hipLaunchKernelGGL(packed_kv_join_kernel<T>, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, st, a);
     AIT_CHECK_LAUNCH();
   }
   return AIT_OK;
 }
+template <typename T, int D, bool BIAS, int NWQ>
+int launch_q(const BwdArgs& a, hipStream_t st) {
+  const int bytes = 2 * a.stages * Tile<T, D>::kBytes + (BIAS ? (bias_row(a.bias.max_distance) + NWQ * (kSums<T, D> + a.bias.n_buckets)) * 4 : 0);
+  if (!launchable((long long)a.qnumbers * a.H, NWQ * 64) || (a.splits > 1 && !launchable(((long long)a.s.total_q * a.H + 3) / 4, 256)))
+    return AIT_EUNSUPPORTED;
+  AIT_TRY_RC((set_lds(packed_bwd_q_kernel<T, D, BIAS, NWQ>, bytes)));
+  if (a.s.total_q == 0) return AIT_OK;
+  hipLaunchKernelGGL((packed_bwd_q_kernel<T, D, BIAS, NWQ>), dim3((unsigned)(a.qnumbers * a.H), (unsigned)a.splits), dim3(NWQ * 64), bytes, st, a);
+  AIT_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(packed_dq_join_kernel<T>, dim3((unsigned)(((long long)a.s.total_q * a.H + 3) / 4)), dim3(256), 0, st, a);
+    AIT_CHECK_LAUNCH();
+  }
+  return AIT_OK;
+}
+template <typename T, int D, bool BIAS>
+int launch_b(const BwdArgs& a, const Shape& sh, hipStream_t st) {
+  AIT_TRY_RC((sh.nw == 2 ? launch_q<T, D, BIAS, 2>(a, st) : launch_q<T, D, BIAS, 4>(a, st)));
+  return sh.kwide ? launch_kv<T, D, BIAS, 1>(a, st) : launch_kv<T, D, BIAS, 2>(a, st);
+}
 template <typename T, int D>
-int launch_d(const BwdArgs& a, int nw, hipStream_t st) {
-  if (a.bias.table) return nw == 2 ? launch<T, D, true, 2>(a, st) : launch<T, D, true, 4>(a, st);
-  return nw == 2 ? launch<T, D, false, 2>(a, st) : launch<T, D, false, 4>(a, st);
+int launch_d(const BwdArgs& a, const Shape& sh, hipStream_t st) {
+  return a.bias.table ? launch_b<T, D, true>(a, sh, st) : launch_b<T, D, false>(a, sh, st);
 }
 template <typename T>
-int launch_t(const BwdArgs& a, int nw, hipStream_t st) {
-  return a.d <= 64 ? launch_d<T, 64>(a, nw, st) : launch_d<T, 128>(a, nw, st);
+int launch_t(const BwdArgs& a, const Shape& sh, hipStream_t st) {
+  return a.d <= 64 ? launch_d<T, 64>(a, sh, st) : launch_d<T, 128>(a, sh, st);
 }
 long long q_numbers(const ait_packed_attn& p, const Shape& s) { return block_numbers(p.total_q, 1, s.nw * 32, p.n_seq, p.zero_rest ? 1 : 0); }
-// floats: delta, the parts of dQ, the parts of the table's gradient
+// floats: delta, the parts of dQ, those of dK and dV, those of the table's gradient
 size_t delta_floats(const ait_packed_attn& p) { return ((size_t)p.heads * p.total_q + 3) / 4 * 4; }
 size_t dq_floats(const ait_packed_attn& p, const Shape& s) { return s.splits > 1 ? (size_t)s.splits * p.total_q * p.heads * p.d : 0; }
+size_t kv_floats(const ait_packed_attn& p, const Shape& s) { return s.kparts > 1 ? (size_t)s.kparts * 2 * p.total_k * p.kv_heads * p.d : 0; }
 }  // namespace
 
 AIT_API size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p) {
   if (ait_packed::check(p) != AIT_OK) return 0;
   const Shape s = shape_of(*p);
-  size_t n = delta_floats(*p) + dq_floats(*p, s);
+  size_t n = delta_floats(*p) + dq_floats(*p, s) + kv_floats(*p, s);
   if (p->bias_table) n += (size_t)s.splits * q_numbers(*p, s) * p->heads * p->n_buckets;
   return n * sizeof(float);
 }
@@ -629,11 +688,12 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
             dq_row, dq_head, dk_row, dk_head, dv_row, dv_head,
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
-            p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, p->scale,
-            static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, d_table};
-  if (p->bias_table && d_table) a.part_table = a.part_dq + dq_floats(*p, sh);
+            p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, sh.kparts, p->scale,
+            static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, nullptr, d_table};
+  a.part_kv = a.part_dq + dq_floats(*p, sh);
+  if (p->bias_table && d_table) a.part_table = a.part_kv + kv_floats(*p, sh);
   const hipStream_t st = ait_stream(stream);
-  AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, sh.nw, st) : launch_t<__bf16>(a, sh.nw, st));
+  AIT_TRY_RC(p->dtype == AIT_DTYPE_F32 ? launch_t<float>(a, sh, st) : launch_t<__bf16>(a, sh, st));
   if (p->bias_table && d_table) {
     if (p->total_q == 0) a.qnumbers = 0;
     hipLaunchKernelGGL(packed_table_kernel, dim3((unsigned)p->heads, (unsigned)((p->n_buckets + 15) / 16)), dim3(256), 0, st, a);

@@ -200,6 +200,39 @@ def test_how_the_work_is_cut_up_does_not_show(dtype, ql, kl, H, Hk, d, causal, b
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ql,kl,cap,H,Hk,d,causal,bias", [
+    ([1100], [70], 90, 4, 2, 64, False, True), ([2100], [64], 64, 1, 1, 128, True, False), ([700, 40, 0, 300], [600, 700, 5, 0], 701, 8, 2, 128, True, False),
+    ([1300], [520], 530, 2, 1, 72, False, False), ([640, 90], [3, 200], 257, 16, 2, 128, False, True), ([900], [900], 900, 2, 2, 64, True, True)])
+def test_gradients_of_few_keys_in_parts(dtype, ql, kl, cap, H, Hk, d, causal, bias):
+    """many queries on few keys: the query axis of the keys' gradients in parts that begin inside a head's tiles; wide blocks of
+    keys; cache rows behind a sequence's length and rows of no sequence get zeros and may hold anything"""
+    q, k, v, do = make(ql, kl, H, Hk, d, dtype, 41, cache=cap)
+    ks = [i * cap for i in range(len(kl) + 1)]
+    for t in (k, v):
+        for i, n in enumerate(kl):
+            t[ks[i] + n:ks[i + 1]] = float("nan")
+        t[ks[-1]:] = float("inf")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    b = None
+    if bias:
+        b = (torch.randn(12, H, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True), packed.relative_buckets(12, 50, True, "cuda"))
+        leaves.append(b[0])
+    args = starts(ql).cuda(), torch.tensor(ks, dtype=torch.int32).cuda()
+    run = lambda: packed.packed_attention(q, k, v, *args, k_len=torch.tensor(kl, dtype=torch.int32).cuda(), causal=causal, bias=b,
+                                          max_q=max(ql), max_k=max(kl))
+    o = run()
+    grads = torch.autograd.grad(o, leaves, do)
+    k, v = (torch.where(torch.isfinite(t), t, torch.zeros_like(t)).detach() for t in (k, v))
+    want = attn_ref(q, k, v, ql, starts(ql).tolist(), kl, ks, causal, d ** -0.5, *(b or (None, None)), do=do)
+    for n, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *grads)):
+        within(t, want[n], n)
+    k, v = leaves[1:3]
+    o2 = run()
+    assert all(torch.equal(x, y) for x, y in zip((o, *grads), (o2, *torch.autograd.grad(o2, leaves, do)))), "not the same twice"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new,kl,cap,H,Hk,d,bias", [
     ([1] * 4, [30, 1, 0, 77], 80, 8, 8, 64, False), ([1] * 2, [5000, 4097], 5001, 8, 2, 128, False), ([1, 1, 3], [700, 64, 65], 900, 32, 4, 64, True),
     ([7], [3000], 3000, 4, 4, 40, True), ([1], [1], 1, 1, 1, 8, True), ([40, 2], [1500, 2], 1600, 8, 2, 64, True)])
