@@ -11,11 +11,11 @@
 // accumulators in one, a wave a SIMD is left or registers spill (734 us against 497).
 //
 // What bounds it: the matrix unit, the exponentials between its products and the clock the chip holds under both.  3 documents of
-// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 240 us over the query rows, 497 over the keys (without its loads 366 of then
-// 508, with all of them to one address 471); of even lengths 1040 and 740 TFLOP/s executed, matrix unit 60 % and 40 % busy at
-// 1.7 GHz, no bank conflicts.  12 documents of 100 to 1800, 8 heads of 64: 65 and 61 us.  (Tried: eight waves a workgroup 291
-// against 257 and 589 against 515; masked and unmasked blocks as two loops: spills, 1694 us; waves that skip the blocks hidden
-// from them: 81 us instead of 86 for sequences of 1 to 49, 62.6 instead of 60.5 elsewhere.)
+// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 240 us over the query rows, 418 over the keys and 20 to join their two parts;
+// 4 of 4096 without a mask: 1010 and 980 TFLOP/s executed, no bank conflicts, matrix unit 60 % busy at 1.7 GHz.  12 documents of
+// 100 to 1800, 8 heads of 64: 65 and 62 us.  (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and
+// unmasked blocks as two loops: spills, 1694 us; waves that skip the blocks hidden from them: 81 us instead of 86 for sequences
+// of 1 to 49, 62.6 instead of 60.5 elsewhere; dK's and dV's workgroups in turn instead of dK's first: 459 us against 424.)
 #include "packed_attn_impl.h"
 
 namespace {
@@ -589,6 +589,13 @@ Shape shape_of(const ait_packed_attn& p) {
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   r.splits = s < 1 ? 1 : (int)s;
+  // Keys: 128 a workgroup for 128-wide bf16 heads, whose products load twice as much for 64 (4 documents of 4096, 16 heads on 4,
+  // no mask: 1404 us against 1845; 16 causal ones of 1000: 260 against 284, 64 of 200: 124 against 120); with a bias it would
+  // spill, and 64-wide heads gain nothing (documents of 100 to 1800: 61 us against 63; with a bias 70 against 63).
+  // Few blocks are cut along the queries, eight tiles at least to a part: of the wide ones, whose longest would outlast the
+  // launch under a causal mask, as many parts as make two rounds (3 documents of 2500 to 4095: 409 us in two and 22 to join them,
+  // 566 uncut; one of 4096: 201 + 13 in four, 504 uncut), of the others as many as fit at once (one of 2048, 8 heads of 64:
+  // 24 + 5 us in two, 31 uncut; two of 512 would lose, 13.5 + 4 against 12.9: eight tiles are all they have)
   const bool split = p.dtype == AIT_DTYPE_BF16 && p.d > 64;
   r.kwide = split && !p.bias_table && max_k >= 512;
   const int bn = r.kwide ? NW * 32 : NW * 16;
@@ -637,7 +644,9 @@ int launch_q(const BwdArgs& a, hipStream_t st) {
 template <typename T, int D, bool BIAS>
 int launch_b(const BwdArgs& a, const Shape& sh, hipStream_t st) {
   AIT_TRY_RC((sh.nw == 2 ? launch_q<T, D, BIAS, 2>(a, st) : launch_q<T, D, BIAS, 4>(a, st)));
-  return sh.kwide ? launch_kv<T, D, BIAS, 1>(a, st) : launch_kv<T, D, BIAS, 2>(a, st);
+  if constexpr (D == 128 && sizeof(T) == 2 && !BIAS)
+    if (sh.kwide) return launch_kv<T, D, BIAS, 1>(a, st);
+  return launch_kv<T, D, BIAS, 2>(a, st);
 }
 template <typename T, int D>
 int launch_d(const BwdArgs& a, const Shape& sh, hipStream_t st) {
