@@ -400,7 +400,7 @@ class on_device:
         self.index = dev.index
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
 

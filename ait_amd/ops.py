@@ -911,7 +911,8 @@ def packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=False):
     L = _lib.lib()
     dev = q.device
     q, k, v, o, d_o = _fit(q), _fit(k), _fit(v), _fit(o), _fit(d_o)
-    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    cf = torch.contiguous_format
+    dq, dk, dv = torch.empty_like(q, memory_format=cf), torch.empty_like(k, memory_format=cf), torch.empty_like(v, memory_format=cf)
     p.zero_rest = 1
     if p.n_seq == 0:
         dq.zero_(), dk.zero_(), dv.zero_()
@@ -921,11 +922,11 @@ def packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=False):
         if p.n_seq == 0 or p.total_q == 0:
             dt.zero_()
     with _lib.on_device(dev):
-        n = L.ait_packed_attn_bwd_workspace_bytes(ctypes.byref(p))
-        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        n = max(L.ait_packed_attn_bwd_workspace_bytes(ctypes.byref(p)), 16)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
         rc = L.ait_packed_attn_bwd(ctypes.byref(p), *_row_head(q), *_row_head(k), *_row_head(v), *_row_head(o),
                                    None if rest is None else rest.data_ptr(), *_row_head(d_o), lse.data_ptr(), *_row_head(dq), *_row_head(dk),
-                                   *_row_head(dv), None if dt is None else dt.data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(dev))
+                                   *_row_head(dv), None if dt is None else dt.data_ptr(), ws.data_ptr(), n, _lib.raw_stream(dev))
     _lib.check(rc, "ait_packed_attn_bwd")
     return dq, dk, dv, dt
 
@@ -1016,18 +1017,20 @@ def gated_norm_bwd(p, x, f, gate, stats, dy, dh):
     L = _lib.lib()
     dev = x.device
     dy, dh = _rows2d(dy), _rows2d(dh)
-    e = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
-    dx, df, dg = e(x), e(f), e(gate)
-    n = 2 + sum(t is not None for t in (p.scale, p.b_post, p.b_pre))
-    flat = torch.empty((n, p.width), dtype=torch.float32, device=dev)
-    it = iter(flat)
-    dwp, dwq = next(it), next(it)
-    ds, dbp, dbq = (next(it) if t is not None else None for t in (p.scale, p.b_post, p.b_pre))
-    vp = lambda t: None if t is None else t.data_ptr()
+    W, cf = p.width, torch.contiguous_format
+    dx, df = torch.empty_like(x, memory_format=cf), torch.empty_like(f, memory_format=cf)
+    dg = None if gate is None else torch.empty_like(gate, memory_format=cf)
+    given = p.scale is not None, p.b_post is not None, p.b_pre is not None
+    par = torch.empty((2 + sum(given), W), dtype=torch.float32, device=dev).unbind(0)
+    dwp, dwq = par[:2]
+    rest = list(par[2:])
+    ds, dbp, dbq = [rest.pop(0) if g else None for g in given]
     with _lib.on_device(dev):
-        nb = L.ait_gated_norm_bwd_workspace_bytes(ctypes.byref(p))
-        ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
-        rc = L.ait_gated_norm_bwd(ctypes.byref(p), vp(stats), vp(dy), dy.stride(0), vp(dh), dh.stride(0), vp(dx), p.width, vp(df), p.width,
-                                  vp(dg), p.width, vp(dwp), vp(dwq), vp(ds), vp(dbp), vp(dbq), vp(ws), ws.numel(), _lib.raw_stream(dev))
+        nb = max(L.ait_gated_norm_bwd_workspace_bytes(ctypes.byref(p)), 16)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        rc = L.ait_gated_norm_bwd(ctypes.byref(p), stats.data_ptr(), dy.data_ptr(), dy.stride(0), dh.data_ptr(), dh.stride(0), dx.data_ptr(), W,
+                                  df.data_ptr(), W, None if dg is None else dg.data_ptr(), W, dwp.data_ptr(), dwq.data_ptr(),
+                                  None if ds is None else ds.data_ptr(), None if dbp is None else dbp.data_ptr(),
+                                  None if dbq is None else dbq.data_ptr(), ws.data_ptr(), nb, _lib.raw_stream(dev))
     _lib.check(rc, "ait_gated_norm_bwd")
     return dx, df, dg, dwp, dbp, dwq, dbq, ds

@@ -21,6 +21,13 @@ def _recorded(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable, whose guard of a second derivative is entered only where one is recorded (autograd's worker thread
+    pays about 8 us for it, of some 160 us that a small training step takes on the host)"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of):
@@ -31,10 +38,10 @@ class _PackedAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_o):
         q, k, v, o, lse, rest, *keep = ctx.saved_tensors
-        p, n = _lib.PackedAttn.from_buffer_copy(ctx.p), ctx.needs_input_grad
+        p, n = ctx.p, ctx.needs_input_grad
         ops.packed_attn_point(p, *keep)
         dq, dk, dv, dt = ops.packed_attn_bwd(p, q, k, v, o, rest, d_o, lse, want_table=n[3])
         return dq if n[0] else None, dk if n[1] else None, dv if n[2] else None, dt, None, None, None, None, \
@@ -53,10 +60,16 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
     knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis).
 
     A query that sees no key gives zeros; so do rows behind the last sequence, and neither takes part in a gradient.  Gradients
-    of q, k, v and the table; a captured backward belongs to a forward captured in the same graph."""
+    of q, k, v and the table, not differentiable again.  In a captured graph the backward belongs to a forward captured with it,
+    while no eager graph of the same leaves is alive (autograd would wait for their streams inside the capture, which ends the
+    process: capture first, or with detached leaves)."""
     table = bucket_of = None
     if bias is not None:
-        table, bucket_of = (bias.weight, bias.bucket_of) if isinstance(bias, RelativePositionBias) else bias
+        if isinstance(bias, RelativePositionBias):
+            bias = bias.weight, bias.bucket_of
+        if not (isinstance(bias, (tuple, list)) and len(bias) == 2 and all(torch.is_tensor(t) for t in bias)):
+            raise _lib.AitHipError("packed_attention: `bias` must be (table, bucket_of) or a RelativePositionBias")
+        table, bucket_of = bias
     if cu_k is None:
         cu_k = cu_q
     if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded(q, k, v, table):
@@ -114,10 +127,10 @@ class _GatedNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy, dh):
         stats, *keep = ctx.saved_tensors
-        p = _lib.GatedNorm.from_buffer_copy(ctx.p)
+        p = ctx.p
         ops.gated_norm_point(p, *keep)
         dx, df, dg, *par = ops.gated_norm_bwd(p, keep[0], keep[1], keep[2], stats, dy, dh)
         grads = [dx, df, dg] + [None if t is None else t.to(dt) for t, dt in zip(par, ctx.types)]
@@ -139,6 +152,8 @@ def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, 
         raise ValueError("gated_norm: kind must be 'rms' or 'layer'")
     if not (torch.is_tensor(x) and torch.is_tensor(f) and x.dim() >= 1 and x.shape == f.shape):
         raise _lib.AitHipError("gated_norm: x and f must be tensors of one shape")
+    if gate is not None and not torch.is_tensor(gate):
+        raise _lib.AitHipError("gated_norm: the gate must be a tensor")
     if cu_seqlens is not None and x.dim() != 2:
         raise _lib.AitHipError("gated_norm: with cu_seqlens x must be [rows, width]")
     for n, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("post_bias", post_bias), ("pre_bias", pre_bias), ("scale", scale)):

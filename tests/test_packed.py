@@ -775,3 +775,41 @@ def test_gradients_against_differences(what):
         near, far = slope(e), slope(2 * e)
         # the steps' error falls by four from 2 e to e: what is left at e is a third of what they differ by
         assert abs(float((grads[i].double() * d.double()).sum()) - near) <= abs(near - far) / 3 * 1.5 + 4 * noise / e, (what, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["attention", "norm"])
+def test_a_graph_is_walked_twice_and_has_no_second_derivative(what):
+    g = torch.Generator().manual_seed(77)
+    t = lambda *s: torch.randn(*s, generator=g).cuda().requires_grad_(True)
+    if what == "attention":
+        leaves, cu = [t(20, 2, 16) for _ in range(3)], starts([9, 11]).cuda()
+        out = (packed.packed_attention(*leaves, cu, causal=True),)
+    else:
+        leaves = [t(20, 24), t(20, 24), t(24), t(24)]
+        out = packed.gated_norm(leaves[0], leaves[1], post_weight=leaves[2], pre_weight=leaves[3])
+    up = [torch.randn(o.shape, generator=g).cuda() for o in out]
+    first = torch.autograd.grad(out, leaves, up, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, up, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    up = [u.requires_grad_(True) for u in up]
+    third = torch.autograd.grad(out, leaves, up, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, third))
+    with pytest.raises(RuntimeError):
+        third[0].sum().backward()
+
+
+def test_arguments_that_are_no_tensors_are_refused():
+    t = lambda *s: torch.zeros(*s, requires_grad=True)
+    cu = starts([2, 3])
+    table, of = t(8, 4), packed.relative_buckets(8, 20, True)
+    for change in (dict(bias=([1.0], of)), dict(bias=(table, [0, 1, 2])), dict(bias=(table,)), dict(bias=table), dict(cu_q=[0, 2, 5]), dict(cu_k=(0, 5)),
+                   dict(k_len=[2, 3]), dict(q=[1.0]), dict(v=None)):
+        with pytest.raises(_lib.AitHipError):
+            packed.packed_attention(**{**dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cu_q=cu), **change})
+            pytest.fail("taken: %s" % list(change))
+    for change in (dict(gate=[1.0]), dict(gate=1.0), dict(x=t(2, 5, 8), f=t(2, 5, 8), gate=2.0), dict(scale=1.0), dict(cu_seqlens=[0, 5], gate=t(1, 8)),
+                   dict(x=None), dict(f=3.0), dict(post_weight=None), dict(pre_weight=1.0)):
+        with pytest.raises(_lib.AitHipError):
+            packed.gated_norm(**{**dict(x=t(5, 8), f=t(5, 8), post_weight=t(8), pre_weight=t(8)), **change})
+            pytest.fail("taken: %s" % list(change))
