@@ -10,11 +10,15 @@
 // parameters' gradients) in registers over the rows of a workgroup; the workgroups' parts are added in order by a second
 // kernel, so results repeat bit for bit.
 //
-// What bounds it: memory.  58800 rows of 512 in f32, LayerNorm: forward 482 MB in 97 us (5.0 TB/s; a large copy reaches 4.9
-// here), backward 722 MB in 153 (4.7).  About 12600 packed rows of 5120, f32 stream and bf16 branch, a gate a sequence: forward
-// 774 MB in 167 to 176 us (4.5), backward 1162 MB in 320 to 335 (3.5): ten waves of a row meet at two barriers a row and one
-// workgroup fits a CU, so its loads pause.  Five rows of 4096: 4.4 us, a launch and three dependent trips to memory.
+// What bounds it: memory.  58800 rows of 512 in f32, LayerNorm: forward 482 MB in 98 us (4.9 TB/s, a large copy's rate here),
+// backward 722 MB in 149 (4.8).  About 12600 packed rows of 5120, f32 stream and bf16 branch, a gate a sequence: forward 774 MB
+// in 165 us (4.7), backward 1162 MB in 241 (4.8).  What it took in the backward, where one workgroup of ten waves fits a CU and
+// its phases meet at barriers: a row's loads without branches around them, so that they are in flight together, sums over the
+// lanes without trips to shared memory, and parameters held (335 us before the three).  Five rows of 4096: 3.8 us, a launch and
+// three dependent trips to memory.
 #include "common.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -95,14 +99,59 @@ __device__ __forceinline__ void store8(T* row, int at, int width, const float* v
   }
 }
 
+// Eight values of a row on their way: loads without a branch around them (behind the row's end its last ones are loaded, and not
+// taken), so that all of a row's loads are in flight together.  In a branch each is waited for before the next one is issued.
+template <bool VEC, typename T> struct In;
+template <> struct In<true, __bf16> {
+  bf16x8 t;
+  __device__ __forceinline__ void load(const __bf16* row, int at, int width) { t = *reinterpret_cast<const bf16x8*>(row + min(at, width - 8)); }
+  __device__ __forceinline__ void get(float* v, bool there) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = there ? (float)t[e] : 0.f;
+  }
+};
+template <> struct In<true, float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* row, int at, int width) {
+    const float* p = row + min(at, width - 8);
+    a = *reinterpret_cast<const f32x4*>(p);
+    b = *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  __device__ __forceinline__ void get(float* v, bool there) const {
+#pragma unroll
+    for (int e = 0; e < 4; e++) { v[e] = there ? a[e] : 0.f; v[4 + e] = there ? b[e] : 0.f; }
+  }
+};
+template <typename T> struct In<false, T> {
+  float t[8];
+  __device__ __forceinline__ void load(const T* row, int at, int width) { load8<false>(row, at, width, t); }
+  __device__ __forceinline__ void get(float* v, bool there) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = there ? t[e] : 0.f;
+  }
+};
+
 template <bool VEC>
 __device__ __forceinline__ bool inside(int at, int e, int width) { return VEC ? at < width : at + e < width; }
 
+// the sum of a wave's lanes, in every lane: inside 16 lanes, over the 16s, from the last lane (no trip to shared memory)
+__device__ __forceinline__ float lane_sum(float v) {
+#define AIT_DPP_ADD(ctrl, rows) \
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, true))
+  AIT_DPP_ADD(0x111, 0xf);
+  AIT_DPP_ADD(0x112, 0xf);
+  AIT_DPP_ADD(0x114, 0xf);
+  AIT_DPP_ADD(0x118, 0xf);
+  AIT_DPP_ADD(0x142, 0xa);
+  AIT_DPP_ADD(0x143, 0xc);
+#undef AIT_DPP_ADD
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 // sums over the G waves of a row, two at a time; every lane gets them.  `slot` alternates so that one barrier a sum is enough
 template <int G>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* lds, int& slot, int group_wave, int wave) {
-  a = wave_sum(a);
-  b = wave_sum(b);
+  a = lane_sum(a);
+  b = lane_sum(b);
   if constexpr (G > 1) {
     float* p = lds + (slot & 1) * 32;
     slot++;
@@ -146,10 +195,21 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_fwd_kernel(cons
   const bool dead = a.gate_kind == 2 && seq == a.n_seq;          // behind the last sequence: left as it is, or set to zero
   const bool write = there && (!dead || a.zero_rest);
   float f[V][8], x[V][8];
+  {
+    In<VEC, F> rf[V];
+    In<VEC, X> rx[V];
 #pragma unroll
-  for (int v = 0; v < V; v++) load8<VEC>(reinterpret_cast<const F*>(a.f) + rc * a.f_row, (gl + v * G * 64) * 8, W, f[v]);
+    for (int v = 0; v < V; v++) {
+      rf[v].load(reinterpret_cast<const F*>(a.f) + rc * a.f_row, (gl + v * G * 64) * 8, W);
+      rx[v].load(reinterpret_cast<const X*>(a.x) + rc * a.x_row, (gl + v * G * 64) * 8, W);
+    }
 #pragma unroll
-  for (int v = 0; v < V; v++) load8<VEC>(reinterpret_cast<const X*>(a.x) + rc * a.x_row, (gl + v * G * 64) * 8, W, x[v]);
+    for (int v = 0; v < V; v++) {
+      const bool in = !VEC || (gl + v * G * 64) * 8 < W;
+      rf[v].get(f[v], in);
+      rx[v].get(x[v], in);
+    }
+  }
   float mean = 0.f, s1 = 0.f, s2 = 0.f;
   if (a.layer) {
 #pragma unroll
@@ -260,23 +320,70 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
     for (int e = 0; e < 8; e++) cp[v][e] = cq[v][e] = cs[v][e] = bp[v][e] = bq[v][e] = cg[v][e] = 0.f;
   const int unit = blockIdx.x * R + group, first = unit * a.per, last = min(first + a.per, a.rows);
   float* gate_parts = a.parts + (size_t)a.blocks * a.n_parts * W;
-  // The parameters of a lane's values, read once for all rows where registers allow it: one block of eight a lane and up to
-  // eight waves (f32 rows of 512: 161 -> 153 us; ten and twelve waves have 168 registers a lane, which spill, and gain nothing)
-  constexpr bool HELD = V == 1 && G <= 8;
-  float w1[1][8], w2[1][8], w3[1][8];
-  if constexpr (HELD) {
-    load8<VEC>(a.w_post, gl * 8, W, w1[0]);
-    load8<VEC>(a.w_pre, gl * 8, W, w2[0]);
+  // The parameters of a lane's values are held over all rows where a lane has one block of eight: in registers up to eight waves,
+  // in shared memory for more, whose 168 registers a lane would spill.  (The next row's loads issued under this one's arithmetic
+  // gain nothing where registers allow it, 150 us against 149, and spill in ten waves: 280 against 241.)
+  constexpr bool HELD = V == 1 && G <= 8, LDSP = V == 1 && !HELD;
+  __shared__ __attribute__((aligned(16))) float wl[LDSP ? (SUMS_B ? 4 : 3) : 1][LDSP ? G * 512 : 4];
+  const float* from[4] = {a.w_post, a.w_pre, a.scale, a.b_post};
+  float w[HELD ? 4 : 1][8];
+  if constexpr (V == 1) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) w3[0][e] = 1.f;
-    if (a.scale) load8<VEC>(a.scale, gl * 8, W, w3[0]);
+    for (int i = 0; i < (SUMS_B ? 4 : 3); i++) {
+      float t[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) t[e] = i == 2 ? 1.f : 0.f;
+      if (from[i]) load8<VEC>(from[i], gl * 8, W, t);
+      if constexpr (HELD) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[i][e] = t[e];
+      } else {      // (a lane reads what it wrote itself: no barrier)
+        store8<true>(&wl[i][0], gl * 8, G * 512, t);
+      }
+    }
   }
-  auto held = [&](const float (&w)[1][8], float* to) {
+  auto parameter = [&](auto which, int at, float* to) {      // 0 w_post, 1 w_pre, 2 scale or 1, 3 b_post or 0
+    constexpr int i = decltype(which)::value;
+    if constexpr (HELD) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) to[e] = w[0][e];
+      for (int e = 0; e < 8; e++) to[e] = w[i][e];
+    } else if constexpr (LDSP) {
+      load8<true>(&wl[i][0], gl * 8, G * 512, to);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) to[e] = i == 2 ? 1.f : 0.f;
+      if (i < 2 || from[i]) load8<VEC>(from[i], at, W, to);
+    }
+  };
+  constexpr std::integral_constant<int, 0> kPost{};
+  constexpr std::integral_constant<int, 1> kPre{};
+  constexpr std::integral_constant<int, 2> kScale{};
+  constexpr std::integral_constant<int, 3> kPostBias{};
+  In<VEC, F> rf[V], rd[V], rg[V];
+  In<VEC, X> ry[V], rt[V];
+  f32x4 rs;
+  auto fetch = [&](int row) {
+    const long long rc = min(row, a.rows - 1);
+    rs = *reinterpret_cast<const f32x4*>(a.stats + 4 * rc);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int at = (gl + v * G * 64) * 8;
+      rf[v].load(reinterpret_cast<const F*>(a.f) + rc * a.f_row, at, W);
+      ry[v].load(reinterpret_cast<const X*>(a.x) + rc * a.x_row, at, W);
+      rd[v].load(reinterpret_cast<const F*>(a.dh) + rc * a.dh_row, at, W);
+      rt[v].load(reinterpret_cast<const X*>(a.dy) + rc * a.dy_row, at, W);
+      if (a.gate_kind == 1) rg[v].load(reinterpret_cast<const F*>(a.gate) + rc * a.g_row, at, W);
+    }
+  };
+  auto fetch_gate = [&](int s) {
+#pragma unroll
+    for (int v = 0; v < V; v++) rg[v].load(reinterpret_cast<const F*>(a.gate) + (s < a.n_seq ? s : 0) * a.g_row, (gl + v * G * 64) * 8, W);
   };
   int seq = 0;
-  if (a.gate_kind == 2 && first < a.rows) seq = seq_of(a.cu, a.n_seq, a.rows, first);
+  if (a.gate_kind == 2) {
+    if (first < a.rows) seq = seq_of(a.cu, a.n_seq, a.rows, first);
+    if (a.n_seq > 0) fetch_gate(seq);
+  }
   for (int i = 0; i < a.per; i++) {          // (every group makes every turn: the sums meet at barriers)
     const int row = first + i;
     const bool there = row < last;
@@ -291,52 +398,46 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
         for (int e = 0; e < 8; e++) cg[v][e] = 0.f;
       }
       seq = seq_of(a.cu, a.n_seq, a.rows, row);
+      fetch_gate(seq);
     }
     const bool dead = !there || (a.gate_kind == 2 && seq == a.n_seq);
     const bool write = there && (!dead || a.zero_rest);
-    const int L = dead ? 0 : W;             // a dead row is a row of zeros, whatever memory holds
-    f32x4 st = *reinterpret_cast<const f32x4*>(a.stats + 4ll * rc);
+    fetch(row);
+    // a dead row is a row of zeros, whatever memory holds
+    f32x4 st = rs;
     if (dead) st[0] = st[1] = st[2] = st[3] = 0.f;
-    float f[V][8], y[V][8], d[V][8], t[V][8];
+    float f[V][8], y[V][8], d[V][8], t[V][8], gate[V][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-      const int at = (gl + v * G * 64) * 8;
-      load8<VEC>(reinterpret_cast<const F*>(a.f) + rc * a.f_row, at, L, f[v]);
-      load8<VEC>(reinterpret_cast<const X*>(a.x) + rc * a.x_row, at, L, y[v]);
-      load8<VEC>(reinterpret_cast<const F*>(a.dh) + rc * a.dh_row, at, L, d[v]);
-      load8<VEC>(reinterpret_cast<const X*>(a.dy) + rc * a.dy_row, at, L, t[v]);
+      const bool in = !dead && (!VEC || (gl + v * G * 64) * 8 < W);
+      rf[v].get(f[v], in);
+      ry[v].get(y[v], in);
+      rd[v].get(d[v], in);
+      rt[v].get(t[v], in);
+#pragma unroll
+      for (int e = 0; e < 8; e++) gate[v][e] = 1.f;
+      if (a.gate_kind) rg[v].get(gate[v], in);
     }
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int at = (gl + v * G * 64) * 8;
       float p[8], q[8], m[8];
-      if constexpr (HELD) held(w1, p);
-      else load8<VEC>(a.w_post, at, W, p);
+      parameter(kPost, at, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         f[v][e] = inside<VEC>(at, e, W) ? (f[v][e] - st[0]) * st[1] : 0.f;       // norm(f)
         m[e] = f[v][e] * p[e];
       }
-      if (SUMS_B && a.b_post) {
-        load8<VEC>(a.b_post, at, W, p);
+      if constexpr (SUMS_B) {
+        parameter(kPostBias, at, p);
 #pragma unroll
         for (int e = 0; e < 8; e++) m[e] += p[e];
       }
+      parameter(kScale, at, q);
 #pragma unroll
-      for (int e = 0; e < 8; e++) p[e] = 1.f;
-      if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
-      if constexpr (HELD) {
-        held(w3, q);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) q[e] = 1.f;
-        if (a.scale) load8<VEC>(a.scale, at, W, q);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[v][e] = inside<VEC>(at, e, W) ? (y[v][e] + m[e] * p[e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
-      if constexpr (HELD) held(w2, p);
-      else load8<VEC>(a.w_pre, at, W, p);
+      for (int e = 0; e < 8; e++) y[v][e] = inside<VEC>(at, e, W) ? (y[v][e] + m[e] * gate[v][e] * q[e] - st[2]) * st[3] : 0.f;      // norm(y)
+      parameter(kPre, at, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         cq[v][e] = __builtin_fmaf(d[v][e], y[v][e], cq[v][e]);
@@ -353,34 +454,24 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int at = (gl + v * G * 64) * 8;
-      float p[8], q[8], m[8], b[8];
+      float q[8], m[8], b[8];
       float* u = t[v];
 #pragma unroll
       for (int e = 0; e < 8; e++) u[e] = u[e] + st[3] * (d[v][e] - s2 - y[v][e] * s1);        // d y
       if (write) store8<VEC>(reinterpret_cast<X*>(a.dx) + rc * a.dx_row, at, W, u);
-#pragma unroll
-      for (int e = 0; e < 8; e++) p[e] = 1.f;
-      if (a.gate_kind) load8<VEC>(reinterpret_cast<const F*>(a.gate) + (a.gate_kind == 2 ? (dead ? 0 : seq) : rc) * a.g_row, at, L, p);
-      if constexpr (HELD) {
-        held(w3, q);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) q[e] = 1.f;
-        if (a.scale) load8<VEC>(a.scale, at, W, q);
-      }
-      if constexpr (HELD) held(w1, m);
-      else load8<VEC>(a.w_post, at, W, m);
+      parameter(kScale, at, q);
+      parameter(kPost, at, m);
 #pragma unroll
       for (int e = 0; e < 8; e++) b[e] = 0.f;
-      if (SUMS_B && a.b_post) load8<VEC>(a.b_post, at, W, b);
+      if constexpr (SUMS_B) parameter(kPostBias, at, b);
       float k[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float um = u[e] * (f[v][e] * m[e] + b[e]);
-        cs[v][e] = __builtin_fmaf(um, p[e], cs[v][e]);
+        cs[v][e] = __builtin_fmaf(um, gate[v][e], cs[v][e]);
         k[e] = um * q[e];                                            // d gate
         cg[v][e] += k[e];
-        u[e] *= p[e] * q[e];                                         // d m
+        u[e] *= gate[v][e] * q[e];                                         // d m
         if (SUMS_B) bp[v][e] += u[e];
         cp[v][e] = __builtin_fmaf(u[e], f[v][e], cp[v][e]);
       }
@@ -510,8 +601,8 @@ int launch_gv(const NormArgs& a, hipStream_t st) {
 }
 template <typename X, typename F, bool BWD>
 int launch_xf(const NormArgs& a, bool vec, hipStream_t st) {
-  // as many waves as the row fills: one block of eight values a lane up to 6144, two beyond (rows of 5120: backward 335 us in
-  // ten waves of one block, 395 in eight of two, forward alike; rows of 512: forward 96 us in one wave, 100 in two)
+  // as many waves as the row fills: one block of eight values a lane up to 6144, two beyond (rows of 5120: backward a
+  // sixth faster in ten waves of one block than in eight of two, forward alike; rows of 512: forward 96 us in one wave, 100 in two)
   if (!vec) {
     if (a.width <= 512) return launch_gv<X, F, BWD, false, 1, 1>(a, st);
     if (a.width <= 2048) return launch_gv<X, F, BWD, false, 4, 1>(a, st);

@@ -163,7 +163,7 @@ def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, 
     if x.dim() != 2:
         if gate is not None and gate.shape != shape:
             raise _lib.AitHipError("gated_norm: a gate without cu_seqlens has x's shape")
-        x, f, gate = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, f, gate))
+        x, f, gate = (None if t is None else t[None] if len(shape) == 1 else t.flatten(0, -2) for t in (x, f, gate))
     if _recorded(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale):
         y, h = _GatedNorm.apply(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale, cu_seqlens, kind == "layer", eps)
     else:

@@ -934,7 +934,7 @@ int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row
  *   x [rows, width] of dtype_x (pitch x_row elements), f of dtype_f; (AIT_DTYPE_F32, F32), (F32, BF16) and (BF16, BF16).
  *     y as x, h as f.  width up to 8192; rows of whole 16-byte vectors (width, pitches, bases) take wide loads, others single ones.
  *   gate NULL, [rows, width] of dtype_f, or with cu_seqlens int32 [n_seq + 1] (ascending from 0) [n_seq, width]: row r's is that
- *     of its sequence; rows behind the last sequence are not read, and what belongs to them is left as it is (zero_rest: zeroed).
+ *     of its sequence; what rows behind the last sequence hold does not count, and what belongs to them is left as it is (zero_rest: zeroed).
  *   scale, b_post, b_pre: NULL or f32 [width]; w_post, w_pre f32 [width].
  *   stats f32 [rows, 4] (16-byte base): what the backward reads; NULL in inference.
  * h is formed from y before its rounding to dtype_x, and so is the backward.  Backward: gradients of everything given (of y and

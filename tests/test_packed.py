@@ -809,7 +809,7 @@ def test_arguments_that_are_no_tensors_are_refused():
             packed.packed_attention(**{**dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cu_q=cu), **change})
             pytest.fail("taken: %s" % list(change))
     for change in (dict(gate=[1.0]), dict(gate=1.0), dict(x=t(2, 5, 8), f=t(2, 5, 8), gate=2.0), dict(scale=1.0), dict(cu_seqlens=[0, 5], gate=t(1, 8)),
-                   dict(x=None), dict(f=3.0), dict(post_weight=None), dict(pre_weight=1.0)):
+                   dict(x=t(2, 3, 0), f=t(2, 3, 0)), dict(x=None), dict(f=3.0), dict(post_weight=None), dict(pre_weight=1.0)):
         with pytest.raises(_lib.AitHipError):
             packed.gated_norm(**{**dict(x=t(5, 8), f=t(5, 8), post_weight=t(8), pre_weight=t(8)), **change})
             pytest.fail("taken: %s" % list(change))
