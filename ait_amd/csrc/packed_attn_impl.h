@@ -183,6 +183,9 @@ __device__ __forceinline__ i32x4 tile_rsrc(const void* base, unsigned bytes) {
   r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(p >> 32) & 0xffffu));
   r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
   r[3] = 0x00027000;
+  // a vector instruction's scalar result (readfirstlane) must be five wait states old where a memory instruction reads it; the
+  // compiler keeps to that for its own instructions but does not look into the asm of the loads below
+  asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
 __device__ __forceinline__ void load_lds16(unsigned voff, const i32x4& rsrc, unsigned dst) {
