@@ -90,15 +90,6 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
     t1 = min(t1, t0 + per);
   }
 
-  Frag<T> qf[NCH];
-  {
-    const T* qr = reinterpret_cast<const T*>(a.q) + (long long)(qstart + pos) * a.qs + (long long)head * a.qh;
-#pragma unroll
-    for (int c = 0; c < NCH; c++) {
-      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < rows);
-      if (a.scale < 0.f) qf[c] = -qf[c];      // (so that the largest product is the largest score)
-    }
-  }
   const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lk, lv;
   lk.init(tid, kstr, dby);
@@ -114,6 +105,16 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
   const float* bl = reinterpret_cast<const float*>(lds + 2 * a.stages * kTile);
   float far_lo = 0.f, far_hi = 0.f;
   if (t0 < t1) fetch(t0, 0);
+  Frag<T> qf[NCH];
+  {
+    // (a negative scale: so that the largest product is the largest score)
+    const unsigned flip = a.scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+    const T* qr = reinterpret_cast<const T*>(a.q) + (long long)(qstart + pos) * a.qs + (long long)head * a.qh;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) {
+      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < rows, flip);
+    }
+  }
   if constexpr (BIAS) {
     const int md = a.bias.max_distance, first = block * BM / a.pack, last = (min(block * BM + BM, rows) - 1) / a.pack;
     far_lo = bias_log2(a.bias, (size_t)bucket(a.bias, -md) * a.H + head);

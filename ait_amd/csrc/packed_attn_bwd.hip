@@ -108,23 +108,31 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
     const T* qr = reinterpret_cast<const T*>(a.q) + at * a.qs + (long long)head * a.qh;
     const T* gr = reinterpret_cast<const T*>(a.d_o) + at * a.dos + (long long)head * a.doh;
     const T* orow = reinterpret_cast<const T*>(a.o) + at * a.os + (long long)head * a.oh;
+    Frag<T> of[NCH], rf[NCH];
+    const bool there = row < qlen, rest = sizeof(T) == 2 && a.rest;
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
-      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, row < qlen);
-      gf[c] = global_frag<T>(gr, 16 * c + 8 * h, a.d, row < qlen);
-      const Frag<T> of = global_frag<T>(orow, 16 * c + 8 * h, a.d, row < qlen);
+      gf[c] = global_frag<T>(gr, 16 * c + 8 * h, a.d, there);
+      of[c] = global_frag<T>(orow, 16 * c + 8 * h, a.d, there);
+      qf[c] = global_frag<T>(qr, 16 * c + 8 * h, a.d, there);
+    }
+    l2 = a.lse[(long long)head * a.s.total_q + at];
+    if (rest) {
+      const T* rr = reinterpret_cast<const T*>(a.rest) + (at * a.H + head) * a.d;
 #pragma unroll
-      for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)of[e], delta);
-      if constexpr (sizeof(T) == 2) {
-        if (a.rest) {
-          const Frag<T> rf = global_frag<T>(reinterpret_cast<const T*>(a.rest) + (at * a.H + head) * a.d, 16 * c + 8 * h, a.d, row < qlen);
+      for (int c = 0; c < NCH; c++) rf[c] = global_frag<T>(rr, 16 * c + 8 * h, a.d, there);
+    }
 #pragma unroll
-          for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)rf[e], delta);
-        }
-      }
+    for (int c = 0; c < NCH; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)of[c][e], delta);
+    if (rest) {
+#pragma unroll
+      for (int c = 0; c < NCH; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) delta = __builtin_fmaf((float)gf[c][e], (float)rf[c][e], delta);
     }
     delta = column_sum(delta);
-    l2 = a.lse[(long long)head * a.s.total_q + at];
     if (row < qlen && h == 0 && blockIdx.y == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
     // (a query that sees one key has no gradient of its scores: exactly zero, not the rounding of dP - delta)
     if (row >= qlen || kmax <= 1) l2 = -kNegInf;

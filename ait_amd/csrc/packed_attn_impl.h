@@ -222,22 +222,23 @@ struct Loader {
 
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(const lds_u8*)p; }
 
-// eight values of a row in memory as an operand (values >= d, and rows that are not there: zero)
+// Eight values of a row in memory as an operand; values >= d, and rows that are not there (`row` is then any row that is): zero.
+// No branch around the load, so that a row's loads are in flight together.  flip: the sign bits to turn over, as bits (negated
+// as a vector of bf16 behind the select, one value in two came out of the compiler with the wrong sign)
 template <typename T>
-__device__ __forceinline__ Frag<T> global_frag(const T* row, int at, int d, bool there) {
-  Frag<T> f;
+__device__ __forceinline__ Frag<T> global_frag(const T* row, int at, int d, bool there, unsigned flip = 0) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  struct Words { u32x4 w[sizeof(T) / 2]; };
+  const T* p = row + min(at, d - 8);
+  const bool in = there && at < d;
+  Words f;
 #pragma unroll
-  for (int e = 0; e < 8; e++) f[e] = (T)0.f;
-  if (there && at < d) {
-    if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const bf16x8*>(row + at);
-    } else {
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(row + at), hi = *reinterpret_cast<const f32x4*>(row + at + 4);
+  for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+    const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
 #pragma unroll
-      for (int e = 0; e < 4; e++) { f[e] = lo[e]; f[4 + e] = hi[e]; }
-    }
+    for (int e = 0; e < 4; e++) f.w[i][e] = (in ? v[e] : 0u) ^ flip;
   }
-  return f;
+  return __builtin_bit_cast(Frag<T>, f);
 }
 
 // four consecutive values of a row
@@ -291,7 +292,7 @@ __device__ __forceinline__ bool find_block(const int* cu, int n_seq, int rest, i
   while (true) {
     const int step = (count + 63) / 64, b = lo + lane * step;
     const bool there = lane * step < count;
-    const int c = there ? clamped(cu, b, total) : 0, e = !there ? 0 : b < n_seq ? clamped(cu, b + 1, total) : total;
+    const int c = clamped(cu, min(b, n_seq), total), next = clamped(cu, min(b + 1, n_seq), total), e = b < n_seq ? next : total;
     // (the first candidate counts in any case; what follows a later one is later, in a table that ascends)
     const unsigned long long ok = __ballot(there && (lane == 0 || (int)((long long)c * mul / bm) + b <= number));
     const int t = 63 - __builtin_clzll(ok);
@@ -364,13 +365,11 @@ struct Seqs {
   int ordered;             // blocks in the order of heaviest_first
 };
 __device__ __forceinline__ void keys_of(const Seqs& s, int seq, int& start, int& len) {
-  start = clamped(s.cu_k, seq, s.total_k);
-  len = clamped(s.cu_k, seq + 1, s.total_k) - start;
-  if (len < 0) len = 0;
-  if (s.k_len) {
-    const int l = s.k_len[seq];
-    len = l < 0 ? 0 : l < len ? l : len;
-  }
+  const int from = s.cu_k[seq], to = s.cu_k[seq + 1];
+  int l = s.total_k;
+  if (s.k_len) l = s.k_len[seq];
+  start = min(max(from, 0), s.total_k);
+  len = max(0, min(min(max(to, 0), s.total_k) - start, l));
 }
 
 // A workgroup's place: block `number` of the query rows (mul rows to a position, bm to a block) or, KEYS, of the key rows (bm to a
@@ -381,11 +380,13 @@ __device__ __forceinline__ bool find_place(const Seqs& s, int mul, int bm, int n
   if (s.ordered) {
     const int lane = threadIdx.x & 63, n = s.n_seq + s.rest, b = lane < n ? lane : n - 1;
     const bool seq = b < s.n_seq;
-    const int qs = clamped(s.cu_q, b, s.total_q), qe = seq ? clamped(s.cu_q, b + 1, s.total_q) : s.total_q;
-    const int ks = clamped(s.cu_k, b, s.total_k), ke = seq ? clamped(s.cu_k, b + 1, s.total_k) : s.total_k;
-    const int len = max(0, qe - qs), room = max(0, ke - ks);
-    int kl = seq ? room : 0;
-    if (s.k_len && seq) kl = max(0, min(kl, s.k_len[b]));
+    // (the loads together, then what is done with them)
+    const int to = min(b + 1, s.n_seq), q0 = s.cu_q[b], q1 = s.cu_q[to], k0 = s.cu_k[b], k1 = s.cu_k[to];
+    int l = s.total_k;
+    if (s.k_len) l = s.k_len[min(b, s.n_seq - 1)];
+    const int qs = min(max(q0, 0), s.total_q), qe = seq ? min(max(q1, 0), s.total_q) : s.total_q;
+    const int ks = min(max(k0, 0), s.total_k), ke = seq ? min(max(k1, 0), s.total_k) : s.total_k;
+    const int len = max(0, qe - qs), room = max(0, ke - ks), kl = seq ? max(0, min(room, l)) : 0;
     const int off = kl - len, rows = KEYS ? room : len * mul, per = KEYS || mul == 1 ? bm : max(1, bm / mul);
     const Turns t{lane < n && rows > 0 ? (rows - 1) / bm + 1 : 0, KEYS ? (kl > 0 ? len : 0) : kl, off, per, !causal, !KEYS};
     if (!heaviest_first(t, number, (KEYS ? s.total_q : s.total_k) / KB + 1, p.seq, p.block)) return false;

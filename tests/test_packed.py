@@ -813,3 +813,36 @@ def test_arguments_that_are_no_tensors_are_refused():
         with pytest.raises(_lib.AitHipError):
             packed.gated_norm(**{**dict(x=t(5, 8), f=t(5, 8), post_weight=t(8), pre_weight=t(8)), **change})
             pytest.fail("taken: %s" % list(change))
+
+
+def test_loads_in_asm_read_settled_scalars(tmp_path):
+    """The tiles' loads are inline asm, which the compiler does not look into: a scalar that a vector instruction wrote must be five
+    wait states old where they read it.  Read from the built objects, straight back from every such load."""
+    import os
+    import re
+    import subprocess
+    from ait_amd import build
+    llvm, seen = "/opt/rocm/lib/llvm/bin/", 0
+    build.build()
+    for name in ("packed_attn", "packed_attn_bwd"):
+        fat, co = str(tmp_path / "fat.bin"), str(tmp_path / "dev.co")
+        subprocess.check_call([llvm + "llvm-objcopy", "--dump-section", ".hip_fatbin=" + fat, os.path.join(build.OBJ, name + ".o"), str(tmp_path / "copy.o")])
+        subprocess.check_call([llvm + "clang-offload-bundler", "--type=o", "--unbundle", "--input=" + fat,
+                               "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", "--output=" + co])
+        text = subprocess.run([llvm + "llvm-objdump", "-d", "--no-show-raw-insn", co], stdout=subprocess.PIPE, text=True, check=True).stdout
+        lines = [l.split("//")[0].strip() for l in text.splitlines() if l.startswith("\t")]
+        for i, line in enumerate(lines):
+            m = re.match(r"buffer_load_dword(?:x4)? \S+ s\[(\d+):(\d+)\],.* lds", line)
+            if not m:
+                continue
+            seen += 1
+            read, waited, j = set(range(int(m[1]), int(m[2]) + 1)), 0, i - 1
+            while j >= 0 and waited < 5:
+                w = re.match(r"v_\S+ (?:s\[(\d+):(\d+)\]|s(\d+))", lines[j])
+                if w:
+                    wrote = {int(w[3])} if w[3] else set(range(int(w[1]), int(w[2]) + 1))
+                    assert not wrote & read, "%s: `%s` %d wait states before `%s`" % (name, lines[j], waited, line)
+                n = re.match(r"s_nop (\d+)", lines[j])
+                waited += int(n[1]) + 1 if n else 1
+                j -= 1
+    assert seen > 500
