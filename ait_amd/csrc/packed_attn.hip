@@ -10,11 +10,11 @@
 // heads that share its keys.
 //
 // What bounds it.  Long sequences: the matrix unit and the exponentials beside it, at the clock the chip holds under them: 7
-// causal prompts of 33 to 4096 tokens, 16 heads on 4 of 128, bf16: 175 GFLOP in 220 us, 800 TFLOP/s (a large bf16 product
+// causal prompts of 33 to 4096 tokens, 16 heads on 4 of 128, bf16: 175 GFLOP in 217 us, 805 TFLOP/s (a large bf16 product
 // reaches 1244 here); the loads alone taken out of it 214, the exponentials alone 219, so neither is in the way.  Matrix unit
 // 42 % busy at 1.7 GHz, no bank conflicts.  (Tried: eight waves a workgroup 247 against 227, two 322 against 231, the next
 // tile's scores under this one's exponentials 255 against 227.)  New tokens: memory: 16 caches of 5000 to 8191, 32 heads on 8 of
-// 128: 432 MB in 84.5 us, 5.1 TB/s, and 4.8 us to join the parts.
+// 128: 432 MB in 82.4 us, 5.2 TB/s, and 4.8 us to join the parts.
 #include "packed_attn_impl.h"
 
 namespace {
@@ -50,7 +50,7 @@ __device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, in
 // REST (bf16 forwards that a backward follows): the probabilities enter the second product as two operands, their bf16 value and
 // what that rounding took, so that delta belongs to the probabilities and not to their rounding: the bias's gradient, a sum over
 // all pairs in which P dP and P delta cancel, is off by 0.0013 to 0.0017 instead of 0.0019 to 0.0023, dQ by 0.0024 instead of up
-// to 0.0026.  It costs a half more products of this pass (long documents 165 -> 212 us of 950 in all); an inference call, which
+// to 0.0026.  It costs a half more products of this pass (long documents 165 -> 215 us of 850 in all); an inference call, which
 // nothing is subtracted from, rounds them once.
 template <typename T, int D, int NW, bool BIAS, bool SPLIT, bool REST>
 __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a) {

@@ -11,9 +11,9 @@
 // accumulators in one, a wave a SIMD is left or registers spill (734 us against 497).
 //
 // What bounds it: the matrix unit, the exponentials between its products and the clock the chip holds under both.  3 documents of
-// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 240 us over the query rows, 418 over the keys and 20 to join their two parts;
+// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 225 us over the query rows, 390 over the keys and 20 to join their two parts;
 // 4 of 4096 without a mask: 1010 and 980 TFLOP/s executed, no bank conflicts, matrix unit 60 % busy at 1.7 GHz.  12 documents of
-// 100 to 1800, 8 heads of 64: 65 and 62 us.  (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and
+// 100 to 1800, 8 heads of 64: 49 and 63 us (65 over the query rows with operand loads in branches, each waited for by itself).  (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and
 // unmasked blocks as two loops: spills, 1694 us; waves that skip the blocks hidden from them: 81 us instead of 86 for sequences
 // of 1 to 49, 62.6 instead of 60.5 elsewhere; dK's and dV's workgroups in turn instead of dK's first: 459 us against 424.)
 #include "packed_attn_impl.h"
