@@ -117,8 +117,8 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
   }
   if constexpr (BIAS) {
     const int md = a.bias.max_distance, first = block * BM / a.pack, last = (min(block * BM + BM, rows) - 1) / a.pack;
-    far_lo = bias_log2(a.bias, (size_t)bucket(a.bias, -md) * a.H + head);
-    far_hi = bias_log2(a.bias, (size_t)bucket(a.bias, md) * a.H + head);
+    const int lowest = bucket(a.bias, -md), highest = bucket(a.bias, md);
+    bias_log2(a.bias, (size_t)lowest * a.H + head, (size_t)highest * a.H + head, far_lo, far_hi);
     if (t1 * KB - 1 - (first + off) > -md && t0 * KB - (last + off) < md) {      // (else every key is in the outermost buckets)
       fill_bias<NT>(a.bias, a.H, head0, a.pack, const_cast<float*>(bl), tid);
       __syncthreads();

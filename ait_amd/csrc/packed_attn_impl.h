@@ -432,17 +432,37 @@ __device__ __forceinline__ int bucket(const Bias& b, int rel) {
   return v < 0 ? 0 : v >= b.n_buckets ? b.n_buckets - 1 : v;
 }
 // in units of the exponent to base 2.  The lowest finite values stay finite: a row that sees nothing else still has its softmax
-__device__ __forceinline__ float bias_log2(const Bias& b, size_t at) {
-  const float t = b.bf16 ? (float)static_cast<const __bf16*>(b.table)[at] : static_cast<const float*>(b.table)[at], v = t * kLog2e;
+__device__ __forceinline__ float to_log2(float t) {
+  const float v = t * kLog2e;
   return (v == kNegInf && t != kNegInf) ? -3.402823466e38f : v;
+}
+// two values at once (a trip to memory each, if one waited for the other)
+__device__ __forceinline__ void bias_log2(const Bias& b, size_t at0, size_t at1, float& v0, float& v1) {
+  float t0, t1;
+  if (b.bf16) {
+    const __bf16 *p = static_cast<const __bf16*>(b.table), u0 = p[at0], u1 = p[at1];
+    t0 = (float)u0;
+    t1 = (float)u1;
+  } else {
+    t0 = static_cast<const float*>(b.table)[at0];
+    t1 = static_cast<const float*>(b.table)[at1];
+  }
+  v0 = to_log2(t0);
+  v1 = to_log2(t1);
 }
 
 template <int NT>
 __device__ __forceinline__ void fill_bias(const Bias& b, int H, int head0, int heads, float* lds, int tid) {
   const int w = bias_row(b.max_distance);
-  for (int x = tid; x < w; x += NT) {
-    const size_t at = (size_t)bucket(b, x - b.max_distance - kPad) * H + head0;
-    for (int g = 0; g < heads; g++) lds[g * w + x] = bias_log2(b, at + g);
+  for (int x = tid; x < w; x += 2 * NT) {
+    const int y = min(x + NT, w - 1);      // (the last value may be written twice)
+    const int bx = bucket(b, x - b.max_distance - kPad), by = bucket(b, y - b.max_distance - kPad);
+    for (int g = 0; g < heads; g++) {
+      float u, v;
+      bias_log2(b, (size_t)bx * H + head0 + g, (size_t)by * H + head0 + g, u, v);
+      lds[g * w + x] = u;
+      lds[g * w + y] = v;
+    }
   }
 }
 
