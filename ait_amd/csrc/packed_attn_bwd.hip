@@ -13,9 +13,11 @@
 // What bounds it: the matrix unit, the exponentials between its products and the clock the chip holds under both.  3 documents of
 // 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 225 us over the query rows, 390 over the keys and 20 to join their two parts;
 // 4 of 4096 without a mask: 1010 and 980 TFLOP/s executed, no bank conflicts, matrix unit 60 % busy at 1.7 GHz.  12 documents of
-// 100 to 1800, 8 heads of 64: 49 and 63 us (65 over the query rows with operand loads in branches, each waited for by itself).  (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and
-// unmasked blocks as two loops: spills, 1694 us; waves that skip the blocks hidden from them: 81 us instead of 86 for sequences
-// of 1 to 49, 62.6 instead of 60.5 elsewhere; dK's and dV's workgroups in turn instead of dK's first: 459 us against 424.)
+// 100 to 1800, 8 heads of 64: 49 and 63 us (65 over the query rows with operand loads in branches, each waited for by itself).
+// Short sequences (300 of 1 to 49 in f32 with a bias: 61 and 86 us): the trips to memory in front of a workgroup's one tile.
+// (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and unmasked blocks as two loops: spills, 1694 us;
+// bf16 waves that skip the blocks hidden from them, as 64-wide f32 ones do: 62.6 against 60.5; dK's and dV's workgroups in turn
+// instead of dK's first: 459 us against 424.)
 #include "packed_attn_impl.h"
 
 namespace {
@@ -415,6 +417,8 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     loads_done_barrier();
     if (it + 1 < total) fetch(stage ^ 1);
     if (++t == t0 + tq) { t = t0; g++; }
+    // a block that is hidden from this wave (f32: 8192 cycles of the matrix unit; 300 sequences of 1 to 49: 86 us, 89 without)
+    if (D == 64 && sizeof(T) == 4 && (key0 >= klen || r0 + 32 * xh >= qlen || (a.causal && r0 + 32 * xh + 31 < key0 - off))) continue;
     const unsigned char* qt = lds + stage * 2 * kTile;
     const unsigned char* gt = qt + kTile;
     const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * 512);
