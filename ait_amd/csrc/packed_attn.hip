@@ -193,6 +193,14 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[b][r] *= alpha;
     }
+    if (__any(rounded(m))) {
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[x][r] = __builtin_fmaf(s[x][r], f, add);
+      f = 1.f;
+      add = 0.f;
+    }
     const float sub = add - (m == kNegInf ? 0.f : m);
 #pragma unroll
     for (int x = 0; x < 2; x++)

@@ -1,6 +1,7 @@
 // ait_amd/csrc/packed_attn_bwd.hip -- ait_packed_attn_bwd (layout of the products: packed_attn_impl.h).
 //
 //   P_ij = exp(s_ij - lse_i),  dP_ij = dO_i . v_j,  dS_ij = P_ij (dP_ij - delta_i),  delta_i = dO_i . O_i
+//   (rows whose lse is large: P_ij = w_i exp(s_ij - lse_i), w_i = 1 / sum_j exp(s_ij - lse_i), formed by the first pass)
 //   dQ_i = scale sum_j dS_ij k_j,   dK_j = scale sum_i dS_ij q_i,   dV_j = sum_i P_ij dO_i,   d table[bucket] = sum dS_ij
 //
 // Two passes that each own what they write, so no sum goes through atomics on memory and results repeat bit for bit: the first
@@ -30,6 +31,7 @@ constexpr int NW = 4, NT = NW * 64;      // waves of the pass over keys
 // ten times as much: 207 us against 60 for the pass over sequences of 17 to 1024 tokens with a distance of 128.)  Where the
 // tiles leave no room for it (f32 rows of 128 values) the atomics on kHist sums remain.
 constexpr int kHist = 64, kSkew = 32 * 64;
+constexpr int kRows = 3 * KB * 4;        // bytes of a stage's rows: lse, delta, weight
 template <typename T, int D> constexpr bool kSkewed = D == 64 || sizeof(T) == 2;
 template <typename T, int D> constexpr int kSums = kSkewed<T, D> ? kSkew : kHist;      // floats of a wave
 
@@ -50,6 +52,8 @@ struct BwdArgs {
   int H, Hk, d, causal, qnumbers, knumbers, splits, stages, kparts;
   float scale;
   float* delta;       // [H][total_q]
+  long long plane;    // floats from delta to the weights [H][total_q]: 1 / a row's sum of 2^(score - lse) where lse is large
+                      // (`rounded`), else 0, which stands for 1
   float* part_dq;     // [splits][total_q * H][d], not yet scaled: only where splits > 1
   float* part_kv;     // [kparts][dK, dV][total_k][Hk][d], dK not yet scaled: only where kparts > 1
   float* part_table;  // [splits * qnumbers][H][n_buckets]; null: the table's gradient is not wanted
@@ -88,6 +92,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
   const int gend = a.causal ? min(klen, min(block * BM + BM, qlen) + off) : klen;
   const int tiles = gend > 0 ? (gend + KB - 1) / KB : 0, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = blockIdx.y * per, t1 = min(tiles, t0 + per);
+  const float sc = a.scale * kLog2e;
 
   const unsigned kstr = (unsigned)(a.ks * sizeof(T)), vstr = (unsigned)(a.vs * sizeof(T)), dby = a.d * sizeof(T);
   Loader<T, D, NT> lk, lv;
@@ -104,7 +109,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
   if (t0 < t1) fetch(t0, 0);
 
   Frag<T> qf[NCH], gf[NCH];
-  float delta = 0.f, l2;
+  float delta = 0.f, l2, weight = 0.f;
+  bool large;      // a row of this wave's has scores so large that its logarithm does not hold its sum
   {
     const long long at = qstart + pos;
     const T* qr = reinterpret_cast<const T*>(a.q) + at * a.qs + (long long)head * a.qh;
@@ -136,8 +142,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
     }
     delta = column_sum(delta);
     if (row < qlen && h == 0 && blockIdx.y == 0) a.delta[(long long)head * a.s.total_q + at] = delta;
-    // (a query that sees one key has no gradient of its scores: exactly zero, not the rounding of dP - delta)
-    if (row >= qlen || kmax <= 1) l2 = -kNegInf;
+    large = __any(row < qlen && rounded(l2));
   }
   float* bl = reinterpret_cast<float*>(lds + 2 * a.stages * kTile);      // the head's bias, then per wave: a block's sums by
   float* hist = bl + (BIAS ? bias_row(md) : 0) + wave * (kSums<T, D> + nb);      // relative position, and the sums by bucket
@@ -152,9 +157,37 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
     far_lo = bl[0];
     far_hi = bl[2 * (md + kPad)];
   }
+  if (large) {
+    // lse = maximum + log2(sum) is one f32, which beyond 2^24 holds nothing of the sum and beyond 2^12 half its digits: the sum over
+    // all of the row's keys is formed again, of 2^(score - lse).  (By each wave from memory, without the tiles: hardly a row needs
+    // it; where none does, this path costs the passes 0 to 3 %, 64-wide f32 heads over the keys 6.)
+    float sum = 0.f;
+    for (int k0 = 0; k0 < wend; k0 += 32) {
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = 0.f;
+      const bool there = k0 + (lane & 31) < klen;
+      const T* kr = kb + (there ? k0 + (lane & 31) : 0) * a.ks;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) s = mma(global_frag<T>(kr, 16 * c + 8 * h, a.d, there), qf[c], s);
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int j = k0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        const float b = BIAS ? bl[min(max(j - pos - off, -md), md) + md + kPad] : 0.f;
+        const float e = fast_exp2(__builtin_fmaf(s[r], sc, b) - l2);
+        sum += j < kmax ? e : 0.f;
+      }
+    }
+    sum = column_sum(sum);
+    if (row < qlen && rounded(l2) && sum > 0.f) weight = 1.f / sum;
+  }
+  if (row < qlen && h == 0 && blockIdx.y == 0) a.delta[a.plane + (long long)head * a.s.total_q + qstart + pos] = weight;
+  if (weight == 0.f) weight = 1.f;
+  delta *= weight;
+  // (a query that sees one key has no gradient of its scores: exactly zero, not the rounding of dP - delta)
+  if (row >= qlen || kmax <= 1) l2 = -kNegInf;
 
   const int rb = row_base<T, D>(lane), cb = col_base<T, D>(lane);
-  const float sc = a.scale * kLog2e;
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; b++)
@@ -186,17 +219,23 @@ __global__ __launch_bounds__(NW * 64, D == 64 || sizeof(T) == 2 ? 2 : 1) void pa
       }
       read_ahead<T, 2 * NCH, 1, 4>();
       const FirstCols<T, D> first(kt, cb, x);
-      if (BIAS && near) {
-        const float* p = bl + (k0 + 32 * x + 4 * h - (pos + off) + md + kPad);
+      if (BIAS && (near || large)) {      // (scores rounded as the forward has them; a far block's bias from the outermost values)
+        const float* p = bl + (near ? k0 + 32 * x + 4 * h - (pos + off) + md + kPad : right ? bias_row(md) - 32 : 0);
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], sc, p[8 * (r >> 2) + (r & 3)] - l2);
+        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], sc, p[8 * (r >> 2) + (r & 3)]) - l2;
       } else {
-        const float f = (BIAS ? (right ? far_hi : far_lo) : 0.f) - l2;
+        float f = sc;
+        if (!BIAS && large) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], sc, f);
+          for (int r = 0; r < 16; r++) s[r] *= sc;
+          f = 1.f;
+        }
+        const float sub = (BIAS ? (right ? far_hi : far_lo) : 0.f) - l2;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], f, sub);
       }
 #pragma unroll
-      for (int r = 0; r < 16; r++) s[r] = fast_exp2(s[r]) * (dp[r] - delta);
+      for (int r = 0; r < 16; r++) s[r] = fast_exp2(s[r]) * __builtin_fmaf(dp[r], weight, -delta);
       if (k0 + KB > wsure) {
         const int lim = kmax - k0 - 32 * x - 4 * h;
 #pragma unroll
@@ -346,7 +385,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   Loader<T, D, NT> lq, lg;
   lq.init(tid, qstr, dby);
   lg.init(tid, gstr, dby);
-  const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse | delta of KB rows
+  const unsigned lds0 = lds_addr(lds), rows0 = lds0 + 4 * kTile;      // behind the tiles: two stages of lse | delta | weight of KB rows
   // the next tile to load: its head, number, rows and rows left (pointers run on: a head's tiles lie one behind another)
   const T *pq = nullptr, *pg = nullptr;
   const float* ps = nullptr;
@@ -355,16 +394,16 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     const long long r = qstart + (long long)nt * KB;
     pq = reinterpret_cast<const T*>(a.q) + r * a.qs + (long long)nhead * a.qh;
     pg = reinterpret_cast<const T*>(a.d_o) + r * a.dos + (long long)nhead * a.doh;
-    ps = (wave ? a.delta : a.lse) + (long long)nhead * a.s.total_q + r;
+    ps = (wave ? a.delta + (wave == 2 ? a.plane : 0) : a.lse) + (long long)nhead * a.s.total_q + r;
     left = qlen - nt * KB;
   };
   auto fetch = [&](int stage) {
     lq.load(pq, left, qstr, dby, lds0 + stage * 2 * kTile, wave);
     lg.load(pg, left, gstr, dby, lds0 + stage * 2 * kTile + kTile, wave);
-    if (wave < 2) {
+    if (wave < 3) {
       const i32x4 rsrc = tile_rsrc(ps, min(KB, left) * 4);
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
-                   : : "v"(lane * 4), "s"(rsrc), "s"(rows0 + stage * 512 + wave * 256) : "m0", "memory");
+                   : : "v"(lane * 4), "s"(rsrc), "s"(rows0 + stage * kRows + wave * 256) : "m0", "memory");
     }
     pq += KB * a.qs;
     pg += KB * a.dos;
@@ -376,7 +415,7 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       to_head();
     }
   };
-  const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile + 1024);
+  const float* bl = reinterpret_cast<const float*>(lds + 4 * kTile + 2 * kRows);
   if (total > 0) {
     to_head();
     fetch(0);
@@ -421,7 +460,8 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
     if (D == 64 && sizeof(T) == 4 && (key0 >= klen || r0 + 32 * xh >= qlen || (a.causal && r0 + 32 * xh + 31 < key0 - off))) continue;
     const unsigned char* qt = lds + stage * 2 * kTile;
     const unsigned char* gt = qt + kTile;
-    const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * 512);
+    const float* rows = reinterpret_cast<const float*>(lds + 4 * kTile + stage * kRows);
+    const float weights = rows[128 + lane];
     const int last = min(r0 + KB, qlen) - 1;
     bool near = false, right = false;
     if constexpr (BIAS) {
@@ -443,13 +483,23 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       const FirstCols<T, D> first(DV ? gt : qt, cb, x);
       const float far = BIAS ? (right ? far_hi : far_lo) : 0.f;
       const float* p = bl + (key - (r0 + 32 * x + 4 * h + off) + md + kPad);
+      // (rows of large scores: see the pass over query rows.  With a bias every score is rounded, at the same number of operations)
+      const bool large = __any(weights != 0.f);
+      float f = sc;
+      if (!BIAS && large) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] *= sc;
+        f = 1.f;
+      }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const f32x4 l2 = *reinterpret_cast<const f32x4*>(rows + 32 * x + 8 * i + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float sub = !BIAS ? -l2[j] : (near ? p[-8 * i - j] : far) - l2[j];
-          s[4 * i + j] = fast_exp2(__builtin_fmaf(s[4 * i + j], sc, sub));
+          float e;
+          if constexpr (BIAS) e = __builtin_fmaf(s[4 * i + j], sc, near ? p[-8 * i - j] : far) - l2[j];
+          else e = __builtin_fmaf(s[4 * i + j], f, -l2[j]);
+          s[4 * i + j] = fast_exp2(e);
         }
       }
       if constexpr (DK) {
@@ -462,8 +512,16 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
       }
       // a row's first positions do not see the wave's last keys; rows behind the sequence and keys behind k_len are zeros in Q,
       // dO, K and V, but their "probabilities" are not; a query that sees one key has no gradient of its scores
-      if (r0 < wsure || r0 + KB > qlen || key0 + 32 > klen) {
+      if (large || r0 < wsure || r0 + KB > qlen || key0 + 32 > klen) {
         const int from = a.causal ? key - off : 0, one = klen <= 1 ? qlen : a.causal ? -off : -1;
+        if (large) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(rows + 128 + 32 * x + 8 * i + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[4 * i + j] *= w[j] == 0.f ? 1.f : w[j];
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int y = r0 + 32 * x + 8 * (r >> 2) + 4 * h + (r & 3);
@@ -622,7 +680,7 @@ Shape shape_of(const ait_packed_attn& p) {
 
 template <typename T, int D, bool BIAS, int XH>
 int launch_kv(BwdArgs a, hipStream_t st) {
-  const int bytes = 4 * Tile<T, D>::kBytes + 1024 + (BIAS ? bias_row(a.bias.max_distance) * 4 : 0);
+  const int bytes = 4 * Tile<T, D>::kBytes + 2 * kRows + (BIAS ? bias_row(a.bias.max_distance) * 4 : 0);
   constexpr bool kSplit = D == 128 && sizeof(T) == 2;
   const long long numbers = block_numbers(a.s.total_k, 1, NW / XH * 32, a.s.n_seq, a.s.rest), wgs = numbers * a.Hk * a.kparts * (kSplit ? 2 : 1);
   const long long vecs = (long long)a.s.total_k * a.Hk * (a.d / 4);
@@ -669,8 +727,8 @@ int launch_t(const BwdArgs& a, const Shape& sh, hipStream_t st) {
   return a.d <= 64 ? launch_d<T, 64>(a, sh, st) : launch_d<T, 128>(a, sh, st);
 }
 long long q_numbers(const ait_packed_attn& p, const Shape& s) { return block_numbers(p.total_q, 1, s.nw * 32, p.n_seq, p.zero_rest ? 1 : 0); }
-// floats: delta, the parts of dQ, those of dK and dV, those of the table's gradient
-size_t delta_floats(const ait_packed_attn& p) { return ((size_t)p.heads * p.total_q + 3) / 4 * 4; }
+// floats: delta and weight, the parts of dQ, those of dK and dV, those of the table's gradient
+size_t rows_floats(const ait_packed_attn& p) { return ((size_t)p.heads * p.total_q + 3) / 4 * 4; }
 size_t dq_floats(const ait_packed_attn& p, const Shape& s) { return s.splits > 1 ? (size_t)s.splits * p.total_q * p.heads * p.d : 0; }
 size_t kv_floats(const ait_packed_attn& p, const Shape& s) { return s.kparts > 1 ? (size_t)s.kparts * 2 * p.total_k * p.kv_heads * p.d : 0; }
 }  // namespace
@@ -678,7 +736,7 @@ size_t kv_floats(const ait_packed_attn& p, const Shape& s) { return s.kparts > 1
 AIT_API size_t ait_packed_attn_bwd_workspace_bytes(const ait_packed_attn* p) {
   if (ait_packed::check(p) != AIT_OK) return 0;
   const Shape s = shape_of(*p);
-  size_t n = delta_floats(*p) + dq_floats(*p, s) + kv_floats(*p, s);
+  size_t n = 2 * rows_floats(*p) + dq_floats(*p, s) + kv_floats(*p, s);
   if (p->bias_table) n += (size_t)s.splits * q_numbers(*p, s) * p->heads * p->n_buckets;
   return n * sizeof(float);
 }
@@ -710,7 +768,7 @@ AIT_API int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long lo
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, (int)q_numbers(*p, sh), 0, sh.splits, sh.stages, sh.kparts, p->scale,
-            static_cast<float*>(workspace), static_cast<float*>(workspace) + delta_floats(*p), nullptr, nullptr, d_table};
+            static_cast<float*>(workspace), (long long)rows_floats(*p), static_cast<float*>(workspace) + 2 * rows_floats(*p), nullptr, nullptr, d_table};
   a.part_kv = a.part_dq + dq_floats(*p, sh);
   if (p->bias_table && d_table) a.part_table = a.part_kv + kv_floats(*p, sh);
   const hipStream_t st = ait_stream(stream);

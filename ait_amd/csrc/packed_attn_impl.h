@@ -26,7 +26,13 @@ typedef __attribute__((address_space(3))) unsigned char lds_u8;
 
 constexpr int KB = 64;              // keys (or, in the gradient of keys and values, queries) of a tile in shared memory
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kNegInf = -__builtin_inff();
+constexpr float kNegInf = -__builtin_inff(), kMaxFinite = 3.402823466e38f;
+// A score scale q.k + bias is an f32 value.  Up to kRounded in size (in units of log2, where a step of f32 is 2^-16) products,
+// bias and what is subtracted from them go through one multiply-add, which keeps more than that.  Beyond it the score is rounded
+// first, everywhere alike, so that a row whose every score is far from zero (a mask's value in the bias, or products of that
+// size) has one softmax, whichever block a key lies in, and the same one in the backward.
+constexpr float kRounded = 256.f;
+__device__ __forceinline__ bool rounded(float t) { return fabsf(t) > kRounded && fabsf(t) <= kMaxFinite; }
 
 template <typename T> struct FragOf;
 template <> struct FragOf<__bf16> { using type = bf16x8; };
@@ -431,10 +437,11 @@ __device__ __forceinline__ int bucket(const Bias& b, int rel) {
   const int m = b.max_distance, i = (rel < -m ? -m : rel > m ? m : rel) + m, v = b.bucket_of[i];
   return v < 0 ? 0 : v >= b.n_buckets ? b.n_buckets - 1 : v;
 }
-// in units of the exponent to base 2.  The lowest finite values stay finite: a row that sees nothing else still has its softmax
+// in units of the exponent to base 2.  Finite values stay finite (those beyond 2.358e38 count as that): a row that sees only a
+// mask's lowest value still has its softmax
 __device__ __forceinline__ float to_log2(float t) {
   const float v = t * kLog2e;
-  return (v == kNegInf && t != kNegInf) ? -3.402823466e38f : v;
+  return fabsf(t) <= kMaxFinite ? fminf(fmaxf(v, -kMaxFinite), kMaxFinite) : v;
 }
 // two values at once (a trip to memory each, if one waited for the other)
 __device__ __forceinline__ void bias_log2(const Bias& b, size_t at0, size_t at1, float& v0, float& v1) {

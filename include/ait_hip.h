@@ -874,6 +874,9 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *   o_i  = sum_j softmax_j(s_ij) v_j        over the keys j that query i sees: all of its sequence, or with `causal`
  *                                           those with j - i <= len_k - len_q (the last query sees every key)
  *
+ * A score is an f32 value: where it is large in size (a mask's value in the bias: -1e9, the type's lowest) it is rounded as such,
+ * and keys whose scores round to the same value share a row's probability evenly, in forward and backward alike.  Finite biases
+ * beyond 2.358e38 in size count as that.
  * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and takes part in no gradient.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
  * multiplied, whatever it holds; a key INSIDE the sequence that a causal mask hides from a query must be finite (its value is
  * multiplied by a probability of zero).

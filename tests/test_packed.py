@@ -846,3 +846,138 @@ def test_loads_in_asm_read_settled_scalars(tmp_path):
                 waited += int(n[1]) + 1 if n else 1
                 j -= 1
     assert seen > 500
+
+
+# ------------------------------------------------------------------------------------------
+# scores so large that a row's logarithm of its sum no longer holds the sum
+# ------------------------------------------------------------------------------------------
+def absorbed_ref(q, k, v, ql, qs, kl, ks, causal, scale, table, bucket_of, do):
+    """attn_ref for tables whose values are below 16 in size, -inf or below -1e8: a score is an f32 value, and next to a bias of -1e9
+    its step is 64 or more, so that with products under 16 (asserted) the score IS the bias, whatever the product: such keys share
+    a row's probability evenly where it sees no others, and have none where it does.  Bounds as in attn_ref, with no error of
+    such a score."""
+    u, f = torch.finfo(q.dtype).eps / 2, 2.0 ** -24
+    table_type = table.dtype
+    q, k, v, do, table = (t.detach().cpu().to(F8) for t in (q, k, v, do, table))
+    bucket_of = bucket_of.cpu().long()
+    H, Hk, d, m = q.shape[1], k.shape[1], q.shape[2], bucket_of.numel() // 2
+    out = {n: [torch.zeros_like(t), torch.zeros_like(t)] for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v), ("dt", table))}
+    for a, qa, b, kb in zip(ql, qs, kl, ks):
+        if a <= 0 or b <= 0:
+            continue
+        rel = torch.arange(b)[None, :] - torch.arange(a)[:, None] - (b - a)
+        at = bucket_of[rel.clamp(-m, m) + m]
+        for h in range(H):
+            c = h * Hk // H
+            Q, K, V, G = q[qa:qa + a, h], k[kb:kb + b, c], v[kb:kb + b, c], do[qa:qa + a, h]
+            t = table[:, h][at]
+            assert bool(((t.abs() < 16) | (t < -1e8)).all()) and float((scale * Q.abs() @ K.abs().t()).max()) < 16
+            down = t < -1e8
+            s = torch.where(down, t, scale * Q @ K.t() + t)
+            es = torch.where(down, 0.0, (d + 8) * f * (abs(scale) * Q.abs() @ K.abs().t()) + 12 * f * (s.abs() + t.abs()))
+            s = s.masked_fill(rel > 0, -math.inf) if causal else s
+            none = s.amax(1, keepdim=True) == -math.inf
+            es = torch.where(torch.isfinite(s), es, 0.0)
+            p = torch.softmax(torch.where(none, 0.0, s), 1) * ~none
+            rp = es + es.amax(1, keepdim=True) + (2 * b + 16) * f
+            O, dp = p @ V, G @ V.t()
+            EO = (p * (rp + u)) @ V.abs() + (b + 8) * f * (p @ V.abs())
+            delta = (G * O).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            eds = p * ((d + 4) * f * (G.abs() @ V.abs().t()) + (G.abs() * EO).sum(1, keepdim=True) + (d + 4) * f * (G.abs() * O.abs()).sum(1, keepdim=True))
+            eds = eds + ds.abs() * (rp + 4 * f) + p * rp * (G.abs() * EO).sum(1, keepdim=True)
+            edr = eds + u * (ds.abs() + eds) + (a * H // Hk + b + 16) * f * ds.abs()
+            for name, i, x, e in (("o", (slice(qa, qa + a), h), O, EO), ("dq", (slice(qa, qa + a), h), scale * ds @ K, abs(scale) * edr @ K.abs()),
+                                  ("dk", (slice(kb, kb + b), c), scale * ds.t() @ Q, abs(scale) * edr.t() @ Q.abs()),
+                                  ("dv", (slice(kb, kb + b), c), p.t() @ G, (p * (rp + u + (a * H // Hk + b + 16) * f)).t() @ G.abs())):
+                out[name][0][i] += x
+                out[name][1][i] += e
+            out["dt"][0][:, h].index_add_(0, at.reshape(-1), ds.reshape(-1))
+            out["dt"][1][:, h].index_add_(0, at.reshape(-1), (eds + (a * b) ** 0.5 * 8 * f * ds.abs()).reshape(-1))
+    out["dt"][1] += 64 * f * out["dt"][0].abs()
+    r = lambda n, x, e: (x, e + (torch.finfo(table_type).eps / 2 if n == "dt" else u) * (x.abs() + e))
+    return {n: r(n, *xe) for n, xe in out.items()}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("low", [-1e9, "lowest"])
+@pytest.mark.parametrize("ql,kl,Hk,d,causal,max_q,max_k", [
+    ([200, 1, 70], None, 2, 64, True, 200, 200), ([150, 30], None, 4, 128, True, 150, 150), ([33, 64, 2], None, 1, 40, False, 64, 64),
+    ([5, 3], [900, 40], 4, 64, True, 5, 900), ([60], [700], 2, 128, False, 60, 700)])
+def test_rows_that_see_only_buckets_far_down(dtype, low, ql, kl, Hk, d, causal, max_q, max_k):
+    """heads whose tables hold a mask's value (and -inf) for all distances, the near ones, the far ones: rows that see nothing else
+    still have their softmax, and the backward the same one as the forward -- in blocks near the diagonal and far from it, and
+    with the key axis in parts"""
+    kl, H = ql if kl is None else kl, 4
+    q, k, v, do = make(ql, kl, H, Hk, d, dtype, 17)
+    q, k = (q * 0.5).requires_grad_(True), (k * 0.5).requires_grad_(True)
+    v.requires_grad_(True)
+    value = torch.finfo(dtype).min if low == "lowest" else low
+    table = torch.randn(10, H, generator=torch.Generator().manual_seed(2)).to(dtype)
+    of = packed.relative_buckets(10, 20, not causal)
+    far, ahead = int(of[0]), int(of[-1])
+    table[:, 0] = value
+    table[:, 1] = value
+    table[far, 1] = 0.5                       # ... but the far ones behind
+    table[[far, ahead], 2] = value            # only the far ones
+    table[:3, 3], table[3:, 3] = -math.inf, value
+    table = table.cuda().requires_grad_(True)
+    cq, ck = starts(ql), starts(kl)
+    o = packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=causal, bias=(table, of.cuda()), scale=0.1, max_q=max_q, max_k=max_k)
+    grads = torch.autograd.grad(o, [q, k, v, table], do)
+    want = absorbed_ref(q, k, v, ql, cq.tolist(), kl, ck.tolist(), causal, 0.1, table, of, do)
+    for n, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *grads)):
+        within(t, want[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("value", [-1e3, -1e4, -1e6, 1e6, "highest"])
+def test_probabilities_of_a_row_add_up_to_one(dtype, value):
+    """whatever the bias that all of a head's keys have: with dO = 1 a sequence's dV adds up to the number of its rows.  A row's
+    probabilities are off from their sum by the f32 roundings of 260 terms (2^-15 covers them), and each dV by its rounding"""
+    lens, H, d = [260, 3], 2, 64
+    q, k, v, do = make(lens, lens, H, H, d, dtype, 19)
+    v.requires_grad_(True)
+    do = torch.ones_like(do)
+    if value == "highest":
+        value = torch.finfo(dtype).max
+    table, of = torch.full((8, H), value, dtype=dtype, device="cuda"), packed.relative_buckets(8, 20, False, "cuda")
+    o = packed.packed_attention(q, k, v, starts(lens).cuda(), causal=True, bias=(table, of))
+    dv, = torch.autograd.grad(o, [v], do)
+    u = torch.finfo(dtype).eps / 2
+    for s, n in zip(starts(lens).tolist(), lens):
+        t = dv[s:s + n].double()
+        # (bf16: a probability is rounded where it enters the product, and so is dV)
+        assert bool(((t.sum(0) - n).abs() <= n * 2.0 ** -15 + (2 * u * n if dtype == torch.bfloat16 else u * n)).all()), float((t.sum(0) / n - 1).abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [24, 36])
+@pytest.mark.parametrize("ql,kl,d", [([70, 5], [130, 64], 64), ([3], [700], 128), ([600], [600], 128)])
+def test_scores_of_any_size(dtype, power, ql, kl, d):
+    """products of 2^power times 0, 1 or 2 (exact: one value of a head is not zero): the keys with the largest share a row evenly"""
+    H, half = 2, 2.0 ** (power // 2)
+    q, k, v, do = make(ql, kl, H, H, d, dtype, 29)
+    g = torch.Generator().manual_seed(7)
+    with torch.no_grad():
+        q.zero_(), k.zero_()
+        q[:, :, 5] = half
+        k[:, :, 5] = half * torch.randint(0, 3, k.shape[:2], generator=g).to(dtype).cuda()
+    cq, ck = starts(ql), starts(kl)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o = packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), scale=1.0, max_q=max(ql), max_k=max(kl))
+    dv, = torch.autograd.grad(o, [v], do)
+    u, f = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    vv, gg, kk = v.detach().cpu().to(F8), do.cpu().to(F8), k.detach().cpu().to(F8)[:, :, 5]
+    for a, qa, b, kb in zip(ql, cq.tolist(), kl, ck.tolist()):
+        for h in range(H):
+            top = kk[kb:kb + b, h] == kk[kb:kb + b, h].max()
+            p = (top / top.sum())[None].expand(a, b).to(F8)
+            V, G = vv[kb:kb + b, h], gg[qa:qa + a, h]
+            e = u + (2 * b + 16) * f
+            within(o[qa:qa + a, h], (p @ V, 1.01 * e * (p @ V.abs()) + u * (p @ V).abs()), "o")
+            within(dv[kb:kb + b, h], (p.t() @ G, 1.01 * (e + a * f) * (p.t() @ G.abs()) + u * (p.t() @ G).abs()), "dv")
