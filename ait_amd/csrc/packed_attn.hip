@@ -248,15 +248,20 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
         if (dd < a.d) store4(p + dd, acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]);
       }
   } else {
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);        // (a row that sees nothing: zeros; NaN stays NaN)
-    if (a.lse && h == 0) a.lse[(long long)head * a.s.total_q + at] = l == 0.f ? -kNegInf : m + __builtin_amdgcn_logf(l);
+    const bool none = l == 0.f;        // a row that sees nothing: zeros, whatever the keys beside it hold
+    const float inv = 1.f / l;
+    if (a.lse && h == 0) a.lse[(long long)head * a.s.total_q + at] = none ? -kNegInf : m + __builtin_amdgcn_logf(l);
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[b][r] = none ? 0.f : acc[b][r] * inv;
     T* p = reinterpret_cast<T*>(a.o) + at * a.os + (long long)head * a.oh;
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int dd = 32 * b + 8 * i + 4 * h;
-        if (dd < a.d) store_o<T>(a, p + dd, at, head, dd, acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv);
+        if (dd < a.d) store_o<T>(a, p + dd, at, head, dd, acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]);
       }
   }
 }
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const FwdArgs a) {
   for (int s0 = 0; s0 < splits; s0 += 64 / LD) {
     const int s = s0 + lane / LD;
     const float ws = __shfl(w, s & 63, 64);
-    if (s < splits && dd < a.d) o += *reinterpret_cast<const f32x4*>(a.part_o + (s * n + id) * a.d + dd) * ws;
+    if (s < splits && dd < a.d && ws != 0.f) o += *reinterpret_cast<const f32x4*>(a.part_o + (s * n + id) * a.d + dd) * ws;
   }
 #pragma unroll
   for (int x = LD; x < 64; x *= 2)

@@ -371,7 +371,9 @@ __device__ __forceinline__ void bwd_kv(const BwdArgs& a, const int index, unsign
   const int kvh = index % a.Hk, group = a.H / a.Hk, part = index / a.Hk % a.kparts, number = index / a.Hk / a.kparts, md = a.bias.max_distance;
   Place place;
   if (!find_place<true>(a.s, 1, BN, number, 0, a.causal, place)) return;
-  const int block = place.block, qstart = place.qstart, qlen = place.qlen, kstart = place.kstart, klen = place.klen, kroom = place.kroom;
+  const int block = place.block, kstart = place.kstart, klen = place.klen, kroom = place.kroom;
+  // (with a causal mask and more queries than keys the first ones see none: they are left out, whatever they and their dO hold)
+  const int blind = a.causal ? max(0, place.qlen - klen) : 0, qstart = place.qstart + blind, qlen = place.qlen - blind;
   const int kc = wave % (NW / XH), xh = wave / (NW / XH), key0 = block * BN + kc * 32, key = key0 + (lane & 31), off = klen - qlen;
   // query rows that see a key j: positions >= j - off with a causal mask
   const int gfirst = a.causal ? max(0, block * BN - off) : 0;

@@ -877,9 +877,10 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  * A score is an f32 value: where it is large in size (a mask's value in the bias: -1e9, the type's lowest) it is rounded as such,
  * and keys whose scores round to the same value share a row's probability evenly, in forward and backward alike.  Finite biases
  * beyond 2.358e38 in size count as that.
- * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and takes part in no gradient.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
- * multiplied, whatever it holds; a key INSIDE the sequence that a causal mask hides from a query must be finite (its value is
- * multiplied by a probability of zero).
+ * A query that sees no key (an empty key side, or causal with more queries than keys) gives zeros and takes part in no gradient,
+ * whatever it and its dO hold.  What lies outside a sequence's keys -- the next sequence, a cache's unwritten tail -- is never
+ * multiplied, whatever it holds.  A key that a causal mask hides from some of its sequence's queries must be finite, and so must
+ * a query and its dO: where the mask hides one from the other they are multiplied by a probability of zero.
  *
  *   q [total_q, heads, d], k / v [total_k, kv_heads, d], o as q: element (row, head, e) at row * _row + head * _head + e, both
  *     pitches and the base multiples of 16 bytes, else AIT_EUNSUPPORTED.  Head h reads key head h / (heads / kv_heads).

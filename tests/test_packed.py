@@ -981,3 +981,32 @@ def test_scores_of_any_size(dtype, power, ql, kl, d):
             e = u + (2 * b + 16) * f
             within(o[qa:qa + a, h], (p @ V, 1.01 * e * (p @ V.abs()) + u * (p @ V).abs()), "o")
             within(dv[kb:kb + b, h], (p.t() @ G, 1.01 * (e + a * f) * (p.t() @ G.abs()) + u * (p.t() @ G).abs()), "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ql,kl,H,Hk,d,bias,max_k", [([70, 5], [2, 0], 4, 2, 64, True, 64), ([300, 90], [150, 70], 2, 1, 128, False, 150), ([1300], [600], 2, 1, 128, False, 600),
+                                                     ([200], [33], 2, 2, 40, True, 33)])
+def test_rows_that_see_no_key_may_hold_anything(dtype, ql, kl, H, Hk, d, bias, max_k):
+    """the padding in front of a sequence with a causal mask: neither its queries nor its gradients enter those of the keys"""
+    q, k, v, do = make(ql, kl, H, Hk, d, dtype, 43)
+    cq, ck = starts(ql), starts(kl)
+    want_q, want_do = q.clone(), do.clone()
+    for a, n, m in zip(cq.tolist(), ql, kl):
+        q[a:a + n - m], do[a:a + n - m] = float("nan"), float("inf")
+        want_q[a:a + n - m], want_do[a:a + n - m] = 0, 0
+    b = None
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    if bias:
+        b = (torch.randn(12, H, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True), packed.relative_buckets(12, 50, False, "cuda"))
+        leaves.append(b[0])
+    o = packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=True, bias=b, max_q=max(ql), max_k=max_k)
+    grads = torch.autograd.grad(o, leaves, do)
+    want = attn_ref(want_q, k, v, ql, cq.tolist(), kl, ck.tolist(), True, d ** -0.5, *(b or (None, None)), do=want_do)
+    for n, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *grads)):
+        within(t, want[n], n)
+    # ... and they are zeros next to a value that is none
+    with torch.no_grad():
+        v[max(0, kl[0] - 1)] = float("nan")
+        o = packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=True, bias=b, max_q=max(ql), max_k=max_k)
+    assert all(bool((o[a:a + n - m] == 0).all()) for a, n, m in zip(cq.tolist(), ql, kl))
