@@ -13,11 +13,15 @@ scratch from torch's allocator per call and may be captured into a graph.
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
 
-def _recorded(*tensors):
+def _recorded(op, *tensors):
+    """whether a gradient of the call is wanted.  A dual tensor of forward mode, whose tangent the kernels would drop, is refused"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _lib.AitHipError(op + ": there is no forward-mode derivative")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -60,9 +64,9 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
     knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis).
 
     A query that sees no key gives zeros; so do rows behind the last sequence, and neither takes part in a gradient.  Gradients
-    of q, k, v and the table, not differentiable again.  In a captured graph the backward belongs to a forward captured with it,
-    while no eager graph of the same leaves is alive (autograd would wait for their streams inside the capture, which ends the
-    process: capture first, or with detached leaves)."""
+    of q, k, v and the table, in reverse mode, not differentiable again.  In a captured graph the backward belongs to a forward
+    captured with it, while no eager graph of the same leaves is alive (autograd would wait for their streams inside the capture,
+    which ends the process: capture first, or with detached leaves)."""
     table = bucket_of = None
     if bias is not None:
         if isinstance(bias, RelativePositionBias):
@@ -72,7 +76,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
         table, bucket_of = bias
     if cu_k is None:
         cu_k = cu_q
-    if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded(q, k, v, table):
+    if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded("packed_attention", q, k, v, table):
         return _PackedAttention.apply(q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of)
     p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)
     return ops.packed_attn_fwd(p, q, k, v)[0]
@@ -164,7 +168,7 @@ def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, 
         if gate is not None and gate.shape != shape:
             raise _lib.AitHipError("gated_norm: a gate without cu_seqlens has x's shape")
         x, f, gate = (None if t is None else t[None] if len(shape) == 1 else t.flatten(0, -2) for t in (x, f, gate))
-    if _recorded(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale):
+    if _recorded("gated_norm", x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale):
         y, h = _GatedNorm.apply(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, scale, cu_seqlens, kind == "layer", eps)
     else:
         p, keep = ops.gated_norm_desc(x, f, _f32(post_weight), _f32(pre_weight), _f32(post_bias), _f32(pre_bias), gate, _f32(scale),

@@ -1010,3 +1010,23 @@ def test_rows_that_see_no_key_may_hold_anything(dtype, ql, kl, H, Hk, d, bias, m
         v[max(0, kl[0] - 1)] = float("nan")
         o = packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=True, bias=b, max_q=max(ql), max_k=max_k)
     assert all(bool((o[a:a + n - m] == 0).all()) for a, n, m in zip(cq.tolist(), ql, kl))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """a dual tensor requires no gradient: taken, its tangent would be lost without a word"""
+    import torch.autograd.forward_ad as fwd_ad
+    t = lambda *s: torch.zeros(*s)
+    cu, table, of = starts([2, 3]), t(8, 4), packed.relative_buckets(8, 20, True)
+    good = dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cu_q=cu, bias=(table, of))
+    norm = dict(x=t(5, 8), f=t(5, 8), post_weight=t(8), pre_weight=t(8), post_bias=t(8), pre_bias=t(8), gate=t(5, 8), scale=t(8))
+    with fwd_ad.dual_level():
+        dual = lambda x: fwd_ad.make_dual(x, torch.ones_like(x))
+        for change in (dict(q=dual(good["q"])), dict(k=dual(good["k"])), dict(v=dual(good["v"])), dict(bias=(dual(table), of))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(_lib.AitHipError, match="forward-mode"):
+                    packed.packed_attention(**{**good, **change})
+        for n in norm:
+            with pytest.raises(_lib.AitHipError, match="forward-mode"):
+                packed.gated_norm(**{**norm, n: dual(norm[n])})
+        with pytest.raises(_lib.AitHipError, match="no CPU fallback"):
+            packed.packed_attention(**good)
