@@ -835,6 +835,10 @@ def packed_attn_desc(q, k, v, cu_q, cu_k, k_len=None, max_q=None, max_k=None, ca
         _refuse(op, "head width %d: a multiple of 8 up to 128 expected", d)
     if max(tq, tk) >= 2 ** 31:
         _refuse(op, "row counts must fit 31 bits")
+    try:
+        scale = d ** -0.5 if scale is None else float(scale)
+    except (TypeError, ValueError, RuntimeError):
+        _refuse(op, "`scale` must be a number")
     if not (torch.is_tensor(cu_q) and cu_q.dim() == 1 and cu_q.numel() > 0):
         _refuse(op, "`cu_q` must be an int32 tensor of n_seq + 1 values")
     n = cu_q.numel() - 1
@@ -860,7 +864,7 @@ def packed_attn_desc(q, k, v, cu_q, cu_k, k_len=None, max_q=None, max_k=None, ca
         p.max_q = min(int(max_q), tq)
     if max_k:
         p.max_k = min(int(max_k), tk)
-    p.dtype, p.causal, p.scale = _lib.DTYPES[q.dtype], 1 if causal else 0, d ** -0.5 if scale is None else float(scale)
+    p.dtype, p.causal, p.scale = _lib.DTYPES[q.dtype], 1 if causal else 0, scale
     keep = (cu_q, cu_k, k_len, table, bucket_of)
     packed_attn_point(p, *keep)
     return p, keep

@@ -59,7 +59,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
     strides, views of a fused projection are read in place where their rows are whole 16-byte vectors and copied where not; d a
     multiple of 8 up to 128).  cu_q, cu_k: int32 starts [n_seq + 1], the first 0, not descending; cu_k None: the keys are packed
     like the queries.  k_len int32 [n_seq]: the sequence's keys are the first k_len of its rows -- a cache whose rows behind them
-    may hold anything.  causal: the last query is level with the last key and a query sees no later key.  scale: d ** -0.5.
+    may hold anything.  causal: the last query is level with the last key and a query sees no later key.  scale: a number, d ** -0.5.
     bias: (table [n_buckets, heads], bucket_of), or a RelativePositionBias.  max_q / max_k: the longest lengths where the host
     knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis).
 
@@ -76,6 +76,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
         table, bucket_of = bias
     if cu_k is None:
         cu_k = cu_q
+    if torch.is_tensor(scale) and scale.requires_grad and torch.is_grad_enabled():
+        raise _lib.AitHipError("packed_attention: `scale` is a number and gets no gradient (multiply q by a learned one)")
     if all(torch.is_tensor(t) for t in (q, k, v)) and _recorded("packed_attention", q, k, v, table):
         return _PackedAttention.apply(q, k, v, table, cu_q, cu_k, k_len, max_q, max_k, causal, scale, bucket_of)
     p, _keep = ops.packed_attn_desc(q, k, v, cu_q, cu_k, k_len, max_q, max_k, causal, scale, table, bucket_of)

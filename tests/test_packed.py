@@ -1030,3 +1030,15 @@ def test_forward_mode_derivatives_are_refused():
                 packed.gated_norm(**{**norm, n: dual(norm[n])})
         with pytest.raises(_lib.AitHipError, match="no CPU fallback"):
             packed.packed_attention(**good)
+
+
+def test_a_scale_with_a_gradient_is_refused():
+    """the scale is a number: as a tensor that wants a gradient it would get none"""
+    t = lambda *s: torch.zeros(*s)
+    good = dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cu_q=starts([2, 3]))
+    for bad in (torch.tensor(0.5, requires_grad=True), torch.ones(3), "large"):
+        with pytest.raises(_lib.AitHipError, match="scale"):
+            packed.packed_attention(**good, scale=bad)
+    for number in (0.5, 1, torch.tensor(0.5)):
+        with pytest.raises(_lib.AitHipError, match="no CPU fallback"):
+            packed.packed_attention(**good, scale=number)
