@@ -30,7 +30,7 @@ struct FwdArgs {
   long long qs, qh, ks, kh, vs, vh, os, oh;      // row and head strides in elements
   Seqs s;
   Bias bias;
-  int H, Hk, d, causal, pack, splits, numbers, stages;
+  int H, Hk, d, causal, pack, splits, numbers, stages, whole;      // whole: unrounded probabilities (REST)
   float scale;
   float* part_o;      // [splits][total_q * H][d] unnormalised, and
   float* part_ml;     // [splits][total_q * H][2] maximum, sum: only where splits > 1
@@ -47,11 +47,13 @@ __device__ __forceinline__ void store_o(const FwdArgs& a, T* p, long long at, in
       store4(reinterpret_cast<T*>(a.rest) + (at * a.H + head) * a.d + dd, v0 - (float)(T)v0, v1 - (float)(T)v1, v2 - (float)(T)v2, v3 - (float)(T)v3);
 }
 
-// REST (bf16 forwards that a backward follows): the probabilities enter the second product as two operands, their bf16 value and
-// what that rounding took, so that delta belongs to the probabilities and not to their rounding: the bias's gradient, a sum over
-// all pairs in which P dP and P delta cancel, is off by 0.0013 to 0.0017 instead of 0.0019 to 0.0023, dQ by 0.0024 instead of up
-// to 0.0026.  It costs a half more products of this pass (long documents 165 -> 215 us of 850 in all); an inference call, which
-// nothing is subtracted from, rounds them once.
+// REST (bf16): the probabilities enter the second product as two operands, their bf16 value and what that rounding took, at the
+// price of a half more products.  Forwards that a backward follows do it, so that delta belongs to the probabilities and not to
+// their rounding: the bias's gradient, a sum over all pairs in which P dP and P delta cancel, is off by 0.0013 to 0.0017 instead
+// of 0.0019 to 0.0023, dQ by 0.0024 instead of up to 0.0026.  So do inference calls with few queries a sequence, which wait for
+// memory: o is then off by its own rounding (0.0017 of its norm) instead of 0.0023, for 82.8 us instead of 81.4 (16 long caches),
+// 7.7 instead of 6.9 (4 short ones), 14.6 instead of 13.5 (300 of up to 49 queries).  Prompts would take 347 us instead of 254
+// (7 of 33 to 4096 tokens), sequences of 17 to 1024 with a bias 31.4 instead of 27.0: they round the probabilities once.
 template <typename T, int D, int NW, bool BIAS, bool SPLIT, bool REST>
 __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a) {
   constexpr int NT = NW * 64, BM = NW * 32, NB = D / 32, NCH = D / 16, kTile = Tile<T, D>::kBytes;
@@ -322,7 +324,7 @@ int launch(const FwdArgs& a, int bias_bytes, hipStream_t st) {
 template <typename T, int D, int NW, bool BIAS, bool SPLIT>
 int launch_rest(const FwdArgs& a, int bias_bytes, hipStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (a.rest) return launch<T, D, NW, BIAS, SPLIT, true>(a, bias_bytes, st);
+    if (a.whole) return launch<T, D, NW, BIAS, SPLIT, true>(a, bias_bytes, st);
   return launch<T, D, NW, BIAS, SPLIT, false>(a, bias_bytes, st);
 }
 template <typename T, int D, int NW>
@@ -340,15 +342,15 @@ int launch_t(const FwdArgs& a, int nw, int bias_bytes, hipStream_t st) {
 }
 
 // what the sizes decide: heads packed to a position, waves of a workgroup, parts of the key axis, tiles in flight
-struct Shape { int pack, nw, splits, stages; };
+struct Shape { int pack, nw, splits, stages; bool few; };
 Shape shape_of(const ait_packed_attn& p) {
   Shape r;
   const int group = p.heads / p.kv_heads;
   const long long max_q = p.max_q > 0 ? p.max_q : p.total_q, max_k = p.max_k > 0 ? p.max_k : p.total_k;
   // a few new tokens: the heads of a key head share a workgroup's columns, and its keys are read once (16 long caches, 4 heads to
   // a key head: 86 us, 185 with a workgroup to a head; with a bias, whose heads each want a row in shared memory, 13.3 and 20.9)
-  const bool few = max_q * group <= 128;
-  r.pack = few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
+  r.few = max_q * group <= 128;
+  r.pack = r.few && (!p.bias_table || (long long)group * bias_row(p.max_distance) * 4 <= 32768) ? group : 1;
   // up to 64 rows in two waves, in four what is longer (sequences of 1 to 49 in f32: 36.3 us against 43.5 in four; prompts: 322 us
   // in two, 231 in four); for single tokens two measure as four and better than one (with bias 11.3, 11.7, 13.3 us)
   r.nw = max_q * r.pack <= 64 ? 2 : 4;
@@ -421,7 +423,7 @@ AIT_API int ait_packed_attn_fwd(const ait_packed_attn* p, const void* q, long lo
             {p->cu_q, p->cu_k, p->k_len, p->n_seq, p->total_q, p->total_k, p->zero_rest ? 1 : 0, sh.splits == 1 && ait_packed::order_blocks(*p)},
             {p->bias_table, p->bucket_of, p->n_buckets, p->max_distance, p->table_dtype == AIT_DTYPE_BF16},
             p->heads, p->kv_heads, p->d, p->causal, sh.pack, sh.splits,
-            (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, p->scale, nullptr, nullptr};
+            (int)ait_packed::block_numbers(p->total_q, sh.pack, sh.nw * 32, p->n_seq, p->zero_rest ? 1 : 0), sh.stages, o_rest || sh.few, p->scale, nullptr, nullptr};
   if (need) {
     a.part_o = static_cast<float*>(workspace_ptr);
     a.part_ml = a.part_o + (size_t)sh.splits * p->total_q * p->heads * p->d;

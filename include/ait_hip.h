@@ -891,7 +891,8 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *   max_q, max_k: the longest lengths as far as the host knows them (0: unknown).  They choose how work is cut up, and nothing
  *     but the order of sums depends on them.
  *   dtype AIT_DTYPE_F32 (exact f32 products) or AIT_DTYPE_BF16 (f32 scores, statistics and sums; probabilities and dS are
- *     rounded to bf16 where they enter a product) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
+ *     rounded to bf16 where they enter a product -- the probabilities of a forward with o_rest, or with at most
+ *     128 / (heads / kv_heads) queries a sequence, are not) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
  *   bias_table [n_buckets, heads] of table_dtype (AIT_DTYPE_*), or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
  *     table): the bucket of relative position key - query, where the last query is level with the last key; further away the
  *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.

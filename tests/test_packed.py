@@ -1042,3 +1042,71 @@ def test_a_scale_with_a_gradient_is_refused():
     for number in (0.5, 1, torch.tensor(0.5)):
         with pytest.raises(_lib.AitHipError, match="no CPU fallback"):
             packed.packed_attention(**good, scale=number)
+
+
+# ------------------------------------------------------------------------------------------
+# how exact bf16 attention is, by norms
+# ------------------------------------------------------------------------------------------
+def _norms64(q, k, v, do, ql, kl, causal, scale, table, of):
+    """in 64 bits: o, dq, dk, dv, d table, and the d table of a backward whose delta comes from a rounded o (`once`), or from one
+    that was formed of rounded probabilities too (`twice`)"""
+    b16 = lambda t: t.to(torch.bfloat16).to(F8)
+    q, k, v, do, table = (t.detach().cpu().to(F8) for t in (q, k, v, do, table))
+    H, Hk, m = q.shape[1], k.shape[1], of.numel() // 2
+    r = dict(o=torch.zeros_like(q), dq=torch.zeros_like(q), dk=torch.zeros_like(k), dv=torch.zeros_like(v))
+    r.update({n: torch.zeros_like(table) for n in ("dt", "once", "twice")})
+    for a, qa, b, kb in zip(ql, starts(ql).tolist(), kl, starts(kl).tolist()):
+        rel = torch.arange(b)[None, :] - torch.arange(a)[:, None] - (b - a)
+        at = of.long()[rel.clamp(-m, m) + m]
+        for h in range(H):
+            c = h * Hk // H
+            Q, K, V, G = q[qa:qa + a, h], k[kb:kb + b, c], v[kb:kb + b, c], do[qa:qa + a, h]
+            s = scale * Q @ K.t() + table[:, h][at]
+            s = s.masked_fill(rel > 0, -math.inf) if causal else s
+            e = torch.exp(s - s.amax(1, keepdim=True))
+            p = e / e.sum(1, keepdim=True)
+            O, dp = p @ V, G @ V.t()
+            r["o"][qa:qa + a, h] = O
+            for name, o in (("dt", O), ("once", b16(O)), ("twice", b16(b16(e) @ V / e.sum(1, keepdim=True)))):
+                ds = p * (dp - (G * o).sum(1, keepdim=True))
+                r[name][:, h].index_add_(0, at.reshape(-1), ds.reshape(-1))
+            ds = p * (dp - (G * O).sum(1, keepdim=True))
+            r["dq"][qa:qa + a, h] = scale * ds @ K
+            r["dk"][kb:kb + b, c] += scale * ds.t() @ Q
+            r["dv"][kb:kb + b, c] += p.t() @ G
+    return r
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl,H,Hk,d,causal,few", [(LONG, None, 4, 1, 64, True, False), ([400], None, 2, 2, 128, False, False), (LONG, None, 4, 2, 40, True, False),
+                                                      ([60], [1500], 2, 2, 128, False, True), ([5, 9], [700, 400], 8, 2, 72, True, True),
+                                                      ([33, 40], None, 2, 1, 64, True, True)])
+def test_how_exact_bf16_attention_is(ql, kl, H, Hk, d, causal, few):
+    """A bf16 value's rounding is off by up to 2^-8 / m of it, m in 1 .. 2 its significand; over spread values that is
+    2^-8 / sqrt(3 E[m^2]) = 0.0015 to 0.0017 of a tensor's norm, and a sum of products with one rounded factor is off by as much.  So
+    what is rounded once is within 0.0019, what is the rounded sum of products with a rounded factor within 1.15 sqrt(2) 0.0017 =
+    0.0027 of its norm.  What rounding took from o is kept for the backward: o and it together leave 2^-8 2^-8 of o and the f32 sums'
+    errors, 2^-14 with room.  The table's gradient (here of an f32 table: no rounding of its own) must be nearer than a quarter
+    of what losing that rest, in o or in the probabilities, would take it away."""
+    kl = ql if kl is None else kl
+    q, k, v, do = (t[:sum(n)] for t, n in zip(make(ql, kl, H, Hk, d, torch.bfloat16, 53), (ql, kl, kl, ql)))
+    table = torch.randn(12, H, generator=torch.Generator().manual_seed(3)).cuda()
+    of = packed.relative_buckets(12, 50, not causal)
+    cq, ck = starts(ql).cuda(), starts(kl).cuda()
+    scale = d ** -0.5
+    want = _norms64(q, k, v, do, ql, kl, causal, scale, table, of)
+    off = lambda t, n, ref=None: float((t.detach().cpu().to(F8) - want[n]).norm() / (want[n] if ref is None else ref).norm())
+    hints = dict(max_q=max(ql), max_k=max(kl))
+    with torch.no_grad():
+        o = packed.packed_attention(q, k, v, cq, ck, causal=causal, bias=(table, of.cuda()), **hints)
+    assert off(o, "o") < (0.0019 if few else 0.0027)
+    p, keep = ops.packed_attn_desc(q, k, v, cq, ck, causal=causal, table=table, bucket_of=of.cuda(), **hints)
+    o, lse, rest = ops.packed_attn_fwd(p, q, k, v, for_backward=True)
+    assert off(o, "o") < 0.0019
+    assert off(o.double() + rest.double(), "o") < 2.0 ** -14
+    dq, dk, dv, dt = ops.packed_attn_bwd(p, q, k, v, o, rest, do, lse, want_table=True)
+    for n, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert off(t, n) < 0.0027, n
+    err = (dt.cpu().to(F8) - want["dt"]).norm()
+    for n in ("once", "twice"):
+        assert float(err) < 0.25 * float((want[n] - want["dt"]).norm()), n
