@@ -1110,3 +1110,27 @@ def test_how_exact_bf16_attention_is(ql, kl, H, Hk, d, causal, few):
     err = (dt.cpu().to(F8) - want["dt"]).norm()
     for n in ("once", "twice"):
         assert float(err) < 0.25 * float((want[n] - want["dt"]).norm()), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("ql,kl,d,bias", [([70, 130], None, 40, False), ([70, 130], None, 64, True), ([70, 130], None, 128, False), ([5, 2], [900, 70], 64, True),
+                                          ([3], [700], 128, False)])
+def test_a_scale_of_any_sign_in_both_types(dtype, scale, ql, kl, d, bias):
+    """with a bias, over the key axis in parts, at widths below the tiles'"""
+    kl = ql if kl is None else kl
+    q, k, v, do = make(ql, kl, 4, 2, d, dtype, 5)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    b = None
+    if bias:
+        b = (torch.randn(8, 4, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True), packed.relative_buckets(8, 30, False, "cuda"))
+        leaves.append(b[0])
+    cq, ck = starts(ql), starts(kl)
+    call = lambda: packed.packed_attention(q, k, v, cq.cuda(), ck.cuda(), causal=True, scale=scale, bias=b, max_q=max(ql), max_k=max(kl))
+    o = call()
+    want = attn_ref(q, k, v, ql, cq.tolist(), kl, ck.tolist(), True, scale, *(b or (None, None)), do=do)
+    for n, t in zip(("o", "dq", "dk", "dv", "dt"), (o, *torch.autograd.grad(o, leaves, do))):
+        within(t, want[n], n)
+    with torch.no_grad():
+        within(call(), want["o"], "o without a gradient")
