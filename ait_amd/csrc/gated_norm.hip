@@ -321,8 +321,10 @@ __global__ __launch_bounds__(Block<G>::kThreads) void gated_norm_bwd_kernel(cons
   const int unit = blockIdx.x * R + group, first = unit * a.per, last = min(first + a.per, a.rows);
   float* gate_parts = a.parts + (size_t)a.blocks * a.n_parts * W;
   // The parameters of a lane's values are held over all rows where a lane has one block of eight: in registers up to eight waves,
-  // in shared memory for more, whose 168 registers a lane would spill.  (The next row's loads issued under this one's arithmetic
-  // gain nothing where registers allow it, 150 us against 149, and spill in ten waves: 280 against 241.)
+  // in shared memory for more, whose 168 registers a lane are too few for both (with biases 12 to 48 bytes a lane spill even so).
+  // Two blocks a lane (rows over 6144, unaligned ones over 4096) read them in place and spill: 12 to 36 bytes a lane without biases,
+  // 164 to 204 with, 208 to 476 unaligned.  (The next row's loads issued under this one's arithmetic gain nothing where registers
+  // allow it, 150 us against 149, and spill in ten waves: 280 against 241.)
   constexpr bool HELD = V == 1 && G <= 8, LDSP = V == 1 && !HELD;
   __shared__ __attribute__((aligned(16))) float wl[LDSP ? (SUMS_B ? 4 : 3) : 1][LDSP ? G * 512 : 4];
   const float* from[4] = {a.w_post, a.w_pre, a.scale, a.b_post};

@@ -184,8 +184,8 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_kernel(const FwdArgs a)
 #pragma unroll
     for (int r = 1; r < 16; r++) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
     top = __builtin_fmaf(column_max(top), f, add);
-    // The maximum is only followed where it rises by more than 2^8: what is summed stays below 2^8 and the same bits are
-    // significant, and nearly every block is spared the rescaling of the accumulators
+    // The maximum is only followed where it rises by more than 2^8 (a published idea: T. Dao, Hot Chips 2025): what is summed
+    // stays below 2^8 and the same bits are significant, and nearly every block is spared the rescaling of the accumulators
     if (__any(top > m + 8.f)) {
       const float mn = fmaxf(m, top), alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
       m = mn;

@@ -325,7 +325,8 @@ __device__ __forceinline__ int lane_scan(int v) {
   return v;
 }
 // The same blocks in another order: those with the most turns first, whatever their sequence, so that a launch does not end on
-// the long ones (7 prompts of 33 to 4096 tokens: 217 us against 227, sequences of 17 to 1024 with a bias 61 against 73 in the pass over query rows).  At most 64 sequences, `rest` among them.
+// the long ones (7 prompts of 33 to 4096 tokens: 217 us against 227, sequences of 17 to 1024 with a bias 61 against 73 in the pass
+// over query rows).  At most 64 sequences, `rest` among them.
 // A block of rows j (of ROWS rows) of a sequence takes turns(j) = ceil(min(all, (j + 1) rows_per + off) / KB) turns if it
 // ascends, ceil((all - max(0, j rows_per - off)) / KB) if not -- the key tiles of a query block, the query tiles of a key block;
 // `flat`: every block takes ceil(all / KB).  The blocks with more than L turns are counted in closed form and L is found by

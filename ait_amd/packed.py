@@ -61,7 +61,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, k_len=None, max_q=None, max_k=
     like the queries.  k_len int32 [n_seq]: the sequence's keys are the first k_len of its rows -- a cache whose rows behind them
     may hold anything.  causal: the last query is level with the last key and a query sees no later key.  scale: a number, d ** -0.5.
     bias: (table [n_buckets, heads], bucket_of), or a RelativePositionBias.  max_q / max_k: the longest lengths where the host
-    knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis).
+    knows them; they guide how the work is cut up (a few new tokens against long caches are spread over the key axis; bfloat16
+    inference rounds its probabilities to bfloat16 only where max_q * heads / kv_heads is over 128).
 
     A query that sees no key gives zeros; so do rows behind the last sequence, and neither takes part in a gradient.  Gradients
     of q, k, v and the table, in reverse mode, not differentiable again.  In a captured graph the backward belongs to a forward
@@ -153,7 +154,7 @@ def gated_norm(x, f, *, post_weight, pre_weight, post_bias=None, pre_bias=None, 
     one of f's shape and type, or with cu_seqlens (int32 [n_seq + 1], the first 0, not descending) one row per sequence of the
     packed rows of a two-dimensional x; rows behind the last sequence then give zeros.  scale: None or [width], the learned
     factor of the branch.  Parameters are float32 or bfloat16 [width]; sums, statistics and the row between the two norms are
-    f32.  width up to 8192."""
+    f32.  width up to 8192; up to 67 million rows of 512, fewer of wider ones (their waves' lanes stay below 2^32)."""
     if kind not in ("rms", "layer"):
         raise ValueError("gated_norm: kind must be 'rms' or 'layer'")
     if not (torch.is_tensor(x) and torch.is_tensor(f) and x.dim() >= 1 and x.shape == f.shape):

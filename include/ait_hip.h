@@ -888,14 +888,16 @@ int ait_sk_sqsum_bwd(const float* dy, const float* a, const float* b, long long 
  *     k_len [n_seq] int32 or NULL: it has k_len[b] keys (at most cu_k[b + 1] - cu_k[b]) from cu_k[b] on -- a cache.  Values
  *     outside the tensors are clamped to them.  Rows of q behind the last sequence are not read; those of o (dq, dk, dv) are
  *     left as they are, or set to zero with zero_rest.
- *   max_q, max_k: the longest lengths as far as the host knows them (0: unknown).  They choose how work is cut up, and nothing
- *     but the order of sums depends on them.
+ *   max_q, max_k: the longest lengths as far as the host knows them (0: unknown, total_q and total_k then).  They choose how work
+ *     is cut up and with it the order of sums, and max_q whether a bf16 forward rounds its probabilities (dtype).
  *   dtype AIT_DTYPE_F32 (exact f32 products) or AIT_DTYPE_BF16 (f32 scores, statistics and sums; probabilities and dS are
- *     rounded to bf16 where they enter a product -- the probabilities of a forward with o_rest, or with at most
- *     128 / (heads / kv_heads) queries a sequence, are not) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
- *   bias_table [n_buckets, heads] of table_dtype (AIT_DTYPE_*), or NULL; bucket_of int32 [2 * max_distance + 1] on the device (entries are clamped to the
- *     table): the bucket of relative position key - query, where the last query is level with the last key; further away the
- *     outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
+ *     rounded to bf16 where they enter a product, except the probabilities of a forward with o_rest or with
+ *     max_q * heads / kv_heads <= 128) of q, k, v, o and their gradients.  d: a multiple of 8 up to 128.
+ *   bias_table [n_buckets, heads] of table_dtype (AIT_DTYPE_*), or NULL; bucket_of int32 [2 * max_distance + 1] on the device
+ *     (entries are clamped to the table): the bucket of relative position key - query, where the last query is level with the
+ *     last key; further away the outermost entry counts.  At most AIT_MAX_BUCKETS buckets, distance AIT_MAX_BIAS_DISTANCE.
+ *   (total_q + n_seq + 1) * heads stays below 2^31, and a launch's work items below 2^32 (a block of 32 query rows and a head is
+ *     64 of them), else AIT_EUNSUPPORTED.
  *   For the backward, else NULL: lse f32 [heads, total_q], the binary logarithm of a row's sum of exp (+infinity where a query
  *     sees no key); o_rest [total_q, heads, d] contiguous, AIT_DTYPE_BF16 only: what rounding took from o, without which the
  *     gradients of q and k carry o's rounding error; with it the forward multiplies unrounded probabilities (bf16 value + rest).
@@ -937,6 +939,7 @@ int ait_packed_attn_bwd(const ait_packed_attn* p, const void* q, long long q_row
  *     m = norm(f) w_post (+ b_post) ;  y = x + scale * gate * m ;  h = norm(y) w_pre (+ b_pre)
  *     layer != 0: norm(t) = (t - mean t) / sqrt(var t + eps), var about the mean; layer == 0: t / sqrt(mean t^2 + eps)
  *   x [rows, width] of dtype_x (pitch x_row elements), f of dtype_f; (AIT_DTYPE_F32, F32), (F32, BF16) and (BF16, BF16).
+ *     rows * 64 * (waves of a row: one up to 512 values, at most 12) stays below 2^32, else AIT_EUNSUPPORTED.
  *     y as x, h as f.  width up to 8192; rows of whole 16-byte vectors (width, pitches, bases) take wide loads, others single ones.
  *   gate NULL, [rows, width] of dtype_f, or with cu_seqlens int32 [n_seq + 1] (ascending from 0) [n_seq, width]: row r's is that
  *     of its sequence; what rows behind the last sequence hold does not count, and what belongs to them is left as it is (zero_rest: zeroed).

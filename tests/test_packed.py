@@ -1134,3 +1134,31 @@ def test_a_scale_of_any_sign_in_both_types(dtype, scale, ql, kl, d, bias):
         within(t, want[n], n)
     with torch.no_grad():
         within(call(), want["o"], "o without a gradient")
+
+
+def test_scratch_of_the_kernels():
+    """Bytes a lane that spill, read from the built objects.  Attention: none, but for queries with a bias in two waves of 128-wide
+    bf16 heads.  The norm's backward: rows of ten and twelve waves with biases, rows of two blocks a lane (over 6144 values, or over
+    4096 that take single loads)."""
+    import os
+    import re
+    from ait_amd import build
+    from test_abi import _kernel_scratch
+    build.build()
+    for name in ("packed_attn", "packed_attn_bwd"):
+        kernels = _kernel_scratch(os.path.join(build.OBJ, name + ".o"))
+        assert len(kernels) > 20
+        for k, n in kernels.items():
+            assert n <= (32 if "packed_bwd_q_kernelIDF16bLi128ELb1ELi2E" in k else 0), "%s: %d bytes of scratch a lane" % (k, n)
+    kernels = _kernel_scratch(os.path.join(build.OBJ, "gated_norm.o"))
+    seen = 0
+    for k, n in kernels.items():
+        m = re.search(r"gated_norm_(fwd|bwd)_kernelI(.*?)Li(\d+)ELi(\d)ELb(\d)E(?:Lb(\d)E)?", k)
+        if not m:
+            assert n == 0, k
+            continue
+        seen += 1
+        waves, blocks, wide, biases = int(m[3]), int(m[4]), m[5] == "1", m[6] == "1"
+        limit = 0 if m[1] == "fwd" else (204 if wide else 476) if blocks == 2 and biases else (36 if wide else 208) if blocks == 2 else 48 if waves >= 10 and biases else 0
+        assert n <= limit, "%s: %d bytes of scratch a lane (limit %d)" % (k, n, limit)
+    assert seen >= 60
