@@ -10,11 +10,12 @@
 // heads that share its keys.
 //
 // What bounds it.  Long sequences: the matrix unit and the exponentials beside it, at the clock the chip holds under them: 7
-// causal prompts of 33 to 4096 tokens, 16 heads on 4 of 128, bf16: 175 GFLOP in 217 us, 805 TFLOP/s (a large bf16 product
-// reaches 1244 here); the loads alone taken out of it 214, the exponentials alone 219, so neither is in the way.  Matrix unit
-// 42 % busy at 1.7 GHz, no bank conflicts.  (Tried: eight waves a workgroup 247 against 227, two 322 against 231, the next
-// tile's scores under this one's exponentials 255 against 227.)  New tokens: memory: 16 caches of 5000 to 8191, 32 heads on 8 of
-// 128: 432 MB in 82.4 us, 5.2 TB/s, and 4.8 us to join the parts.
+// causal prompts of 33 to 4096 tokens, 16 heads on 4 of 128, bf16: 175 GFLOP in 190 to 196 us a pass, 910 TFLOP/s (a large bf16
+// product reaches 1244 here), 223 to 228 for a launch traced by itself.  Of 227 traced, 25 go without the tiles' loads and 13
+// without the exponentials; the matrix unit is 48 % busy at 1.7 GHz, no bank conflicts (64-wide heads: a third of the LDS
+// cycles, 34 % busy).  (Tried: eight waves a workgroup 247 against 227, two 322 against 231, the next tile's scores under this
+// one's exponentials 255 against 227.)  New tokens: memory: 16 caches of 5000 to 8191, 32 heads on 8 of 128: 432 MB in 85 us,
+// 5.1 TB/s, and 4.7 us to join the parts.
 #include "packed_attn_impl.h"
 
 namespace {

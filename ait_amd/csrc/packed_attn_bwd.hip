@@ -12,10 +12,11 @@
 // accumulators in one, a wave a SIMD is left or registers spill (734 us against 497).
 //
 // What bounds it: the matrix unit, the exponentials between its products and the clock the chip holds under both.  3 documents of
-// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 225 us over the query rows, 390 over the keys and 20 to join their two parts;
-// 4 of 4096 without a mask: 1010 and 980 TFLOP/s executed, no bank conflicts, matrix unit 60 % busy at 1.7 GHz.  12 documents of
-// 100 to 1800, 8 heads of 64: 49 and 63 us (65 over the query rows with operand loads in branches, each waited for by itself).
-// Short sequences (300 of 1 to 49 in f32 with a bias: 61 and 86 us): the trips to memory in front of a workgroup's one tile.
+// 2500 to 4095, 16 heads on 4 of 128, bf16, causal: 228 us over the query rows, 412 over the keys and 17 to join their two parts;
+// 4 of 4096 without a mask: 1036 and 1006 TFLOP/s executed, no bank conflicts, matrix unit 63 and 61 % busy at 1.6 GHz.  12
+// documents of 100 to 1800, 8 heads of 64: 48 and 63 us, matrix unit 32 and 25 % busy, bank conflicts in 40 and 22 % of the LDS
+// cycles (65 us over the query rows with operand loads in branches, each waited for by itself).  Short sequences (300 of 1 to 49
+// in f32 with a bias: 61 and 86 us): the trips to memory in front of a workgroup's one tile.
 // (Tried: eight waves a workgroup 291 against 257 and 589 against 515; masked and unmasked blocks as two loops: spills, 1694 us;
 // bf16 waves that skip the blocks hidden from them, as 64-wide f32 ones do: 62.6 against 60.5; dK's and dV's workgroups in turn
 // instead of dK's first: 459 us against 424.)
