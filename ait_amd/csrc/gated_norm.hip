@@ -12,10 +12,10 @@
 //
 // What bounds it: memory.  58800 rows of 512 in f32, LayerNorm: forward 482 MB in 98 us (4.9 TB/s, a large copy's rate here),
 // backward 722 MB in 149 (4.8).  About 12600 packed rows of 5120, f32 stream and bf16 branch, a gate a sequence: forward 774 MB
-// in 162 to 180 us (4.8 to 4.3), backward 1162 MB in 240 to 250 (4.8 to 4.6).  What it took in the backward, where one workgroup of ten waves fits a CU and
-// its phases meet at barriers: a row's loads without branches around them, so that they are in flight together, sums over the
-// lanes without trips to shared memory, and parameters held (335 us before the three).  Five rows of 4096: 3.8 us, a launch and
-// three dependent trips to memory.
+// in 162 to 180 us (4.8 to 4.3), backward 1162 MB in 240 to 250 (4.8 to 4.6).  What it took in the backward, where one workgroup
+// of ten waves fits a CU and its phases meet at barriers: a row's loads without branches around them, so that they are in flight
+// together, sums over the lanes without trips to shared memory, and parameters held (335 us before the three).  Five rows of
+// 4096: 3.8 us, a launch and three dependent trips to memory.
 #include "common.h"
 
 #include <type_traits>
